@@ -553,6 +553,48 @@ int ontovae_vae_decode_step(const ontovae_vae_ctx_t* ctx, const float* heads, co
 int ontovae_vae_adamw_apply(const ontovae_vae_ctx_t* ctx, const ontovae_adamw_t* opt, void* stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Operators of a dense block on sample-major (channels-last) device matrices: 8-bit products, group norm with an activation,
+ * dropout.  The models' paths that use them: ONTOVAE_FLAG_INT8_ENCODER and ontovae_vae_ext_t below; the Python face is
+ * onto_vae_amd/ops.py.  No counterpart in the reference, whose blocks are torch's Linear / BatchNorm1d / Dropout / ReLU
+ * (onto_vae/modules.py:43-64, 116-133).  Element types: ONTOVAE_F32 / _BF16 / _F16; every sum and statistic is held in 32 bits,
+ * each output is rounded once.  Asynchronous on `stream`, no allocation, safe under graph capture (seed and offset are
+ * recorded by value: a replay draws the same mask).
+ * -------------------------------------------------------------------------------------------*/
+enum { ONTOVAE_F32 = 0, ONTOVAE_BF16 = 1, ONTOVAE_F16 = 2 };
+enum { ONTOVAE_ACT_NONE = 0, ONTOVAE_ACT_RELU = 1, ONTOVAE_ACT_SILU = 2, ONTOVAE_ACT_GELU = 3 };
+
+/* Row m of x (row rows[m] of the n_src rows when rows != NULL), K elements at stride ldx, in 8 bits:
+ *   scale[m] = max_k |x| / 127 (float32),  q[m * ldq + k] = rint(x / scale[m]) (the true quotient, ties to even) in [-127, 127].
+ * Columns [K, ldq) of q are set to 0 (pad ldq to a multiple of 64: ontovae_int8_matmul then takes its aligned path).
+ * A zero row: scale 0.  A row with an infinity or a NaN, or a row index outside [0, n_src): scale NaN, q 0. */
+int ontovae_quantize_rows(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, int32_t M, int32_t K,
+                          int8_t* q, int64_t ldq, float* scale, void* stream);
+/* y[m * ldy + n] = sa[m] sb[n] sum_k a[m * lda + k] b[n * ldb + k] + bias[n] (bias may be NULL), the sum exact (K <= 131071),
+ * the rest in float32, rounded once to `dtype`.  workspace: ontovae_int8_matmul_workspace_bytes, 256-byte aligned (0 bytes: NULL). */
+int64_t ontovae_int8_matmul_workspace_bytes(int32_t M, int32_t N, int32_t K);
+int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb,
+                        const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t dtype, int64_t ldy, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+/* x [N, S, C] contiguous; statistics per sample and group over S rows x C / groups channels.  y = D act(xhat weight + bias);
+ * weight / bias [C] of type wdtype or NULL (1 / 0); mean, rstd [N, groups] float32, what the backward pass takes.
+ * D = dropout of the result with probability drop, keyed as ontovae_dropout keys the rows of [N S, C].
+ * workspace: ontovae_group_norm_act_workspace_bytes(..., backward), 256-byte aligned (0 bytes: NULL).
+ * Backward: dx [N, S, C]; dweight, dbias [C] float32 (either may be NULL), the same drop / seed / offset.  With N S = 0 they are 0. */
+int64_t ontovae_group_norm_act_workspace_bytes(int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, int32_t backward);
+int ontovae_group_norm_act(const void* x, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, const void* weight,
+                           const void* bias, int32_t wdtype, float eps, int32_t act, float drop, uint64_t seed, uint64_t offset, void* y,
+                           float* mean, float* rstd, void* workspace, int64_t workspace_bytes, void* stream);
+int ontovae_group_norm_act_backward(const void* dy, const void* x, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups,
+                                    const void* weight, const void* bias, int32_t wdtype, const float* mean, const float* rstd,
+                                    int32_t act, float drop, uint64_t seed, uint64_t offset, void* dx, float* dweight, float* dbias,
+                                    void* workspace, int64_t workspace_bytes, void* stream);
+/* y[r * C + c] = x[rows ? rows[r] : r][c] / (1 - p) or 0: inverted dropout, the mask drawn from (seed, offset, r, c) by
+ * Philox4x32-10 (16 bits an element: p is taken to the nearest 2^-16) wherever it is needed and never stored; the backward
+ * pass is the same call on dy.  A row index outside [0, n_src) gives a row of NaN. */
+int ontovae_dropout(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, int32_t R, int32_t C, float p,
+                    uint64_t seed, uint64_t offset, void* y, void* stream);
+
+/* ------------------------------------------------------------------------------------------
  * Per-phase timing with HIP events on the launch stream (measurement only; the reference has no
  * counterpart).  ontovae_profile_begin enables the phases in `phase_mask` (bit = phase id) and
  * reserves `capacity` event pairs per phase; every later launch of an enabled phase is bracketed

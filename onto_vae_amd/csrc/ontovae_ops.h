@@ -1,0 +1,38 @@
+// Shared by the dense-block operators (ontovae_ops.hip): element types, 8-element loads, wave and block reductions.
+#ifndef ONTOVAE_OPS_H
+#define ONTOVAE_OPS_H
+
+#include "ontovae_device.h"
+#include "ontovae_internal.h"
+
+#define OV_OPS_LAUNCH_CHECK(what)                                                                                     \
+    do {                                                                                                              \
+        hipError_t e_ = hipGetLastError();                                                                            \
+        if (e_ != hipSuccess) { ontovae_set_error("%s: %s", what, hipGetErrorString(e_)); return ONTOVAE_EHIP; }      \
+    } while (0)
+
+typedef __bf16 ov_bf;
+typedef _Float16 ov_hf;
+
+// one rounding to the element type, to the nearest even
+template <typename T> __device__ __forceinline__ T ov_from_f(float v) { return (T)v; }
+template <typename T> __device__ __forceinline__ float ov_to_f(T v) { return (float)v; }
+
+__device__ __forceinline__ uint32_t ov_wave_max_u(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    return v;
+}
+
+// sum over the workgroup (a multiple of 64 threads, every thread calls); red: 16 floats of LDS
+__device__ __forceinline__ float ov_block_sum(float v, float* red) {
+    v = ov_wave_sum(v);
+    __syncthreads();
+    if (ov_lane() == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    float s = 0.f;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) s += red[w];
+    return s;
+}
+
+#endif

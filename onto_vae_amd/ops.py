@@ -1,0 +1,225 @@
+"""Operators of a dense block on the device: 8-bit linear layers, group norm with an activation, dropout.
+
+Functions on device tensors like onto_vae_amd.stats: the arithmetic is in libontovae_hip.so (ontovae_quantize_rows,
+ontovae_int8_matmul, ontovae_group_norm_act, ontovae_dropout of include/ontovae_hip.h), torch allocates the buffers, there is no CPU
+path.  Forward and backward are explicit calls, no autograd graph is recorded.  Tensors are float32, bfloat16 or float16, channels
+last ([..., C]); every sum and statistic is held in 32 bits and each output is rounded once.  Work is queued on the
+current stream of the tensors' device, which need not be the current device.
+
+The reference has no counterpart: its blocks are torch's Linear, BatchNorm1d, Dropout and ReLU (onto_vae/modules.py:43-64, 116-133).
+The models use these operators through set_precision('int8') and VAE(norm='group', input_drop=...).
+"""
+import ctypes as C
+import math
+
+import torch
+
+from . import _lib
+from .stats import _need_gpu, _ptr, _stream, _workspace
+
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
+I32_MAX = 2 ** 31 - 1
+
+
+def _dtype(t, what):
+    if t.dtype not in DTYPES:
+        raise ValueError(f"{what}: float32, bfloat16 or float16 expected, got {t.dtype}")
+    return DTYPES[t.dtype]
+
+
+def _size(n, what):
+    if n > I32_MAX:
+        raise ValueError(f"{what}: a dimension of {n} exceeds {I32_MAX}")
+    return int(n)
+
+
+def _matrix(x, what):
+    """[..., C] as a 2-D view with unit inner stride (copied only when its strides leave no other way)."""
+    if x.dim() < 1:
+        raise ValueError(f"{what}: at least one dimension expected")
+    m = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    if m.stride(1) != 1 and m.shape[1] > 1 or m.stride(0) < m.shape[1] and m.shape[0] > 1:
+        m = m.contiguous()
+    _size(m.shape[0], what)
+    _size(m.shape[1], what)
+    return m, max(m.stride(0), m.shape[1]) if m.shape[0] > 1 else m.shape[1]
+
+
+def _rows(rows, x, what):
+    if rows is None:
+        return None
+    if rows.dim() != 1 or rows.dtype not in (torch.int32, torch.int64) or rows.device != x.device:
+        raise ValueError(f"{what}: rows must be an int32 or int64 vector on {x.device}")
+    if x.dim() != 2:
+        raise ValueError(f"{what}: rows select from a 2-D matrix")
+    if rows.dtype == torch.int64:          # an index outside int32 stays outside the matrix
+        rows = rows.clamp(-1, I32_MAX)
+    return rows.to(torch.int32).contiguous()
+
+
+def _vector(t, n, device, what, dtypes=(torch.float32,)):
+    if t is None:
+        return None
+    if t.shape != (n,) or t.dtype not in dtypes or t.device != device:
+        raise ValueError(f"{what} must be {' / '.join(str(d).split('.')[-1] for d in dtypes)} [{n}] on {device}")
+    return t.contiguous()
+
+
+def _u64(v, what):
+    v = int(v)
+    if not 0 <= v < 2 ** 64:
+        raise ValueError(f"{what} must be in [0, 2^64)")
+    return v
+
+
+# ---------------------------------------------------------------- 8-bit linear layers
+def quantize_rows(x, rows=None):
+    """(q, scale): the rows of a [..., K] tensor (of the rows x[rows] of a matrix) in 8 bits, scale = max|row| / 127 in float32 and
+    q = x / scale rounded to the nearest integer, ties to even.  q has shape [..., K] and a row stride padded with zeros to a
+    multiple of 64, the layout int8_matmul reads fastest.  A row that holds an infinity or a NaN (or a row index outside x) gets
+    the scale NaN."""
+    _need_gpu(x, "quantize_rows")
+    dt = _dtype(x, "quantize_rows")
+    rows = _rows(rows, x, "quantize_rows")
+    xm, ld = _matrix(x, "quantize_rows")
+    K = xm.shape[1]
+    M = xm.shape[0] if rows is None else rows.shape[0]
+    lead = tuple(x.shape[:-1]) if rows is None else (M,)
+    ldq = max((K + 63) // 64 * 64, 64)
+    with torch.cuda.device(x.device):
+        q = torch.empty(M, ldq, dtype=torch.int8, device=x.device)
+        scale = torch.empty(M, dtype=torch.float32, device=x.device)
+        _lib.check(_lib.lib().ontovae_quantize_rows(_ptr(xm), dt, ld, _ptr(rows), xm.shape[0], M, K, _ptr(q), ldq, _ptr(scale), _stream(x.device)),
+                   "quantize_rows")
+    qk = q[:, :K]
+    return (qk if len(lead) == 1 else qk.view(*lead, K) if M else q.new_empty(*lead, K)), scale.view(lead)
+
+
+def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
+    """y [..., N] = (a [..., K] . b [N, K]^T) a_scale[..., None] b_scale + bias: int8 operands with one float32 scale per row of each
+    (quantize_rows), the sum over K (at most 131071) exact, bias float32 [N], y rounded once to `dtype`."""
+    _need_gpu(a, "int8_matmul")
+    if a.dtype != torch.int8 or b.dtype != torch.int8 or b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1] or a.device != b.device:
+        raise ValueError("int8_matmul: int8 a [..., K] and b [N, K] on one device expected")
+    if dtype not in DTYPES:
+        raise ValueError(f"int8_matmul: dtype must be float32, bfloat16 or float16, got {dtype}")
+    am, lda = _matrix(a, "int8_matmul")
+    bm, ldb = _matrix(b, "int8_matmul")
+    M, K, N = am.shape[0], am.shape[1], bm.shape[0]
+    lead = tuple(a.shape[:-1])
+    if tuple(a_scale.shape) != lead:
+        raise ValueError(f"int8_matmul: a_scale must have shape {lead}, got {tuple(a_scale.shape)}")
+    sa = _vector(a_scale.reshape(-1), M, a.device, "int8_matmul: a_scale")
+    sb = _vector(b_scale, N, a.device, "int8_matmul: b_scale")
+    bias = _vector(bias, N, a.device, "int8_matmul: bias")
+    L = _lib.lib()
+    with torch.cuda.device(a.device):
+        y = torch.empty(*lead, N, dtype=dtype, device=a.device)
+        keep, ws, nbytes = _workspace(L.ontovae_int8_matmul_workspace_bytes(M, N, K), a.device)
+        _lib.check(L.ontovae_int8_matmul(_ptr(am), lda, _ptr(sa), _ptr(bm), ldb, _ptr(sb), _ptr(bias), M, N, K, _ptr(y), DTYPES[dtype], N,
+                                         ws, nbytes, _stream(a.device)), "int8_matmul")
+    return y
+
+
+def int8_linear(x, weight, weight_scale, bias=None, rows=None, dtype=None):
+    """x weight^T + bias with an 8-bit weight [N, K] (quantize_rows of the layer's float weight, done once) and the rows of x (of
+    x[rows]) quantised on the way: one scale per token and per output channel.  dtype: that of y, x's by default."""
+    q, s = quantize_rows(x, rows)
+    return int8_matmul(q, s, weight, weight_scale, bias, x.dtype if dtype is None else dtype)
+
+
+# ---------------------------------------------------------------- group norm with an activation
+def _gn_args(x, groups, weight, bias, act, drop, seed, offset, what):
+    _need_gpu(x, what)
+    dt = _dtype(x, what)
+    if x.dim() < 2:
+        raise ValueError(f"{what}: x must be [N, ..., C], channels last")
+    N, Cn = _size(x.shape[0], what), _size(x.shape[-1], what)
+    S = _size(math.prod(x.shape[1:-1]), what)
+    groups = int(groups)
+    if groups < 1 or Cn % groups or Cn < groups:
+        raise ValueError(f"{what}: {groups} groups do not divide {Cn} channels")
+    if act not in ACTIVATIONS:
+        raise ValueError(f"{what}: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
+    if not 0.0 <= float(drop) <= 1.0:
+        raise ValueError(f"{what}: drop = {drop} outside [0, 1]")
+    both = tuple(dict.fromkeys((torch.float32, x.dtype)))
+    weight, bias = _vector(weight, Cn, x.device, f"{what}: weight", both), _vector(bias, Cn, x.device, f"{what}: bias", both)
+    if weight is not None and bias is not None and weight.dtype != bias.dtype:
+        raise ValueError(f"{what}: weight and bias must share one type")
+    par = weight if weight is not None else bias
+    wdt = torch.float32 if par is None else par.dtype
+    return dt, N, S, Cn, groups, weight, bias, wdt, ACTIVATIONS[act], float(drop), _u64(seed, f"{what}: seed"), _u64(offset, f"{what}: offset")
+
+
+def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", drop=0.0, seed=0, offset=0):
+    """(y, mean, rstd): group norm of x [N, ..., C] over each sample's C / groups neighbouring channels and all inner positions,
+    then weight and bias ([C], float32 or x's type), then the activation ('none', 'relu', 'silu', 'gelu'), then dropout with
+    probability `drop` (masked as `dropout` masks y: same seed and offset, same mask).  mean, rstd: float32 [N, groups], for
+    group_norm_act_backward."""
+    dt, N, S, Cn, groups, weight, bias, wdt, a, drop, seed, offset = _gn_args(x, groups, weight, bias, act, drop, seed, offset, "group_norm_act")
+    if not float(eps) >= 0.0:
+        raise ValueError(f"group_norm_act: eps = {eps}")
+    x = x.contiguous()
+    L = _lib.lib()
+    with torch.cuda.device(x.device):
+        y = torch.empty_like(x)
+        mean = torch.empty(N, groups, dtype=torch.float32, device=x.device)
+        rstd = torch.empty_like(mean)
+        if y.numel() == 0:          # no rows to take statistics of
+            return y, mean.zero_(), rstd.zero_()
+        keep, ws, nbytes = _workspace(L.ontovae_group_norm_act_workspace_bytes(dt, N, S, Cn, groups, 0), x.device)
+        _lib.check(L.ontovae_group_norm_act(_ptr(x), dt, N, S, Cn, groups, _ptr(weight), _ptr(bias), DTYPES[wdt], float(eps), a, drop, seed,
+                                            offset, _ptr(y), _ptr(mean), _ptr(rstd), ws, nbytes, _stream(x.device)), "group_norm_act")
+    return y, mean, rstd
+
+
+def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, act="none", drop=0.0, seed=0, offset=0, eps=None):
+    """(dx, dweight, dbias) of group_norm_act with the mean and rstd it returned and the same further arguments.  dweight and dbias
+    are float32 sums, None where the parameter is None; eps is part of rstd and accepted so that the arguments can be passed on."""
+    dt, N, S, Cn, groups, weight, bias, wdt, a, drop, seed, offset = _gn_args(x, groups, weight, bias, act, drop, seed, offset,
+                                                                              "group_norm_act_backward")
+    if dy.shape != x.shape or dy.dtype != x.dtype or dy.device != x.device:
+        raise ValueError("group_norm_act_backward: dy must match x in shape, type and device")
+    for t, n in ((mean, "mean"), (rstd, "rstd")):
+        if t.shape != (N, groups) or t.dtype != torch.float32 or t.device != x.device:
+            raise ValueError(f"group_norm_act_backward: {n} must be float32 [{N}, {groups}] on {x.device}")
+    dy, x, mean, rstd = dy.contiguous(), x.contiguous(), mean.contiguous(), rstd.contiguous()
+    L = _lib.lib()
+    with torch.cuda.device(x.device):
+        dx = torch.empty_like(x)
+        dw = torch.empty(Cn, dtype=torch.float32, device=x.device) if weight is not None else None
+        db = torch.empty(Cn, dtype=torch.float32, device=x.device) if bias is not None else None
+        if x.numel() == 0:
+            return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None
+        keep, ws, nbytes = _workspace(L.ontovae_group_norm_act_workspace_bytes(dt, N, S, Cn, groups, 1), x.device)
+        _lib.check(L.ontovae_group_norm_act_backward(_ptr(dy), _ptr(x), dt, N, S, Cn, groups, _ptr(weight), _ptr(bias), DTYPES[wdt], _ptr(mean),
+                                                     _ptr(rstd), a, drop, seed, offset, _ptr(dx), _ptr(dw), _ptr(db), ws, nbytes,
+                                                     _stream(x.device)), "group_norm_act_backward")
+    return dx, dw, db
+
+
+# ---------------------------------------------------------------- dropout
+def dropout(x, p, seed, offset=0, rows=None):
+    """Inverted dropout of a [..., C] tensor (of the rows x[rows] of a matrix): each element is 0 with probability p, else divided
+    by 1 - p.  The mask is a function of (seed, offset, row, channel) alone -- Philox4x32-10, 16 bits an element, so p is taken to
+    the nearest 2^-16 -- and is never stored; use another offset for each draw.  A non-finite element in a dropped place gives 0."""
+    _need_gpu(x, "dropout")
+    dt = _dtype(x, "dropout")
+    if not 0.0 <= float(p) <= 1.0:
+        raise ValueError(f"dropout: p = {p} outside [0, 1]")
+    seed, offset = _u64(seed, "dropout: seed"), _u64(offset, "dropout: offset")
+    rows = _rows(rows, x, "dropout")
+    xm, ld = _matrix(x, "dropout")
+    R = xm.shape[0] if rows is None else rows.shape[0]
+    with torch.cuda.device(x.device):
+        y = torch.empty(x.shape if rows is None else (R, xm.shape[1]), dtype=x.dtype, device=x.device)
+        _lib.check(_lib.lib().ontovae_dropout(_ptr(xm), dt, ld, _ptr(rows), xm.shape[0], R, xm.shape[1], float(p), seed, offset, _ptr(y),
+                                              _stream(x.device)), "dropout")
+    return y
+
+
+def dropout_backward(dy, p, seed, offset=0):
+    """The gradient of dropout(x, p, seed, offset) with respect to x (of x[rows] where rows were given): the same mask and factor on dy."""
+    return dropout(dy, p, seed, offset)
