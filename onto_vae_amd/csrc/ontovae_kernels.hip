@@ -454,7 +454,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
     const int l = blockIdx.x, tid = threadIdx.x;
     float* xr = xhat + (int64_t)l * ldb;
     float* ar = a + (int64_t)l * ldb;
-    float mean, var;
+    float mean, var, rest = 0.f;
     if (mode == 1 || mode == 2) {
         const float bias = b0[l];
         float sum = 0.f;
@@ -475,16 +475,20 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
             *reinterpret_cast<f32x4*>(xr + b) = h4;
         }
         mean = ov_wg_sum256(sum, red) / (float)B;
-        float q = 0.f;
+        // the rounding of the mean shifts every xhat of the row alike, and with them a whole row of dW0: what is left of the mean
+        // is summed in the same pass as the squares and taken off
+        float q = 0.f, left = 0.f;
         for (int b = tid * 4; b < ldb; b += 1024) {
             const f32x4 h4 = *reinterpret_cast<const f32x4*>(xr + b);       // this thread's own stores
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const float dlt = h4[j] - mean;
                 q += b + j < B ? dlt * dlt : 0.f;
+                left += b + j < B ? dlt : 0.f;
             }
         }
         q = ov_wg_sum256(q, red);
+        rest = ov_wg_sum256(left, red) / (float)B;
         if (mode == 2) {
             if (tid == 0) { stats[l] = mean; stats[L + l] = q; }
             return;
@@ -531,7 +535,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
         for (int j = 0; j < 4; ++j) {
             float xh = 0.f, y = 0.f;
             if (b + j < B) {
-                xh = (h4[j] - mean) * invstd;
+                xh = ((h4[j] - mean) - rest) * invstd;
                 y = xh * g + be;
                 if (dropping) y *= ov_dropout_scale(drop, seed, rng_off, OV_RNG_DROP, (uint64_t)l * 0x100000000ull + (b + j));
                 y = fmaxf(y, 0.f);
