@@ -2,12 +2,17 @@
 //
 //   s_m = max_k |x_mk| / 127,  q_mk = rint(x_mk / s_m)          (ov_q8_rows_kernel)
 //   y_mn = s_m t_n sum_k q_mk w_nk + b_n                        (ov_q8_gemm_kernel), the sum exact in 32-bit integers
+//
+// Integer sums are exact in any order, so the K axis may be cut into slabs (ov_q8_combine_kernel) without a rounding.
 #ifndef ONTOVAE_INT8_H
 #define ONTOVAE_INT8_H
 
 #include "ontovae_ops.h"
 
 #define OV_Q8_MAX_K 131071          // 128 * 128 * K < 2^31
+
+typedef int ov_i32x4 __attribute__((ext_vector_type(4)));
+typedef int ov_i32x16 __attribute__((ext_vector_type(16)));
 
 // A row's scale from the bits of its largest magnitude: NaN if the row holds an infinity or a NaN.
 __device__ __forceinline__ float ov_q8_scale(uint32_t amax_bits) {
@@ -37,47 +42,283 @@ struct OvQ8 {
     }
 };
 
-template <typename T>
-__global__ __launch_bounds__(256) void ov_q8_rows_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ rows, int n_src,
-                                                         int K, int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
-    __shared__ uint32_t red[4];
-    const int64_t m = blockIdx.x;
+__device__ __forceinline__ uint32_t ov_abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
+
+// One row per group of THREADS threads (a wave: 4 rows per workgroup; else one), the row held in registers between the search
+// for its maximum and the rounding, 16 B per lane and load: x is read once.  Bound by that read (and the write of a quarter
+// or half of it).  Rows of more than THREADS * NV pieces re-read the rest, from the cache.  Rows may start at any element:
+// the loads are not assumed aligned.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS < 256 ? 256 : THREADS) void ov_q8_rows_kernel(const T* __restrict__ x, int64_t ldx,
+                                                                                    const int32_t* __restrict__ rows, int n_src, int M, int K,
+                                                                                    int8_t* __restrict__ q, int64_t ldq, float* __restrict__ scale) {
+    constexpr int VE = 16 / sizeof(T);
+    __shared__ uint32_t red[16];
+    const int tid = THREADS < 256 ? ov_lane() : (int)threadIdx.x;
+    const int64_t m = THREADS < 256 ? (int64_t)blockIdx.x * 4 + ov_wave_id() : (int64_t)blockIdx.x;
+    if (THREADS < 256 && m >= M) return;
     int64_t src = m;
     bool ok = true;
     if (rows) { src = rows[m]; ok = src >= 0 && src < n_src; }
     const T* xr = x + (ok ? src : 0) * ldx;
+    const int nfull = ok ? K / VE : 0, kt = nfull * VE;      // whole 16-B pieces; the rest of the row goes element by element
+    OvVec<T> v[NV];
     uint32_t a = ok ? 0u : 0x7fffffffu;
-    if (ok)
-        for (int k = threadIdx.x; k < K; k += 256) a = max(a, __builtin_bit_cast(uint32_t, ov_to_f<T>(xr[k])) & 0x7fffffffu);
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int p = tid + i * THREADS;
+        if (p < nfull) v[i].load(xr + (int64_t)p * VE);
+        else v[i].zero();
+    }
+    T t = (T)0.f;
+    if (ok && kt + tid < K) t = xr[kt + tid];                // fewer than VE elements
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+#pragma unroll
+        for (int j = 0; j < VE; ++j) a = max(a, ov_abs_bits(ov_to_f<T>(v[i].e[j])));
+    a = max(a, ov_abs_bits(ov_to_f<T>(t)));
+    for (int p = tid + NV * THREADS; p < nfull; p += THREADS) {
+        OvVec<T> w;
+        w.load(xr + (int64_t)p * VE);
+#pragma unroll
+        for (int j = 0; j < VE; ++j) a = max(a, ov_abs_bits(ov_to_f<T>(w.e[j])));
+    }
     a = ov_wave_max_u(a);
-    if (ov_lane() == 0) red[threadIdx.x >> 6] = a;
-    __syncthreads();
-    const float s = ov_q8_scale(max(max(red[0], red[1]), max(red[2], red[3])));
+    if (THREADS >= 256) {
+        if (ov_lane() == 0) red[threadIdx.x >> 6] = a;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; ++w) a = max(a, red[w]);
+    }
+    const float s = ov_q8_scale(a);
     const OvQ8 f(s);
-    for (int64_t k = threadIdx.x; k < ldq; k += 256) q[m * ldq + k] = k < K && ok ? (int8_t)f(ov_to_f<T>(xr[k])) : (int8_t)0;
-    if (threadIdx.x == 0) scale[m] = s;
+    int8_t* qr = q + m * ldq;
+    const bool qal = ((reinterpret_cast<uintptr_t>(q) | (uintptr_t)ldq) & 7) == 0;
+    auto put = [&](int p, const OvVec<T>& w) {
+        int8_t o[VE];
+#pragma unroll
+        for (int j = 0; j < VE; ++j) o[j] = (int8_t)f(ov_to_f<T>(w.e[j]));
+        if (qal) {
+            if (VE == 8) *reinterpret_cast<uint64_t*>(qr + (int64_t)p * VE) = __builtin_bit_cast(uint64_t, *reinterpret_cast<const OvBytes<8>*>(o));
+            else *reinterpret_cast<uint32_t*>(qr + (int64_t)p * VE) = __builtin_bit_cast(uint32_t, *reinterpret_cast<const OvBytes<4>*>(o));
+        } else {
+#pragma unroll
+            for (int j = 0; j < VE; ++j) qr[(int64_t)p * VE + j] = o[j];
+        }
+    };
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int p = tid + i * THREADS;
+        if (p < nfull) put(p, v[i]);
+    }
+    for (int p = tid + NV * THREADS; p < nfull; p += THREADS) {
+        OvVec<T> w;
+        w.load(xr + (int64_t)p * VE);
+        put(p, w);
+    }
+    for (int64_t k = kt + tid; k < ldq; k += THREADS) qr[k] = k < K && ok ? (int8_t)f(ov_to_f<T>(t)) : (int8_t)0;
+    if (tid == 0) scale[m] = s;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void ov_q8_gemm_kernel(const int8_t* __restrict__ A, int64_t lda, const float* __restrict__ sa,
-                                                         const int8_t* __restrict__ B, int64_t ldb, const float* __restrict__ sb,
-                                                         const float* __restrict__ bias, int M, int N, int K, T* __restrict__ y, int64_t ldy) {
-    __shared__ int8_t As[16][68], Bs[16][68];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const int64_t m0 = (int64_t)blockIdx.y * 16, n0 = (int64_t)blockIdx.x * 16;
-    int acc = 0;
-    for (int k0 = 0; k0 < K; k0 += 64) {
-        for (int e = threadIdx.x; e < 1024; e += 256) {
-            const int r = e >> 6, k = e & 63;
-            As[r][k] = m0 + r < M && k0 + k < K ? A[(m0 + r) * lda + k0 + k] : (int8_t)0;
-            Bs[r][k] = n0 + r < N && k0 + k < K ? B[(n0 + r) * ldb + k0 + k] : (int8_t)0;
-        }
-        __syncthreads();
-        for (int k = 0; k < 64; ++k) acc += (int)As[ty][k] * (int)Bs[tx][k];
-        __syncthreads();
+struct OvQ8Gemm {
+    const int8_t* A; int64_t lda;        // [M, K]
+    const int8_t* B; int64_t ldb;        // [N, K]
+    const float* sa; const float* sb; const float* bias;
+    int M, N, K, kchunk;                 // kchunk % 128 == 0: K range of a slab
+    int nm, nn;                          // tiles
+    int32_t* slab;                       // split: [splits][M][N]
+    void* y; int64_t ldy;
+};
+
+// Tile BM x BN of the product, waves of WM x WN on v_mfma_i32_32x32x32_i8, K in steps of 128 bytes through a ring of ST LDS
+// stages, one barrier a step.  DIRECT: the pieces go from memory to LDS without passing registers, and the wait before the
+// barrier leaves the ST - 2 youngest stages in flight.  A row of a stage is 128 B = 8 pieces of 16 B, stored with the piece
+// index xor-ed with the row's low bits (the source address is permuted, LDS is written in lane order): a wave's 16-B fragment
+// reads then spread over all banks.  Rows beyond M / N repeat the last one, their results are dropped.  The last, partial step
+// of K is loaded with its bytes masked, so nothing is assumed of what stands behind column K.
+// !DIRECT: operands whose rows do not start on 16 B; the same loads through registers, unaligned.
+// T = int32_t: the raw sums to slab blockIdx.y.
+template <int BM, int BN, int WM, int WN, int ST, bool DIRECT, typename T>
+__global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ov_q8_gemm_kernel(const OvQ8Gemm g) {
+    constexpr int THREADS = (BM / WM) * (BN / WN) * 64, ROWS = BM + BN, STAGE = ROWS * 128, NL = ROWS * 8 / THREADS;
+    constexpr int FM = WM / 32, FN = WN / 32;
+    static_assert(ROWS * 8 % THREADS == 0 && BM * 8 % THREADS == 0, "whole loads per thread");
+    extern __shared__ __attribute__((aligned(16))) int8_t ov_q8_lds[];
+    // workgroups are dealt to the 8 XCDs round-robin: XCD x takes a contiguous run of tiles, in which the tiles of up to 8
+    // neighbouring row panels share their B panels (and the column panels their A) in that XCD's L2
+    int tm, tn;
+    {
+        const int nt = g.nm * g.nn;
+        int id = blockIdx.x;
+        const int per = nt >> 3, rem = nt & 7, x = id & 7, j = id >> 3;
+        id = x * per + min(x, rem) + j;
+        const int gs = 8 * g.nn, gid = id / gs, first = gid * 8, rows = min(g.nm - first, 8), r = id - gid * gs;
+        tm = first + r % rows;
+        tn = r / rows;
     }
-    const int64_t m = m0 + ty, n = n0 + tx;
-    if (m < M && n < N) y[m * ldy + n] = ov_from_f<T>((float)acc * sa[m] * sb[n] + (bias ? bias[n] : 0.f));
+    const int m0 = tm * BM, n0 = tn * BN;
+    const int kbeg = blockIdx.y * g.kchunk, kend = min(g.K, kbeg + g.kchunk);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / (BN / WN) * WM, wn = wave % (BN / WN) * WN;
+    const int8_t* Ab = g.A + (int64_t)m0 * g.lda + kbeg;
+    const int8_t* Bb = g.B + (int64_t)n0 * g.ldb + kbeg;
+    const int len = max(kend - kbeg, 0), full = len >> 7;
+
+    ov_i32x16 acc[FM][FN];
+#pragma unroll
+    for (int i = 0; i < FM; ++i)
+#pragma unroll
+        for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[i][j][e] = 0;
+
+    // piece i of this thread: row (tid + i THREADS) / 8 of the stage (A rows, then B rows), LDS piece tid % 8
+    const int piece = (tid & 7) ^ ((tid >> 3) & 7);                       // THREADS / 8 is a multiple of 8: the same for every i
+    auto row_of = [&](int i) { return (tid >> 3) + i * (THREADS / 8); };
+    uint32_t off[NL];
+#pragma unroll
+    for (int i = 0; i < NL; ++i) {
+        const int r = row_of(i);
+        off[i] = (i < BM * 8 / THREADS ? (uint32_t)min(r, g.M - 1 - m0) * (uint32_t)g.lda : (uint32_t)min(r - BM, g.N - 1 - n0) * (uint32_t)g.ldb) +
+                 (uint32_t)piece * 16u;
+    }
+    auto dma = [&](int step, int stage) {
+        int8_t* dst = ov_q8_lds + stage * STAGE + wave * 1024;
+#pragma unroll
+        for (int i = 0; i < NL; ++i) {
+            const int8_t* src = (i < BM * 8 / THREADS ? Ab : Bb) + (int64_t)step * 128 + off[i];
+            __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)src,
+                                             (__attribute__((address_space(3))) void*)(dst + i * (THREADS * 16)), 16, 0, 0);
+        }
+    };
+    auto compute = [&](int stage) {
+        const int8_t* sA = ov_q8_lds + stage * STAGE + (wm + (lane & 31)) * 128;
+        const int8_t* sB = ov_q8_lds + stage * STAGE + (BM + wn + (lane & 31)) * 128;
+        const int sw = lane & 7;                                          // the fragment rows differ by multiples of 32
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) {
+            const int p = ((kk * 2 + (lane >> 5)) ^ sw) * 16;
+            ov_i32x4 a[FM], b[FN];
+#pragma unroll
+            for (int i = 0; i < FM; ++i) a[i] = *reinterpret_cast<const ov_i32x4*>(sA + i * 32 * 128 + p);
+#pragma unroll
+            for (int j = 0; j < FN; ++j) b[j] = *reinterpret_cast<const ov_i32x4*>(sB + j * 32 * 128 + p);
+#pragma unroll
+            for (int i = 0; i < FM; ++i)
+#pragma unroll
+                for (int j = 0; j < FN; ++j) acc[i][j] = __builtin_amdgcn_mfma_i32_32x32x32_i8(a[i], b[j], acc[i][j], 0, 0, 0);
+        }
+    };
+    // a 16-B piece of a row through registers: bytes from kend on are 0 and not read
+    auto masked = [&](int i, int k0) {
+        const int r = row_of(i);
+        const int8_t* base = i < BM * 8 / THREADS ? Ab + (int64_t)min(r, g.M - 1 - m0) * g.lda : Bb + (int64_t)min(r - BM, g.N - 1 - n0) * g.ldb;
+        const int k = k0 + piece * 16, n = len - k;
+        OvBytes<16> v = {};
+        if (n >= 16) __builtin_memcpy(&v, base + k, 16);
+        else
+#pragma unroll
+            for (int j = 0; j < 15; ++j)
+                if (j < n) v.b[j] = base[k + j];
+        return __builtin_bit_cast(ov_i32x4, v);
+    };
+    auto put = [&](int stage, int i, ov_i32x4 v) {
+        *reinterpret_cast<ov_i32x4*>(ov_q8_lds + stage * STAGE + tid * 16 + i * (THREADS * 16)) = v;
+    };
+
+    if (DIRECT) {
+#pragma unroll
+        for (int s = 0; s < ST - 1; ++s)
+            if (s < full) dma(s, s);
+        int cur = 0;
+        for (int s = 0; s < full; ++s) {
+            // the stage of this step has landed when at most the younger stages' loads are outstanding
+            if (s + ST - 2 < full) ov_wait_vm<NL * (ST - 2)>();
+            else ov_wait_vm<0>();
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            int nx = cur + ST - 1;
+            nx -= nx >= ST ? ST : 0;
+            if (s + ST - 1 < full) dma(s + ST - 1, nx);                   // read by nobody since the barrier above
+            compute(cur);
+            cur = cur + 1 == ST ? 0 : cur + 1;
+        }
+        if (len & 127) {
+            __syncthreads();                                              // every stage is free
+#pragma unroll
+            for (int i = 0; i < NL; ++i) put(0, i, masked(i, full * 128));
+            __syncthreads();
+            compute(0);
+        }
+    } else {
+        const int steps = (len + 127) >> 7;
+        ov_i32x4 v[NL];
+        if (steps > 0) {
+#pragma unroll
+            for (int i = 0; i < NL; ++i) v[i] = masked(i, 0);
+        }
+        for (int s = 0; s < steps; ++s) {
+            const int st = s & 1;
+#pragma unroll
+            for (int i = 0; i < NL; ++i) put(st, i, v[i]);
+            __syncthreads();
+            if (s + 1 < steps) {
+#pragma unroll
+                for (int i = 0; i < NL; ++i) v[i] = masked(i, (s + 1) * 128);
+            }
+            compute(st);
+        }
+    }
+
+    // C/D map of a 32 x 32 tile: column = lane & 31, row = (e & 3) + 8 (e >> 2) + 4 (lane >> 5)
+#pragma unroll
+    for (int j = 0; j < FN; ++j) {
+        const int n = n0 + wn + 32 * j + (lane & 31);
+        if (n >= g.N) continue;
+        float tb = 0.f, bi = 0.f;
+        if (!__is_same(T, int32_t)) { tb = g.sb[n]; bi = g.bias ? g.bias[n] : 0.f; }
+#pragma unroll
+        for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const int m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
+                if (m >= g.M) continue;
+                if constexpr (__is_same(T, int32_t)) g.slab[((int64_t)blockIdx.y * g.M + m) * g.N + n] = acc[i][j][e];
+                else static_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = ov_from_f<T>((float)acc[i][j][e] * g.sa[m] * tb + bi);
+            }
+    }
+}
+
+// sum of the slabs, scales, bias: one element per thread and trip
+template <typename T>
+__global__ __launch_bounds__(256) void ov_q8_combine_kernel(const OvQ8Gemm g, int splits) {
+    const int64_t total = (int64_t)g.M * g.N;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
+        const int m = (int)(i / g.N), n = (int)(i - (int64_t)m * g.N);
+        int a = 0;
+#pragma unroll 8
+        for (int z = 0; z < splits; ++z) a += g.slab[z * total + i];
+        static_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = ov_from_f<T>((float)a * g.sa[m] * g.sb[n] + (g.bias ? g.bias[n] : 0.f));
+    }
+}
+
+// ---------------------------------------------------------------- host
+template <typename T>
+static void ov_q8_rows_launch(const void* x, int64_t ldx, const int32_t* rows, int n_src, int M, int K, int8_t* q, int64_t ldq, float* scale,
+                              hipStream_t st) {
+    constexpr int VE = 16 / sizeof(T);
+    const int p = (K + VE - 1) / VE;
+    const T* xt = static_cast<const T*>(x);
+#define OV_Q8_ROWS(TH, NV) \
+    hipLaunchKernelGGL((ov_q8_rows_kernel<T, TH, NV>), dim3(TH < 256 ? (M + 3) / 4 : M), dim3(TH < 256 ? 256 : TH), 0, st, xt, ldx, rows, n_src, M, K, q, \
+                       ldq, scale)
+    if (p <= 64) OV_Q8_ROWS(64, 1);
+    else if (p <= 256) OV_Q8_ROWS(64, 4);
+    else if (p <= 1024) OV_Q8_ROWS(256, 4);
+    else if (p <= 2048) OV_Q8_ROWS(512, 4);
+    else if (p <= 5120) OV_Q8_ROWS(512, 10);
+    else OV_Q8_ROWS(1024, 16);
+#undef OV_Q8_ROWS
 }
 
 extern "C" int ontovae_quantize_rows(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, int32_t M, int32_t K,
@@ -91,17 +332,73 @@ extern "C" int ontovae_quantize_rows(const void* x, int32_t dtype, int64_t ldx, 
     if (!scale || (K > 0 && (!x || !q))) { ontovae_set_error("quantize_rows: NULL argument"); return ONTOVAE_EINVAL; }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (dtype) {
-        case ONTOVAE_F32: hipLaunchKernelGGL(ov_q8_rows_kernel<float>, dim3(M), dim3(256), 0, st, (const float*)x, ldx, rows, n_src, K, q, ldq, scale); break;
-        case ONTOVAE_BF16: hipLaunchKernelGGL(ov_q8_rows_kernel<ov_bf>, dim3(M), dim3(256), 0, st, (const ov_bf*)x, ldx, rows, n_src, K, q, ldq, scale); break;
-        default: hipLaunchKernelGGL(ov_q8_rows_kernel<ov_hf>, dim3(M), dim3(256), 0, st, (const ov_hf*)x, ldx, rows, n_src, K, q, ldq, scale); break;
+        case ONTOVAE_F32: ov_q8_rows_launch<float>(x, ldx, rows, n_src, M, K, q, ldq, scale, st); break;
+        case ONTOVAE_BF16: ov_q8_rows_launch<ov_bf>(x, ldx, rows, n_src, M, K, q, ldq, scale, st); break;
+        default: ov_q8_rows_launch<ov_hf>(x, ldx, rows, n_src, M, K, q, ldq, scale, st); break;
     }
     OV_OPS_LAUNCH_CHECK("quantize_rows");
     return ONTOVAE_OK;
 }
 
+// Tile and split of a product.
+struct OvQ8Plan { int cfg, splits, kchunk; };
+enum { OV_Q8_T32 = 0, OV_Q8_T64 = 1, OV_Q8_T128 = 2, OV_Q8_T192 = 3, OV_Q8_T256 = 4 };
+static const int ov_q8_bm[5] = {32, 64, 128, 128, 256}, ov_q8_bn[5] = {128, 64, 128, 192, 256};
+
+static OvQ8Plan ov_q8_plan(int M, int N, int K) {
+    OvQ8Plan p;
+    auto tiles = [&](int c) { return (int64_t)((M + ov_q8_bm[c] - 1) / ov_q8_bm[c]) * ((N + ov_q8_bn[c] - 1) / ov_q8_bn[c]); };
+    p.cfg = M <= 32 ? OV_Q8_T32 : OV_Q8_T64;
+    for (int c = OV_Q8_T128; c <= OV_Q8_T256; ++c)
+        if (tiles(c) >= 256) p.cfg = c;
+    const int steps = std::max((K + 127) / 128, 1);
+    const int64_t t = tiles(p.cfg);
+    int s = 1;
+    if (t < 256) s = (int)std::min<int64_t>((256 + t - 1) / t, std::max(steps / 4, 1));
+    const int per = (steps + s - 1) / s;
+    p.kchunk = per * 128;
+    p.splits = (steps + per - 1) / per;
+    return p;
+}
+
+template <int BM, int BN, int WM, int WN, int ST, bool DIRECT, typename T>
+static int ov_q8_gemm_go(const OvQ8Gemm& g, int splits, hipStream_t st) {
+    constexpr int THREADS = (BM / WM) * (BN / WN) * 64, LDS = (DIRECT ? ST : 2) * (BM + BN) * 128;
+    auto* fn = ov_q8_gemm_kernel<BM, BN, WM, WN, ST, DIRECT, T>;
+    static std::atomic<uint64_t> raised{0};                               // bit = device: the limit is raised once
+    int dev = 0;
+    if (LDS > 65536 && (hipGetDevice(&dev) != hipSuccess || dev > 63 || !(raised.load() >> dev & 1))) {
+        hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+        if (e != hipSuccess) { ontovae_set_error("int8_matmul: %d bytes of LDS: %s", LDS, hipGetErrorString(e)); return ONTOVAE_EHIP; }
+        if (dev >= 0 && dev < 64) raised |= 1ull << dev;
+    }
+    hipLaunchKernelGGL(fn, dim3(g.nm * g.nn, splits), dim3(THREADS), LDS, st, g);
+    return ONTOVAE_OK;
+}
+
+template <typename T>
+static int ov_q8_gemm_launch(OvQ8Gemm g, const OvQ8Plan& p, bool direct, hipStream_t st) {
+    g.nm = (g.M + ov_q8_bm[p.cfg] - 1) / ov_q8_bm[p.cfg];
+    g.nn = (g.N + ov_q8_bn[p.cfg] - 1) / ov_q8_bn[p.cfg];
+    g.kchunk = p.kchunk;
+    if (!direct) {
+        g.nm = (g.M + 63) / 64;
+        g.nn = (g.N + 63) / 64;
+        return ov_q8_gemm_go<64, 64, 32, 32, 2, false, T>(g, p.splits, st);
+    }
+    switch (p.cfg) {
+        case OV_Q8_T32: return ov_q8_gemm_go<32, 128, 32, 32, 4, true, T>(g, p.splits, st);
+        case OV_Q8_T64: return ov_q8_gemm_go<64, 64, 32, 32, 4, true, T>(g, p.splits, st);
+        case OV_Q8_T128: return ov_q8_gemm_go<128, 128, 64, 64, 2, true, T>(g, p.splits, st);
+        case OV_Q8_T192: return ov_q8_gemm_go<128, 192, 64, 96, 3, true, T>(g, p.splits, st);
+        default: return ov_q8_gemm_go<256, 256, 128, 64, 2, true, T>(g, p.splits, st);
+    }
+}
+
 extern "C" int64_t ontovae_int8_matmul_workspace_bytes(int32_t M, int32_t N, int32_t K) {
-    (void)M; (void)N; (void)K;
-    return 0;
+    if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K) return 0;
+    const OvQ8Plan p = ov_q8_plan(M, N, K);
+    return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
 }
 
 extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb,
@@ -116,17 +413,34 @@ extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa
     if (dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) { ontovae_set_error("int8_matmul: unknown element type %d", dtype); return ONTOVAE_EINVAL; }
     if (M == 0 || N == 0) return ONTOVAE_OK;
     if (!sa || !sb || !y || (K > 0 && (!a || !b))) { ontovae_set_error("int8_matmul: NULL argument"); return ONTOVAE_EINVAL; }
-    if (workspace_bytes < ontovae_int8_matmul_workspace_bytes(M, N, K)) {
-        ontovae_set_error("int8_matmul: workspace of %lld bytes needed", (long long)ontovae_int8_matmul_workspace_bytes(M, N, K));
+    const int64_t need = ontovae_int8_matmul_workspace_bytes(M, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) {
+        ontovae_set_error("int8_matmul: workspace of %lld bytes, 256-B aligned, needed", (long long)need);
         return ONTOVAE_EINVAL;
     }
-    (void)workspace;
+    if (((int64_t)M + 31) / 32 * (((int64_t)N + 63) / 64) > INT32_MAX) { ontovae_set_error("int8_matmul: M = %d, N = %d: too many tiles", M, N); return ONTOVAE_EINVAL; }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((N + 15) / 16, (M + 15) / 16);
-    switch (dtype) {
-        case ONTOVAE_F32: hipLaunchKernelGGL(ov_q8_gemm_kernel<float>, grid, dim3(256), 0, st, a, lda, sa, b, ldb, sb, bias, M, N, K, (float*)y, ldy); break;
-        case ONTOVAE_BF16: hipLaunchKernelGGL(ov_q8_gemm_kernel<ov_bf>, grid, dim3(256), 0, st, a, lda, sa, b, ldb, sb, bias, M, N, K, (ov_bf*)y, ldy); break;
-        default: hipLaunchKernelGGL(ov_q8_gemm_kernel<ov_hf>, grid, dim3(256), 0, st, a, lda, sa, b, ldb, sb, bias, M, N, K, (ov_hf*)y, ldy); break;
+    const OvQ8Plan p = ov_q8_plan(M, N, K);
+    // 16-B pieces at 32-bit offsets inside a tile's rows
+    const bool direct = ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (uintptr_t)lda | (uintptr_t)ldb) & 15) == 0 &&
+                        std::max(lda, ldb) < (1 << 23);
+    OvQ8Gemm g{a, lda, b, ldb, sa, sb, bias, M, N, K, 0, 0, 0, static_cast<int32_t*>(workspace), y, ldy};
+    int rc;
+    if (p.splits > 1) {
+        if ((rc = ov_q8_gemm_launch<int32_t>(g, p, direct, st))) return rc;
+        const dim3 grid((unsigned)std::min<int64_t>(((int64_t)M * N + 255) / 256, 4096));
+        switch (dtype) {
+            case ONTOVAE_F32: hipLaunchKernelGGL(ov_q8_combine_kernel<float>, grid, dim3(256), 0, st, g, p.splits); break;
+            case ONTOVAE_BF16: hipLaunchKernelGGL(ov_q8_combine_kernel<ov_bf>, grid, dim3(256), 0, st, g, p.splits); break;
+            default: hipLaunchKernelGGL(ov_q8_combine_kernel<ov_hf>, grid, dim3(256), 0, st, g, p.splits); break;
+        }
+    } else {
+        switch (dtype) {
+            case ONTOVAE_F32: rc = ov_q8_gemm_launch<float>(g, p, direct, st); break;
+            case ONTOVAE_BF16: rc = ov_q8_gemm_launch<ov_bf>(g, p, direct, st); break;
+            default: rc = ov_q8_gemm_launch<ov_hf>(g, p, direct, st); break;
+        }
+        if (rc) return rc;
     }
     OV_OPS_LAUNCH_CHECK("int8_matmul");
     return ONTOVAE_OK;

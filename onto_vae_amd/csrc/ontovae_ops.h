@@ -18,6 +18,28 @@ typedef _Float16 ov_hf;
 template <typename T> __device__ __forceinline__ T ov_from_f(float v) { return (T)v; }
 template <typename T> __device__ __forceinline__ float ov_to_f(T v) { return (float)v; }
 
+template <int N> struct OvBytes { int8_t b[N]; };
+
+// 16 bytes of elements, loaded and stored at any element's address (unaligned 16-B accesses are one instruction here)
+template <typename T>
+struct OvVec {
+    static constexpr int N = 16 / sizeof(T);
+    T e[N];
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(e, p, 16); }
+    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, e, 16); }
+    __device__ __forceinline__ void zero() {
+#pragma unroll
+        for (int j = 0; j < N; ++j) e[j] = (T)0.f;
+    }
+};
+
+// waits until at most N vector-memory operations of the wave are outstanding
+template <int N>
+__device__ __forceinline__ void ov_wait_vm() {
+    static_assert(N < 64, "the counter holds 63");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 __device__ __forceinline__ uint32_t ov_wave_max_u(uint32_t v) {
 #pragma unroll
     for (int o = 32; o > 0; o >>= 1) v = max(v, (uint32_t)__shfl_xor((int)v, o, 64));

@@ -43,7 +43,7 @@ def _matrix(x, what):
         m = m.contiguous()
     _size(m.shape[0], what)
     _size(m.shape[1], what)
-    return m, max(m.stride(0), m.shape[1]) if m.shape[0] > 1 else m.shape[1]
+    return m, max(m.stride(0), m.shape[1])
 
 
 def _rows(rows, x, what):
