@@ -575,6 +575,13 @@ int64_t ontovae_int8_matmul_workspace_bytes(int32_t M, int32_t N, int32_t K);
 int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb,
                         const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t dtype, int64_t ldy, void* workspace,
                         int64_t workspace_bytes, void* stream);
+/* y = x W^T + bias with W in 8 bits (w, sw: ontovae_quantize_rows of the float weight) and the rows of x (x[rows]) quantised on
+ * the way: ontovae_quantize_rows and ontovae_int8_matmul in one call; up to 4 rows in one launch.
+ * workspace: ontovae_int8_linear_workspace_bytes, 256-byte aligned (0 bytes: NULL). */
+int64_t ontovae_int8_linear_workspace_bytes(int32_t M, int32_t N, int32_t K);
+int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, const int8_t* w, int64_t ldw,
+                        const float* sw, const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t ydtype, int64_t ldy,
+                        void* workspace, int64_t workspace_bytes, void* stream);
 /* x [N, S, C] contiguous; statistics per sample and group over S rows x C / groups channels.  y = D act(xhat weight + bias);
  * weight / bias [C] of type wdtype or NULL (1 / 0); mean, rstd [N, groups] float32, what the backward pass takes.
  * D = dropout of the result with probability drop, keyed as ontovae_dropout keys the rows of [N S, C].

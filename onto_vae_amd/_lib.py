@@ -152,6 +152,7 @@ def lib():
         "ontovae_decoder_forward_train": [C.POINTER(Ctx), vp, i32, u64, vp, i64, vp],
         "ontovae_quantize_rows": [vp, i32, i64, vp, i32, i32, i32, vp, i64, vp, vp],
         "ontovae_int8_matmul": [vp, i64, vp, vp, i64, vp, vp, i32, i32, i32, vp, i32, i64, vp, i64, vp],
+        "ontovae_int8_linear": [vp, i32, i64, vp, i32, vp, i64, vp, vp, i32, i32, i32, vp, i32, i64, vp, i64, vp],
         "ontovae_group_norm_act": [vp, i32, i32, i32, i32, i32, vp, vp, i32, f32, i32, f32, u64, u64, vp, vp, vp, vp, i64, vp],
         "ontovae_group_norm_act_backward": [vp, vp, i32, i32, i32, i32, i32, vp, vp, i32, vp, vp, i32, f32, u64, u64, vp, vp, vp, vp, i64, vp],
         "ontovae_dropout": [vp, i32, i64, vp, i32, i32, i32, f32, u64, u64, vp, vp],
@@ -176,8 +177,9 @@ def lib():
     for name in ("ontovae_wilcoxon_workspace_bytes", "ontovae_fdr_workspace_bytes"):
         getattr(L, name).argtypes = [i32, i32]
         getattr(L, name).restype = C.c_int64
-    L.ontovae_int8_matmul_workspace_bytes.argtypes = [i32, i32, i32]
-    L.ontovae_int8_matmul_workspace_bytes.restype = C.c_int64
+    for name in ("ontovae_int8_matmul_workspace_bytes", "ontovae_int8_linear_workspace_bytes"):
+        getattr(L, name).argtypes = [i32, i32, i32]
+        getattr(L, name).restype = C.c_int64
     L.ontovae_group_norm_act_workspace_bytes.argtypes = [i32] * 6
     L.ontovae_group_norm_act_workspace_bytes.restype = C.c_int64
     _lib = L
@@ -195,7 +197,8 @@ EXPORTED = ["ontovae_last_error", "ontovae_abi_version", "ontovae_plan_create", 
             "ontovae_to_feature_major",
             "ontovae_vae_layout", "ontovae_vae_workspace_bytes", "ontovae_vae_train_step", "ontovae_vae_forward", "ontovae_vae_adamw_apply",
             "ontovae_vae_decode_forward", "ontovae_vae_decode_step", "ontovae_decoder_backward", "ontovae_decoder_forward_train",
-            "ontovae_quantize_rows", "ontovae_int8_matmul_workspace_bytes", "ontovae_int8_matmul", "ontovae_group_norm_act_workspace_bytes",
+            "ontovae_quantize_rows", "ontovae_int8_matmul_workspace_bytes", "ontovae_int8_matmul", "ontovae_int8_linear_workspace_bytes",
+            "ontovae_int8_linear", "ontovae_group_norm_act_workspace_bytes",
             "ontovae_group_norm_act", "ontovae_group_norm_act_backward", "ontovae_dropout",
             "ontovae_profile_begin", "ontovae_profile_read", "ontovae_profile_end", "ontovae_profile_overhead"]
 

@@ -28,36 +28,99 @@ static inline int ov_drop_from(float p, uint64_t seed, uint64_t offset, OvDrop* 
     return 0;
 }
 
-// bit j: element j of the block is kept
-__device__ __forceinline__ uint32_t ov_drop_bits(const OvDrop& d, uint64_t block) {
-    const OvPhilox r = ov_philox(d.seed, d.offset, OV_RNG_OP, block);
-    uint32_t m = 0;
+// The block's draws.  ov_philox with the two 32 x 32-bit products of a round as one 64-bit multiply each.
+__device__ __forceinline__ OvPhilox ov_drop_draw(const OvDrop& d, uint64_t block) {
+    uint32_t k0 = (uint32_t)d.seed, k1 = (uint32_t)(d.seed >> 32);
+    uint32_t c0 = (uint32_t)block, c1 = (uint32_t)(block >> 32) ^ (OV_RNG_OP << 24), c2 = (uint32_t)d.offset, c3 = (uint32_t)(d.offset >> 32);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        m |= ((r.c[w] & 0xFFFFu) >= d.t ? 1u : 0u) << (2 * w);
-        m |= ((r.c[w] >> 16) >= d.t ? 1u : 0u) << (2 * w + 1);
+    for (int r = 0; r < 10; ++r) {
+        const uint64_t p0 = (uint64_t)c0 * 0xD2511F53u, p1 = (uint64_t)c2 * 0xCD9E8D57u;
+        c0 = (uint32_t)(p1 >> 32) ^ c1 ^ k0;
+        c1 = (uint32_t)p1;
+        c2 = (uint32_t)(p0 >> 32) ^ c3 ^ k1;
+        c3 = (uint32_t)p0;
+        k0 += 0x9E3779B9u;
+        k1 += 0xBB67AE85u;
     }
-    return m;
+    OvPhilox o;
+    o.c[0] = c0; o.c[1] = c1; o.c[2] = c2; o.c[3] = c3;
+    return o;
+}
+
+// draw j of the block decides element j
+__device__ __forceinline__ bool ov_drop_kept(const OvDrop& d, const OvPhilox& r, int j) {
+    return ((j & 1) ? r.c[j >> 1] >> 16 : r.c[j >> 1] & 0xFFFFu) >= d.t;
+}
+
+__device__ __forceinline__ float ov_drop_apply(const OvDrop& d, const OvPhilox& r, int j, float v) {
+    return ov_drop_kept(d, r, j) ? v * d.scale : 0.f;
+}
+
+// A workgroup takes 256 U consecutive blocks; a thread has U blocks of 8 elements in flight, 16 B a load whatever the
+// alignment.  Its place in the matrix is one 64-bit division per workgroup and a small one per block.
+template <typename T, int U>
+__global__ __launch_bounds__(256) void ov_dropout_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ rows, int n_src,
+                                                         int R, int C, uint32_t nb, OvDrop d, T* __restrict__ y) {
+    constexpr int VE = 16 / sizeof(T), NV = 8 / VE;
+    const int64_t first = (int64_t)blockIdx.x * (256 * U), row0 = first / nb;
+    const uint32_t col0 = (uint32_t)(first - row0 * nb);
+    OvVec<T> v[U][NV];
+    int64_t row[U];
+    uint32_t c0[U];
+    bool ok[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const uint32_t t = col0 + threadIdx.x + 256 * u, dr = t / nb;
+        row[u] = row0 + dr;
+        c0[u] = (t - dr * nb) * 8;
+        ok[u] = true;
+        if (row[u] >= R) continue;
+        int64_t src = row[u];
+        if (rows) { src = rows[src]; ok[u] = src >= 0 && src < n_src; }
+        const T* xr = x + (ok[u] ? src : 0) * ldx + c0[u];
+        if (c0[u] + 8 <= (uint32_t)C) {
+            if (ok[u]) {
+#pragma unroll
+                for (int i = 0; i < NV; ++i) v[u][i].load(xr + i * VE);
+            }
+        } else if (ok[u]) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[u][j / VE].e[j % VE] = c0[u] + j < (uint32_t)C ? xr[j] : (T)0.f;
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        if (row[u] >= R) continue;
+        const OvPhilox r = ov_drop_draw(d, (uint64_t)first + threadIdx.x + 256 * u);
+        T* yr = y + row[u] * C + c0[u];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            T& e = v[u][j / VE].e[j % VE];
+            e = ov_from_f<T>(ok[u] ? ov_drop_apply(d, r, j, ov_to_f<T>(e)) : __builtin_nanf(""));
+        }
+        if (c0[u] + 8 <= (uint32_t)C) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) v[u][i].store(yr + i * VE);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (c0[u] + j < (uint32_t)C) yr[j] = v[u][j / VE].e[j % VE];
+        }
+    }
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ov_dropout_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ rows, int n_src,
-                                                         int R, int C, OvDrop d, T* __restrict__ y) {
-    const int nb = (C + 7) / 8;
+static int ov_dropout_launch(const void* x, int64_t ldx, const int32_t* rows, int n_src, int R, int C, const OvDrop& d, void* y, hipStream_t st) {
+    const uint32_t nb = ((uint32_t)C + 7) / 8;
     const int64_t total = (int64_t)R * nb;
-    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-        const int64_t r = i / nb;
-        const int c0 = (int)(i - r * nb) * 8;
-        int64_t src = r;
-        bool ok = true;
-        if (rows) { src = rows[r]; ok = src >= 0 && src < n_src; }
-        const uint32_t m = ov_drop_bits(d, (uint64_t)i);
-        for (int j = 0; j < 8 && c0 + j < C; ++j) {
-            float v = __builtin_nanf("");
-            if (ok) v = (m >> j) & 1 ? ov_to_f<T>(x[src * ldx + c0 + j]) * d.scale : 0.f;
-            y[r * C + c0 + j] = ov_from_f<T>(v);
-        }
-    }
+    const T* xt = static_cast<const T*>(x);
+    T* yt = static_cast<T*>(y);
+    // few blocks: one per thread, so that they spread over the CUs
+    const int64_t wg = total >= (1 << 20) ? (total + 1023) / 1024 : (total + 255) / 256;
+    if (wg > INT32_MAX) { ontovae_set_error("dropout: %d x %d elements are too many for one launch", R, C); return ONTOVAE_EINVAL; }
+    if (total >= (1 << 20)) hipLaunchKernelGGL((ov_dropout_kernel<T, 4>), dim3((unsigned)wg), dim3(256), 0, st, xt, ldx, rows, n_src, R, C, nb, d, yt);
+    else hipLaunchKernelGGL((ov_dropout_kernel<T, 1>), dim3((unsigned)wg), dim3(256), 0, st, xt, ldx, rows, n_src, R, C, nb, d, yt);
+    return ONTOVAE_OK;
 }
 
 extern "C" int ontovae_dropout(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, int32_t R, int32_t C, float p,
@@ -72,13 +135,13 @@ extern "C" int ontovae_dropout(const void* x, int32_t dtype, int64_t ldx, const 
     if (R == 0 || C == 0) return ONTOVAE_OK;
     if (!x || !y) { ontovae_set_error("dropout: NULL argument"); return ONTOVAE_EINVAL; }
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const int64_t total = (int64_t)R * ((C + 7) / 8);
-    const dim3 grid((unsigned)std::min<int64_t>((total + 255) / 256, 8192));
+    int rc;
     switch (dtype) {
-        case ONTOVAE_F32: hipLaunchKernelGGL(ov_dropout_kernel<float>, grid, dim3(256), 0, st, (const float*)x, ldx, rows, n_src, R, C, d, (float*)y); break;
-        case ONTOVAE_BF16: hipLaunchKernelGGL(ov_dropout_kernel<ov_bf>, grid, dim3(256), 0, st, (const ov_bf*)x, ldx, rows, n_src, R, C, d, (ov_bf*)y); break;
-        default: hipLaunchKernelGGL(ov_dropout_kernel<ov_hf>, grid, dim3(256), 0, st, (const ov_hf*)x, ldx, rows, n_src, R, C, d, (ov_hf*)y); break;
+        case ONTOVAE_F32: rc = ov_dropout_launch<float>(x, ldx, rows, n_src, R, C, d, y, st); break;
+        case ONTOVAE_BF16: rc = ov_dropout_launch<ov_bf>(x, ldx, rows, n_src, R, C, d, y, st); break;
+        default: rc = ov_dropout_launch<ov_hf>(x, ldx, rows, n_src, R, C, d, y, st); break;
     }
+    if (rc) return rc;
     OV_OPS_LAUNCH_CHECK("dropout");
     return ONTOVAE_OK;
 }

@@ -48,7 +48,7 @@ __device__ __forceinline__ float ov_act_grad(float v, int act) {
 
 __device__ __forceinline__ bool ov_gn_kept(const OvGn& p, int64_t row, int c) {
     if (p.drop.t == 0) return true;
-    return (ov_drop_bits(p.drop, (uint64_t)row * ((p.C + 7) / 8) + (c >> 3)) >> (c & 7)) & 1;
+    return ov_drop_kept(p.drop, ov_drop_draw(p.drop, (uint64_t)row * ((p.C + 7) / 8) + (c >> 3)), c & 7);
 }
 
 // one workgroup per (sample, group)

@@ -42,6 +42,14 @@ struct OvQ8 {
     }
 };
 
+// the epilogue of every variant, bit for bit: the float32 result is pinned before its rounding to the output type (which the
+// compiler otherwise merges into the fma for float16 where it can see both)
+__device__ __forceinline__ float ov_q8_out(int acc, float sa, float sb, float bias) {
+    float v = fmaf((float)acc * sa, sb, bias);
+    asm("" : "+v"(v));
+    return v;
+}
+
 __device__ __forceinline__ uint32_t ov_abs_bits(float v) { return __builtin_bit_cast(uint32_t, v) & 0x7fffffffu; }
 
 // One row per group of THREADS threads (a wave: 4 rows per workgroup; else one), the row held in registers between the search
@@ -284,7 +292,7 @@ __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ov_q8_gemm_kernel(
                 const int m = m0 + wm + 32 * i + (e & 3) + 8 * (e >> 2) + 4 * (lane >> 5);
                 if (m >= g.M) continue;
                 if constexpr (__is_same(T, int32_t)) g.slab[((int64_t)blockIdx.y * g.M + m) * g.N + n] = acc[i][j][e];
-                else static_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = ov_from_f<T>((float)acc[i][j][e] * g.sa[m] * tb + bi);
+                else static_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = ov_from_f<T>(ov_q8_out(acc[i][j][e], g.sa[m], tb, bi));
             }
     }
 }
@@ -298,7 +306,109 @@ __global__ __launch_bounds__(256) void ov_q8_combine_kernel(const OvQ8Gemm g, in
         int a = 0;
 #pragma unroll 8
         for (int z = 0; z < splits; ++z) a += g.slab[z * total + i];
-        static_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = ov_from_f<T>((float)a * g.sa[m] * g.sb[n] + (g.bias ? g.bias[n] : 0.f));
+        static_cast<T*>(g.y)[(int64_t)m * g.ldy + n] = ov_from_f<T>(ov_q8_out(a, g.sa[m], g.sb[n], g.bias ? g.bias[n] : 0.f));
+    }
+}
+
+// One to four rows of x against a layer, rows quantised on the way: the latency of one launch instead of three.  Every
+// workgroup reads the MT rows of x (from the L2 after the first), rounds its threads' pieces of 16 elements into registers and
+// walks weight rows blockIdx, + gridDim, ... with them: a thread meets the same 16 columns of every row, so neither operand
+// passes LDS.  Bound by the read of the weights.  The next weight row is requested before the current one is reduced.
+template <typename T, int MT, int NP>
+__global__ __launch_bounds__(256) void ov_q8_few_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ rows, int n_src, int M,
+                                                        const OvQ8Gemm g, int ytype) {
+    constexpr int VE = 16 / sizeof(T);
+    __shared__ uint32_t redu[4][MT];
+    __shared__ int redi[2][4][MT];
+    const int tid = threadIdx.x, lane = ov_lane(), wave = ov_wave_id();
+    ov_i32x4 w[NP];
+    auto wload = [&](int n) {
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            const int k = (tid + i * 256) * 16;
+            w[i] = ov_i32x4{0, 0, 0, 0};
+            const int8_t* src = g.B + (int64_t)n * g.ldb + k;
+            if (k + 16 <= g.K) __builtin_memcpy(&w[i], src, 16);
+            else if (k < g.K) {
+                OvBytes<16> b = {};
+#pragma unroll
+                for (int j = 0; j < 15; ++j)
+                    if (k + j < g.K) b.b[j] = src[j];
+                w[i] = __builtin_bit_cast(ov_i32x4, b);
+            }
+        }
+    };
+    wload(blockIdx.x);
+    ov_i32x4 q[MT][NP];
+    float s[MT];
+    {
+        T v[NP][16];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            int64_t src = m;
+            bool ok = m < M;
+            if (ok && rows) { src = rows[m]; ok = src >= 0 && src < n_src; }
+            const T* xr = x + (ok ? src : 0) * ldx;
+            uint32_t a = ok ? 0u : 0x7fffffffu;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const int k = (tid + i * 256) * 16;
+                if (ok && k + 16 <= g.K) {
+#pragma unroll
+                    for (int c = 0; c < 16 / VE; ++c) __builtin_memcpy(&v[i][c * VE], xr + k + c * VE, 16);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) v[i][j] = ok && k + j < g.K ? xr[k + j] : (T)0.f;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int j = 0; j < 16; ++j) a = max(a, ov_abs_bits(ov_to_f<T>(v[i][j])));
+            a = ov_wave_max_u(a);
+            if (lane == 0) redu[wave][m] = a;
+            __syncthreads();
+            s[m] = ov_q8_scale(max(max(redu[0][m], redu[1][m]), max(redu[2][m], redu[3][m])));
+            const OvQ8 f(s[m]);
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                OvBytes<16> b;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) b.b[j] = (int8_t)f(ov_to_f<T>(v[i][j]));
+                q[m][i] = __builtin_bit_cast(ov_i32x4, b);
+            }
+        }
+    }
+    int buf = 0;
+    for (int n = blockIdx.x; n < g.N; n += gridDim.x, buf ^= 1) {
+        int acc[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            acc[m] = 0;
+#pragma unroll
+            for (int i = 0; i < NP; ++i)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) acc[m] = __builtin_amdgcn_sdot4(q[m][i][c], w[i][c], acc[m], false);
+        }
+        if (n + (int)gridDim.x < g.N) wload(n + gridDim.x);
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+#pragma unroll
+            for (int o = 32; o > 0; o >>= 1) acc[m] += __shfl_xor(acc[m], o, 64);
+            if (lane == 0) redi[buf][wave][m] = acc[m];
+        }
+        __syncthreads();                     // two buffers: the next row's sums go to the other one
+        if (tid < MT && tid < M) {
+            const int a = (redi[buf][0][tid] + redi[buf][1][tid]) + (redi[buf][2][tid] + redi[buf][3][tid]);
+            float sm = s[0];
+#pragma unroll
+            for (int m = 1; m < MT; ++m) sm = tid == m ? s[m] : sm;
+            const float v = ov_q8_out(a, sm, g.sb[n], g.bias ? g.bias[n] : 0.f);
+            const int64_t o = (int64_t)tid * g.ldy + n;
+            if (ytype == ONTOVAE_F32) static_cast<float*>(g.y)[o] = v;
+            else if (ytype == ONTOVAE_BF16) static_cast<ov_bf*>(g.y)[o] = ov_from_f<ov_bf>(v);
+            else static_cast<ov_hf*>(g.y)[o] = ov_from_f<ov_hf>(v);
+        }
     }
 }
 
@@ -444,6 +554,74 @@ extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa
     }
     OV_OPS_LAUNCH_CHECK("int8_matmul");
     return ONTOVAE_OK;
+}
+
+// ---- linear layer with its input quantised on the way
+static int64_t ov_q8_ldq(int K) { return std::max<int64_t>(((int64_t)K + 63) / 64 * 64, 64); }
+// few rows: the fused kernel.  Up to 4 rows and 8 pieces of 16 columns per thread (K <= 32768), 32 registers a row
+static bool ov_q8_few(int M, int K) { return M <= 4 && K <= 32768 && (M <= 2 || K <= 20480); }
+
+extern "C" int64_t ontovae_int8_linear_workspace_bytes(int32_t M, int32_t N, int32_t K) {
+    if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K || ov_q8_few(M, K)) return 0;
+    const int64_t head = (M * ov_q8_ldq(K) + 255) / 256 * 256 + ((int64_t)M * 4 + 255) / 256 * 256;
+    return head + ontovae_int8_matmul_workspace_bytes(M, N, K);
+}
+
+template <typename T, int MT>
+static void ov_q8_few_go(const void* x, int64_t ldx, const int32_t* rows, int n_src, int M, const OvQ8Gemm& g, int ytype, hipStream_t st) {
+    const T* xt = static_cast<const T*>(x);
+    const dim3 grid((unsigned)std::min(g.N, 512));
+    const int np = (g.K + 4095) / 4096;
+    if (np <= 1) hipLaunchKernelGGL((ov_q8_few_kernel<T, MT, 1>), grid, dim3(256), 0, st, xt, ldx, rows, n_src, M, g, ytype);
+    else if (np <= 2) hipLaunchKernelGGL((ov_q8_few_kernel<T, MT, 2>), grid, dim3(256), 0, st, xt, ldx, rows, n_src, M, g, ytype);
+    else if (np <= 5) hipLaunchKernelGGL((ov_q8_few_kernel<T, MT, 5>), grid, dim3(256), 0, st, xt, ldx, rows, n_src, M, g, ytype);
+    else if constexpr (MT <= 2) hipLaunchKernelGGL((ov_q8_few_kernel<T, MT, 8>), grid, dim3(256), 0, st, xt, ldx, rows, n_src, M, g, ytype);
+}
+template <typename T>
+static void ov_q8_few_launch(const void* x, int64_t ldx, const int32_t* rows, int n_src, int M, const OvQ8Gemm& g, int ytype, hipStream_t st) {
+    if (M == 1) ov_q8_few_go<T, 1>(x, ldx, rows, n_src, M, g, ytype, st);
+    else if (M == 2) ov_q8_few_go<T, 2>(x, ldx, rows, n_src, M, g, ytype, st);
+    else ov_q8_few_go<T, 4>(x, ldx, rows, n_src, M, g, ytype, st);
+}
+
+extern "C" int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, const int8_t* w, int64_t ldw,
+                                   const float* sw, const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t ydtype, int64_t ldy,
+                                   void* workspace, int64_t workspace_bytes, void* stream) {
+    if (M < 0 || N < 0 || K < 0 || n_src < 0 || ldx < K || ldw < K || ldy < N || (!rows && n_src < M)) {
+        ontovae_set_error("int8_linear: M = %d, N = %d, K = %d, n_src = %d, ldx = %lld, ldw = %lld, ldy = %lld", M, N, K, n_src, (long long)ldx,
+                          (long long)ldw, (long long)ldy);
+        return ONTOVAE_EINVAL;
+    }
+    if (K > OV_Q8_MAX_K) { ontovae_set_error("int8_linear: K = %d, the sums are exact in 32 bits up to %d", K, OV_Q8_MAX_K); return ONTOVAE_EINVAL; }
+    if (dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16 || ydtype < ONTOVAE_F32 || ydtype > ONTOVAE_F16) {
+        ontovae_set_error("int8_linear: unknown element type %d / %d", dtype, ydtype);
+        return ONTOVAE_EINVAL;
+    }
+    if (M == 0 || N == 0) return ONTOVAE_OK;
+    if (!sw || !y || (K > 0 && (!x || !w))) { ontovae_set_error("int8_linear: NULL argument"); return ONTOVAE_EINVAL; }
+    const int64_t need = ontovae_int8_linear_workspace_bytes(M, N, K);
+    if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) {
+        ontovae_set_error("int8_linear: workspace of %lld bytes, 256-B aligned, needed", (long long)need);
+        return ONTOVAE_EINVAL;
+    }
+    if (ov_q8_few(M, K)) {
+        hipStream_t st = reinterpret_cast<hipStream_t>(stream);
+        OvQ8Gemm g{nullptr, 0, w, ldw, nullptr, sw, bias, M, N, K, 0, 0, 0, nullptr, y, ldy};
+        if (dtype == ONTOVAE_F32) ov_q8_few_launch<float>(x, ldx, rows, n_src, M, g, ydtype, st);
+        else if (dtype == ONTOVAE_BF16) ov_q8_few_launch<ov_bf>(x, ldx, rows, n_src, M, g, ydtype, st);
+        else ov_q8_few_launch<ov_hf>(x, ldx, rows, n_src, M, g, ydtype, st);
+        OV_OPS_LAUNCH_CHECK("int8_linear");
+        return ONTOVAE_OK;
+    }
+    const int64_t ldq = ov_q8_ldq(K);
+    char* p = static_cast<char*>(workspace);
+    int8_t* q = reinterpret_cast<int8_t*>(p);
+    p += (M * ldq + 255) / 256 * 256;
+    float* s = reinterpret_cast<float*>(p);
+    p += ((int64_t)M * 4 + 255) / 256 * 256;
+    int rc = ontovae_quantize_rows(x, dtype, ldx, rows, n_src, M, K, q, ldq, s, stream);
+    if (rc) return rc;
+    return ontovae_int8_matmul(q, ldq, s, w, ldw, sw, bias, M, N, K, y, ydtype, ldy, p, workspace_bytes - (p - static_cast<char*>(workspace)), stream);
 }
 
 #endif

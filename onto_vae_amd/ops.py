@@ -9,17 +9,41 @@ current stream of the tensors' device, which need not be the current device.
 The reference has no counterpart: its blocks are torch's Linear, BatchNorm1d, Dropout and ReLU (onto_vae/modules.py:43-64, 116-133).
 The models use these operators through set_precision('int8') and VAE(norm='group', input_drop=...).
 """
-import ctypes as C
+import contextlib
 import math
 
 import torch
 
 from . import _lib
-from .stats import _need_gpu, _ptr, _stream, _workspace
+from .stats import _need_gpu
 
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3}
 I32_MAX = 2 ** 31 - 1
+
+
+_SAME = contextlib.nullcontext()
+
+
+def _on(device):
+    """The tensors' device as the current one (entering torch's guard only when it changes something)."""
+    return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _p(t):
+    return None if t is None else t.data_ptr()
+
+
+def _stream(device):
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _workspace(nbytes, device):
+    """(buffer, address, bytes): torch's device allocations are 512-byte aligned, the library asks for 256."""
+    if nbytes <= 0:
+        return None, None, 0
+    buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return buf, buf.data_ptr(), nbytes
 
 
 def _dtype(t, what):
@@ -38,7 +62,7 @@ def _matrix(x, what):
     """[..., C] as a 2-D view with unit inner stride (copied only when its strides leave no other way)."""
     if x.dim() < 1:
         raise ValueError(f"{what}: at least one dimension expected")
-    m = x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
+    m = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
     if m.stride(1) != 1 and m.shape[1] > 1 or m.stride(0) < m.shape[1] and m.shape[0] > 1:
         m = m.contiguous()
     _size(m.shape[0], what)
@@ -87,10 +111,10 @@ def quantize_rows(x, rows=None):
     M = xm.shape[0] if rows is None else rows.shape[0]
     lead = tuple(x.shape[:-1]) if rows is None else (M,)
     ldq = max((K + 63) // 64 * 64, 64)
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         q = torch.empty(M, ldq, dtype=torch.int8, device=x.device)
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
-        _lib.check(_lib.lib().ontovae_quantize_rows(_ptr(xm), dt, ld, _ptr(rows), xm.shape[0], M, K, _ptr(q), ldq, _ptr(scale), _stream(x.device)),
+        _lib.check(_lib.lib().ontovae_quantize_rows(_p(xm), dt, ld, _p(rows), xm.shape[0], M, K, _p(q), ldq, _p(scale), _stream(x.device)),
                    "quantize_rows")
     qk = q[:, :K]
     return (qk if len(lead) == 1 else qk.view(*lead, K) if M else q.new_empty(*lead, K)), scale.view(lead)
@@ -114,10 +138,10 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
     sb = _vector(b_scale, N, a.device, "int8_matmul: b_scale")
     bias = _vector(bias, N, a.device, "int8_matmul: bias")
     L = _lib.lib()
-    with torch.cuda.device(a.device):
+    with _on(a.device):
         y = torch.empty(*lead, N, dtype=dtype, device=a.device)
         keep, ws, nbytes = _workspace(L.ontovae_int8_matmul_workspace_bytes(M, N, K), a.device)
-        _lib.check(L.ontovae_int8_matmul(_ptr(am), lda, _ptr(sa), _ptr(bm), ldb, _ptr(sb), _ptr(bias), M, N, K, _ptr(y), DTYPES[dtype], N,
+        _lib.check(L.ontovae_int8_matmul(_p(am), lda, _p(sa), _p(bm), ldb, _p(sb), _p(bias), M, N, K, _p(y), DTYPES[dtype], N,
                                          ws, nbytes, _stream(a.device)), "int8_matmul")
     return y
 
@@ -125,8 +149,28 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
 def int8_linear(x, weight, weight_scale, bias=None, rows=None, dtype=None):
     """x weight^T + bias with an 8-bit weight [N, K] (quantize_rows of the layer's float weight, done once) and the rows of x (of
     x[rows]) quantised on the way: one scale per token and per output channel.  dtype: that of y, x's by default."""
-    q, s = quantize_rows(x, rows)
-    return int8_matmul(q, s, weight, weight_scale, bias, x.dtype if dtype is None else dtype)
+    _need_gpu(x, "int8_linear")
+    dt = _dtype(x, "int8_linear")
+    if dtype is None:
+        dtype = x.dtype
+    elif dtype not in DTYPES:
+        raise ValueError(f"int8_linear: dtype must be float32, bfloat16 or float16, got {dtype}")
+    rows = _rows(rows, x, "int8_linear")
+    if weight.dtype != torch.int8 or weight.dim() != 2 or weight.device != x.device or x.dim() < 1 or x.shape[-1] != weight.shape[1]:
+        raise ValueError("int8_linear: x [..., K] and int8 weight [N, K] on one device expected")
+    xm, ld = _matrix(x, "int8_linear")
+    wm, ldw = _matrix(weight, "int8_linear")
+    K, N = xm.shape[1], wm.shape[0]
+    M = xm.shape[0] if rows is None else rows.shape[0]
+    sw = _vector(weight_scale, N, x.device, "int8_linear: weight_scale")
+    bias = _vector(bias, N, x.device, "int8_linear: bias")
+    L = _lib.lib()
+    with _on(x.device):
+        y = torch.empty((*x.shape[:-1], N) if rows is None else (M, N), dtype=dtype, device=x.device)
+        keep, ws, nbytes = _workspace(L.ontovae_int8_linear_workspace_bytes(M, N, K), x.device)
+        _lib.check(L.ontovae_int8_linear(_p(xm), dt, ld, _p(rows), xm.shape[0], _p(wm), ldw, _p(sw), _p(bias), M, N, K, _p(y), DTYPES[dtype], N,
+                                         ws, nbytes, _stream(x.device)), "int8_linear")
+    return y
 
 
 # ---------------------------------------------------------------- group norm with an activation
@@ -163,15 +207,15 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", drop
         raise ValueError(f"group_norm_act: eps = {eps}")
     x = x.contiguous()
     L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         y = torch.empty_like(x)
         mean = torch.empty(N, groups, dtype=torch.float32, device=x.device)
         rstd = torch.empty_like(mean)
         if y.numel() == 0:          # no rows to take statistics of
             return y, mean.zero_(), rstd.zero_()
         keep, ws, nbytes = _workspace(L.ontovae_group_norm_act_workspace_bytes(dt, N, S, Cn, groups, 0), x.device)
-        _lib.check(L.ontovae_group_norm_act(_ptr(x), dt, N, S, Cn, groups, _ptr(weight), _ptr(bias), DTYPES[wdt], float(eps), a, drop, seed,
-                                            offset, _ptr(y), _ptr(mean), _ptr(rstd), ws, nbytes, _stream(x.device)), "group_norm_act")
+        _lib.check(L.ontovae_group_norm_act(_p(x), dt, N, S, Cn, groups, _p(weight), _p(bias), DTYPES[wdt], float(eps), a, drop, seed,
+                                            offset, _p(y), _p(mean), _p(rstd), ws, nbytes, _stream(x.device)), "group_norm_act")
     return y, mean, rstd
 
 
@@ -187,15 +231,15 @@ def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, a
             raise ValueError(f"group_norm_act_backward: {n} must be float32 [{N}, {groups}] on {x.device}")
     dy, x, mean, rstd = dy.contiguous(), x.contiguous(), mean.contiguous(), rstd.contiguous()
     L = _lib.lib()
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         dx = torch.empty_like(x)
         dw = torch.empty(Cn, dtype=torch.float32, device=x.device) if weight is not None else None
         db = torch.empty(Cn, dtype=torch.float32, device=x.device) if bias is not None else None
         if x.numel() == 0:
             return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None
         keep, ws, nbytes = _workspace(L.ontovae_group_norm_act_workspace_bytes(dt, N, S, Cn, groups, 1), x.device)
-        _lib.check(L.ontovae_group_norm_act_backward(_ptr(dy), _ptr(x), dt, N, S, Cn, groups, _ptr(weight), _ptr(bias), DTYPES[wdt], _ptr(mean),
-                                                     _ptr(rstd), a, drop, seed, offset, _ptr(dx), _ptr(dw), _ptr(db), ws, nbytes,
+        _lib.check(L.ontovae_group_norm_act_backward(_p(dy), _p(x), dt, N, S, Cn, groups, _p(weight), _p(bias), DTYPES[wdt], _p(mean),
+                                                     _p(rstd), a, drop, seed, offset, _p(dx), _p(dw), _p(db), ws, nbytes,
                                                      _stream(x.device)), "group_norm_act_backward")
     return dx, dw, db
 
@@ -213,9 +257,9 @@ def dropout(x, p, seed, offset=0, rows=None):
     rows = _rows(rows, x, "dropout")
     xm, ld = _matrix(x, "dropout")
     R = xm.shape[0] if rows is None else rows.shape[0]
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         y = torch.empty(x.shape if rows is None else (R, xm.shape[1]), dtype=x.dtype, device=x.device)
-        _lib.check(_lib.lib().ontovae_dropout(_ptr(xm), dt, ld, _ptr(rows), xm.shape[0], R, xm.shape[1], float(p), seed, offset, _ptr(y),
+        _lib.check(_lib.lib().ontovae_dropout(_p(xm), dt, ld, _p(rows), xm.shape[0], R, xm.shape[1], float(p), seed, offset, _p(y),
                                               _stream(x.device)), "dropout")
     return y
 

@@ -149,7 +149,8 @@ def test_int8_extremes_are_exact():
 
 
 @pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("M,K,N", [(1, 360, 720), (130, 1000, 129), (40, 5893, 229), (9, 20000, 360)])
+@pytest.mark.parametrize("M,K,N", [(1, 360, 720), (130, 1000, 129), (40, 5893, 229), (9, 20000, 360), (1, 20000, 360), (2, 5893, 700), (3, 333, 41),
+                                   (4, 20000, 9), (2, 32768, 5), (1, 32769, 5), (4, 1, 600), (3, 17, 2000), (5, 64, 3)])
 def test_int8_linear(M, K, N, dtype):
     t = DT[dtype]
     x, w, bias = rnd(1, M, K, dtype=t), rnd(2, N, K, scale=K ** -0.5), rnd(3, N)
@@ -165,11 +166,13 @@ def test_int8_linear(M, K, N, dtype):
     bound = (np.abs(f64(x)).sum(1)[:, None] * f64(sw)[None] / 2 + np.abs(f64(w)).sum(1)[None] * sx.astype(np.float64)[:, None] / 2 +
              K * sx.astype(np.float64)[:, None] * f64(sw)[None] / 4)
     assert (np.abs(want - full) <= bound).all()
+    assert torch.equal(y, ops.int8_matmul(*ops.quantize_rows(x), qw, sw, bias, dtype=t))      # the fused form of few rows, bit for bit
+    idx = torch.tensor([M - 1, 0, -1, M], device=DEV)
+    yr = ops.int8_linear(x, qw, sw, bias, rows=idx)
+    assert torch.equal(yr[:2], y[[M - 1, 0]]) and torch.isnan(yr[2:]).all()
     x[0, K // 2] = float("nan")
     y = ops.int8_linear(x, qw, sw, bias, dtype=torch.float32)
     assert torch.isnan(y[0]).all() and torch.isfinite(y[1:]).all() and y.dtype == torch.float32
-    rows = torch.tensor([M - 1, 0], device=DEV)
-    assert torch.equal(ops.int8_linear(x, qw, sw, bias, rows=rows)[0], ops.int8_linear(x[M - 1:], qw, sw, bias)[0]) or M == 1
 
 
 # ---------------------------------------------------------------- group norm
@@ -428,7 +431,9 @@ def test_refusals():
                 lambda: ops.quantize_rows(x.sum()), lambda: ops.int8_matmul(x, s, q, s), lambda: ops.int8_matmul(q, s, q[:, :8], s),
                 lambda: ops.int8_matmul(q, s[:2], q, s), lambda: ops.int8_matmul(q, s, q, s[:2]), lambda: ops.int8_matmul(q, s, q, s, bias=s[:1]),
                 lambda: ops.int8_matmul(q, s.half(), q, s), lambda: ops.int8_matmul(q, s, q, s, dtype=torch.float64),
-                lambda: ops.int8_matmul(q, s, q.cpu(), s), lambda: ops.group_norm_act(x, 3), lambda: ops.group_norm_act(x, 0),
+                lambda: ops.int8_matmul(q, s, q.cpu(), s), lambda: ops.int8_linear(x, q, s[:1]), lambda: ops.int8_linear(x, x, s),
+                lambda: ops.int8_linear(x[:, :8], q, s), lambda: ops.int8_linear(x, q, s, bias=s[:2]), lambda: ops.int8_linear(x, q, s, dtype=torch.int8),
+                lambda: ops.int8_linear(x.double(), q, s), lambda: ops.int8_linear(x.view(2, 2, 16), q, s, rows=torch.tensor([0], device=DEV)), lambda: ops.group_norm_act(x, 3), lambda: ops.group_norm_act(x, 0),
                 lambda: ops.group_norm_act(x[0], 4), lambda: ops.group_norm_act(x, 4, act="tanh"), lambda: ops.group_norm_act(x, 4, drop=1.5),
                 lambda: ops.group_norm_act(x, 4, drop=float("nan")), lambda: ops.group_norm_act(x, 4, eps=-1.0), lambda: ops.group_norm_act(x, 4, seed=-1),
                 lambda: ops.group_norm_act(x, 4, weight=x[0, :8]), lambda: ops.group_norm_act(x, 4, weight=x[0].double()),

@@ -77,6 +77,16 @@ def test_int8_matmul_needs_its_workspace(L):
             assert L.ontovae_int8_matmul(P, K, P, P, K, P, NULL, M, N, K, P, 0, N, NULL, need, NULL) == -1
 
 
+@pytest.mark.parametrize("change", [dict(M=-1), dict(N=-1), dict(K=-1), dict(ldx=3), dict(ldw=3), dict(ldy=2), dict(n_src=1), dict(dtype=3), dict(ydtype=-1),
+                                    dict(K=131072, ldx=1 << 20, ldw=1 << 20), dict(x=NULL), dict(w=NULL), dict(sw=NULL), dict(y=NULL),
+                                    dict(M=9, n_src=9, nbytes=8), dict(M=9, n_src=9, ws=NULL), dict(M=9, n_src=9, ws=C.c_void_p((1 << 20) + 16))])
+def test_int8_linear_refusals(L, change):
+    a = dict(x=P, dtype=0, ldx=4, rows=NULL, n_src=2, w=P, ldw=4, sw=P, bias=NULL, M=2, N=3, K=4, y=P, ydtype=0, ldy=3, ws=P, nbytes=1 << 30, stream=NULL)
+    a.update(change)
+    assert L.ontovae_int8_linear(*a.values()) == -1
+    assert b"int8_linear" in L.ontovae_last_error()
+
+
 GN = dict(x=P, dtype=0, N=2, S=3, C=8, groups=2, w=P, b=P, wdtype=0, eps=1e-5, act=0, drop=0.0, seed=0, offset=0, y=P, mean=P, rstd=P, ws=P,
           nbytes=1 << 30, stream=NULL)
 
