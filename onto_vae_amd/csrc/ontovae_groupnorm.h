@@ -28,111 +28,671 @@ __device__ __forceinline__ float ov_gn_param(const void* p, int wtype, int c, fl
     return (float)static_cast<const ov_hf*>(p)[c];
 }
 
-__device__ __forceinline__ float ov_act(float v, int act) {
-    if (act == ONTOVAE_ACT_RELU) return v > 0.f ? v : (v <= 0.f ? 0.f : v);          // NaN stays NaN
-    if (act == ONTOVAE_ACT_SILU) return v / (1.f + __expf(-v));
-    if (act == ONTOVAE_ACT_GELU) return 0.5f * v * (1.f + erff(v * 0.70710678118654752f));
-    return v;
-}
+// sigma(v) and what silu and gelu and their slopes need of exp and erf
+__device__ __forceinline__ float ov_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
-__device__ __forceinline__ float ov_act_grad(float v, int act) {
-    if (act == ONTOVAE_ACT_RELU) return v > 0.f ? 1.f : (v <= 0.f ? 0.f : v);
-    if (act == ONTOVAE_ACT_SILU) {
-        const float s = 1.f / (1.f + __expf(-v));
-        return s * (1.f + v * (1.f - s));
+// act over E values: the switch stands outside the loop (act is uniform)
+template <int E>
+__device__ __forceinline__ void ov_act(float (&v)[E], int act) {
+    if (act == ONTOVAE_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];                    // NaN stays NaN
+    } else if (act == ONTOVAE_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = v[j] * ov_sigmoid(v[j]);
+    } else if (act == ONTOVAE_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = 0.5f * v[j] * (1.f + erff(v[j] * 0.70710678118654752f));
     }
-    if (act == ONTOVAE_ACT_GELU)
-        return 0.5f * (1.f + erff(v * 0.70710678118654752f)) + v * __expf(-0.5f * v * v) * 0.39894228040143268f;
-    return 1.f;
 }
 
-__device__ __forceinline__ bool ov_gn_kept(const OvGn& p, int64_t row, int c) {
-    if (p.drop.t == 0) return true;
-    return ov_drop_kept(p.drop, ov_drop_draw(p.drop, (uint64_t)row * ((p.C + 7) / 8) + (c >> 3)), c & 7);
+// d act / d v
+template <int E>
+__device__ __forceinline__ void ov_act_grad(float (&v)[E], int act) {
+    if (act == ONTOVAE_ACT_NONE) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = 1.f;
+    } else if (act == ONTOVAE_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v[j] = v[j] > 0.f ? 1.f : (v[j] <= 0.f ? 0.f : v[j]);
+    } else if (act == ONTOVAE_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+            const float s = ov_sigmoid(v[j]);
+            v[j] = s * (1.f + v[j] * (1.f - s));
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            v[j] = 0.5f * (1.f + erff(v[j] * 0.70710678118654752f)) + v[j] * __expf(-0.5f * v[j] * v[j]) * 0.39894228040143268f;
+    }
 }
 
-// one workgroup per (sample, group)
+// dropout of E neighbours of a row from column c on (E <= 8: at most two of the row's blocks of eight): f[j] v[j], f = 0 or scale
+template <int E>
+__device__ __forceinline__ void ov_gn_drop(const OvGn& p, int64_t row, int c, float (&v)[E]) {
+    if (p.drop.t == 0) return;
+    const uint64_t block = (uint64_t)row * ((p.C + 7) / 8) + (c >> 3);
+    const int o = c & 7;
+    OvPhilox r = ov_drop_draw(p.drop, block);
+    uint32_t m = 0;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) m |= (ov_drop_kept(p.drop, r, j) ? 1u : 0u) << j;
+    if (o + E > 8) {
+        r = ov_drop_draw(p.drop, block + 1);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) m |= (ov_drop_kept(p.drop, r, j) ? 1u : 0u) << (8 + j);
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] = (m >> (o + j)) & 1 ? v[j] * p.drop.scale : 0.f;
+}
+
+// 16 bytes of a row (cnt of them valid: a group's or a row's last piece), as floats; nothing is read behind cnt
 template <typename T>
-__global__ __launch_bounds__(256) void ov_gn_fwd_kernel(const T* __restrict__ x, const OvGn p, T* __restrict__ y, float* __restrict__ mean,
-                                                        float* __restrict__ rstd) {
+__device__ __forceinline__ void ov_gn_load(const T* x, int cnt, float (&f)[OvVec<T>::N]) {
+    constexpr int E = OvVec<T>::N;
+    OvVec<T> v;
+    if (cnt >= E) v.load(x);
+    else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) v.e[j] = j < cnt ? x[j] : (T)0.f;
+    }
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = ov_to_f<T>(v.e[j]);
+}
+template <typename T>
+__device__ __forceinline__ void ov_gn_store(T* y, int cnt, const float (&f)[OvVec<T>::N]) {
+    constexpr int E = OvVec<T>::N;
+    OvVec<T> v;
+#pragma unroll
+    for (int j = 0; j < E; ++j) v.e[j] = ov_from_f<T>(f[j]);
+    if (cnt >= E) v.store(y);
+    else {
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+            if (j < cnt) y[j] = v.e[j];
+    }
+}
+
+template <int E>
+__device__ __forceinline__ void ov_gn_store_f(float* y, int cnt, const float (&f)[E]) {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+        if (j < cnt) y[j] = f[j];
+}
+
+// sum over the LPG threads of a group: lanes of a wave, or the workgroup
+template <int LPG>
+__device__ __forceinline__ float ov_gn_sum(float v, float* red) {
+    if (LPG <= 64) {
+#pragma unroll
+        for (int o = LPG / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+        return v;
+    }
+    return ov_block_sum(v, red);
+}
+
+// ---------------------------------------------------------------- S = 1: a group is one contiguous run of cg elements
+// LPG threads hold a group in registers, NV pieces of 16 bytes each; a slot of LPG threads keeps its group and walks the
+// samples rs, rs + RS, ...: weight and bias (and the sums of their gradients) stay in registers.  Neighbouring slots take
+// neighbouring groups, so a workgroup reads contiguous memory.  One read of x (and dy), one write: bound by memory.
+template <typename T, int LPG, int NV>
+__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(const T* __restrict__ x, const OvGn p, int RS, T* __restrict__ y,
+                                                                             float* __restrict__ mean, float* __restrict__ rstd) {
+    constexpr int E = OvVec<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
+    __shared__ float red[16];
+    const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
+    const int j = threadIdx.x % LPG, g = (int)(slot % p.groups), rs = (int)(slot / p.groups);
+    if (rs >= RS) return;
+    float w[NV][E], b[NV][E];
+    int cnt[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int o = (j + i * LPG) * E;
+        cnt[i] = min(p.cg - o, E);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            w[i][k] = k < cnt[i] ? ov_gn_param(p.w, p.wtype, g * p.cg + o + k, 1.f) : 0.f;
+            b[i][k] = k < cnt[i] ? ov_gn_param(p.b, p.wtype, g * p.cg + o + k, 0.f) : 0.f;
+        }
+    }
+    const float len = (float)p.cg;
+    for (int n = rs; n < p.N; n += RS) {
+        const int64_t base = (int64_t)n * p.C + g * p.cg;
+        float v[NV][E];
+        float s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) ov_gn_load<T>(x + base + (j + i * LPG) * E, cnt[i], v[i]);
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < E; ++k) s += v[i][k];
+        const float mu = ov_gn_sum<LPG>(s, red) / len;
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                const float d = v[i][k] - mu;
+                s += k < cnt[i] ? d * d : 0.f;
+            }
+        const float r = 1.f / sqrtf(ov_gn_sum<LPG>(s, red) / len + p.eps);
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (cnt[i] <= 0) continue;
+            const int o = (j + i * LPG) * E;
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[i][k] = (v[i][k] - mu) * r * w[i][k] + b[i][k];
+            ov_act<E>(v[i], p.act);
+            ov_gn_drop<E>(p, n, g * p.cg + o, v[i]);
+            ov_gn_store<T>(y + base + o, cnt[i], v[i]);
+        }
+        if (j == 0) {
+            mean[(int64_t)n * p.groups + g] = mu;
+            rstd[(int64_t)n * p.groups + g] = r;
+        }
+    }
+}
+
+// part: [2][RS][C]: the slots' sums of dv xhat, then of dv (written for every slot, also one without a sample)
+template <typename T, int LPG, int NV>
+__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p, int RS,
+                                                                             const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                                             T* __restrict__ dx, float* __restrict__ part) {
+    constexpr int E = OvVec<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
+    __shared__ float red[16];
+    const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
+    const int j = threadIdx.x % LPG, g = (int)(slot % p.groups), rs = (int)(slot / p.groups);
+    if (rs >= RS) return;
+    float w[NV][E], b[NV][E], sw[NV][E], sb[NV][E];
+    int cnt[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int o = (j + i * LPG) * E;
+        cnt[i] = min(p.cg - o, E);
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            w[i][k] = k < cnt[i] ? ov_gn_param(p.w, p.wtype, g * p.cg + o + k, 1.f) : 0.f;
+            b[i][k] = k < cnt[i] ? ov_gn_param(p.b, p.wtype, g * p.cg + o + k, 0.f) : 0.f;
+            sw[i][k] = sb[i][k] = 0.f;
+        }
+    }
+    const float len = (float)p.cg;
+    for (int n = rs; n < p.N; n += RS) {
+        const int64_t base = (int64_t)n * p.C + g * p.cg;
+        const float mu = mean[(int64_t)n * p.groups + g], r = rstd[(int64_t)n * p.groups + g];
+        float v[NV][E], d[NV][E];
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            ov_gn_load<T>(x + base + (j + i * LPG) * E, cnt[i], v[i]);
+            ov_gn_load<T>(dy + base + (j + i * LPG) * E, cnt[i], d[i]);
+        }
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (cnt[i] <= 0) continue;
+            ov_gn_drop<E>(p, n, g * p.cg + (j + i * LPG) * E, d[i]);
+            float a[E];
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                v[i][k] = (v[i][k] - mu) * r;
+                a[k] = v[i][k] * w[i][k] + b[i][k];
+            }
+            ov_act_grad<E>(a, p.act);
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                if (k >= cnt[i]) { v[i][k] = 0.f; a[k] = 0.f; }
+                const float dv = d[i][k] == 0.f ? 0.f : d[i][k] * a[k];        // a dropped place: 0 whatever act' is
+                sw[i][k] += dv * v[i][k];
+                sb[i][k] += dv;
+                d[i][k] = dv * w[i][k];
+                s1 += d[i][k];
+                s2 += d[i][k] * v[i][k];
+            }
+        }
+        s1 = ov_gn_sum<LPG>(s1, red) / len;
+        s2 = ov_gn_sum<LPG>(s2, red) / len;
+#pragma unroll
+        for (int i = 0; i < NV; ++i) {
+            if (cnt[i] <= 0) continue;
+#pragma unroll
+            for (int k = 0; k < E; ++k) d[i][k] = r * (d[i][k] - s1 - v[i][k] * s2);
+            ov_gn_store<T>(dx + base + (j + i * LPG) * E, cnt[i], d[i]);
+        }
+    }
+    if (!part) return;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int64_t o = (int64_t)rs * p.C + g * p.cg + (j + i * LPG) * E;
+        ov_gn_store_f<E>(part + o, cnt[i], sw[i]);
+        ov_gn_store_f<E>(part + (int64_t)RS * p.C + o, cnt[i], sb[i]);
+    }
+}
+
+// column sums of part [2][R][C] in a fixed order: 16 channels x 16 rows at a time per workgroup
+__global__ __launch_bounds__(256) void ov_gn_param_kernel(const float* __restrict__ part, int64_t R, int C, float* __restrict__ dw,
+                                                          float* __restrict__ db) {
+    __shared__ float red[16][17];
+    float* out = blockIdx.y ? db : dw;
+    if (!out) return;
+    const float* src = part + (blockIdx.y ? R * C : 0);
+    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    if (c < C) {
+        int64_t r = ty;
+        for (; r + 112 < R; r += 128) {
+            float t[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) t[u] = src[(r + 16 * u) * C + c];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) s[u & 3] += t[u];
+        }
+        for (; r < R; r += 16) s[0] += src[r * C + c];
+    }
+    red[ty][tx] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (ty == 0 && c < C) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) t += red[k][tx];
+        out[c] = t;
+    }
+}
+
+// ---------------------------------------------------------------- S > 1: tiles of rows x channels
+// A workgroup takes rows [r0, r1) of a sample and a block of whole groups (all channels if they fit): 256 threads as TX pieces
+// of 16 bytes x TY rows, a thread's channels fixed, so that weight, bias and the per-channel sums stay in registers; channel
+// sums meet in LDS, group sums are sums of channel sums (a piece may hold parts of several groups).
+//   MODE 0: sums of the tile only      MODE 1: the output, from the sums of the sample's tiles
+//   MODE 2: the tile is the whole sample; both in one launch, the second read from the cache
+// Modes 0 and 1 read x (and dy) once each; mode 1 takes the tiles in the opposite order, so that what the last-level cache still
+// holds of mode 0's reads is taken first.
+struct OvGnTile {
+    int gb, nblk;            // groups of a channel block, channel blocks
+    int tx, ty;              // pieces of a block's row, rows at a time
+    int chunks, rows;        // tiles along S, rows of one
+    float* part;             // per tile and group: 2 floats, [N][chunks][groups][2]
+};
+
+struct OvGnPlace { int n, chunk, c0, cb, g0, ng, r0, r1; };
+__device__ __forceinline__ OvGnPlace ov_gn_place(const OvGn& p, const OvGnTile& t, bool reverse) {
+    OvGnPlace q;
+    int id = reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
+    const int blk = id % t.nblk;
+    id /= t.nblk;
+    q.chunk = id % t.chunks;
+    q.n = id / t.chunks;
+    q.g0 = blk * t.gb;
+    q.ng = min(t.gb, p.groups - q.g0);
+    q.c0 = q.g0 * p.cg;
+    q.cb = q.ng * p.cg;
+    q.r0 = q.chunk * t.rows;
+    q.r1 = min(q.r0 + t.rows, p.S);
+    return q;
+}
+
+// count-weighted combination of the chunks' (first, second) over a group; lanes of the workgroup share the groups out.
+// FWD: (mean, M2) by Chan's formula about the overall mean -> (mu, r).  Else: plain sums / count.
+template <bool FWD>
+__device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, const OvGnPlace& q, float2* st) {
+    int lg = 64;                                         // lanes per group
+    while (lg > 1 && (lg > t.chunks || lg * q.ng > 256)) lg >>= 1;
+    for (int g = threadIdx.x / lg; g < q.ng; g += 256 / lg) {
+        const int l = threadIdx.x % lg;
+        const float2* src = reinterpret_cast<const float2*>(t.part) + ((int64_t)q.n * t.chunks * p.groups + q.g0 + g);
+        float a = 0.f, b = 0.f;
+        for (int k = l; k < t.chunks; k += lg) {
+            const float2 v = src[(int64_t)k * p.groups];
+            a += FWD ? v.x * (float)(min(t.rows, p.S - k * t.rows) * p.cg) : v.x;
+            b += v.y;
+        }
+        for (int o = lg / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
+        const float total = (float)((int64_t)p.S * p.cg);
+        if (FWD) {
+            const float mu = a / total;
+            float d2 = 0.f;
+            for (int k = l; k < t.chunks; k += lg) {
+                const float d = src[(int64_t)k * p.groups].x - mu;
+                d2 += d * d * (float)(min(t.rows, p.S - k * t.rows) * p.cg);
+            }
+            for (int o = lg / 2; o > 0; o >>= 1) d2 += __shfl_xor(d2, o, 64);
+            if (l == 0) st[g] = make_float2(mu, 1.f / sqrtf((b + d2) / total + p.eps));
+        } else if (l == 0) {
+            st[g] = make_float2(a / total, b / total);
+        }
+    }
+    __syncthreads();
+}
+
+#define OV_GN_MAX_CB(E) (256 * (E))
+
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict__ x, const OvGn p, const OvGnTile t, T* __restrict__ y,
+                                                             float* __restrict__ mean, float* __restrict__ rstd) {
+    constexpr int E = OvVec<T>::N, RB = 8;
+    __shared__ float2 cs[OV_GN_MAX_CB(E)];               // (mean, M2) of a thread's rows of a channel
+    __shared__ float2 st[OV_GN_MAX_CB(E)];               // per group: (mean, M2), then (mu, r)
+    const OvGnPlace q = ov_gn_place(p, t, MODE == 1);
+    const int tid = threadIdx.x, ty = tid / t.tx, tx = tid - ty * t.tx;
+    const bool on = ty < t.ty;
+    const int cnt = on ? min(q.cb - tx * E, E) : 0;      // <= 0: no channel of the block
+    const int64_t row0 = (int64_t)q.n * p.S;
+    const T* xc = x + q.c0 + tx * E;
+    if (MODE != 1) {
+        float m[E], m2[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) m[k] = m2[k] = 0.f;
+        int have = 0;
+        if (cnt > 0)
+            for (int r = q.r0 + ty; r < q.r1; r += RB * t.ty) {
+                float v[RB][E];
+                const int nb = min((q.r1 - r + t.ty - 1) / t.ty, RB);
+#pragma unroll
+                for (int i = 0; i < RB; ++i) ov_gn_load<T>(xc + (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C, cnt, v[i]);
+                // mean and second moment of these rows, then Chan's combination with the ones before
+                const float fb = (float)nb, ft = (float)(have + nb), wgt = fb / ft, cross = (float)have * wgt;
+#pragma unroll
+                for (int k = 0; k < E; ++k) {
+                    float s = 0.f, s2 = 0.f;
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) s += i < nb ? v[i][k] : 0.f;
+                    const float mb = s / fb;
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) {
+                        const float d = v[i][k] - mb;
+                        s2 += i < nb ? d * d : 0.f;
+                    }
+                    const float d = mb - m[k];
+                    m[k] += d * wgt;
+                    m2[k] += s2 + d * d * cross;
+                }
+                have += nb;
+            }
+        if (on)
+#pragma unroll
+            for (int k = 0; k < E; ++k) cs[ty * t.tx * E + tx * E + k] = make_float2(m[k], m2[k]);
+        __syncthreads();
+        // a channel's mean and M2 over the ty's (their row counts follow from ty), into the place of ty = 0
+        const int rows = q.r1 - q.r0;
+        for (int c = tid; c < q.cb; c += 256) {
+            float a = 0.f, b = 0.f;
+            for (int k = 0; k < t.ty; ++k) a += cs[k * t.tx * E + c].x * (float)((rows - k + t.ty - 1) / t.ty);
+            a /= (float)rows;
+            for (int k = 0; k < t.ty; ++k) {
+                const float2 v = cs[k * t.tx * E + c];
+                const float d = v.x - a;
+                b += v.y + d * d * (float)((rows - k + t.ty - 1) / t.ty);
+            }
+            st[c] = make_float2(a, b);
+        }
+        __syncthreads();
+        for (int g = tid; g < q.ng; g += 256) {
+            float a = 0.f, b = 0.f;
+            for (int k = 0; k < p.cg; ++k) a += st[g * p.cg + k].x;
+            a /= (float)p.cg;
+            for (int k = 0; k < p.cg; ++k) {
+                const float2 v = st[g * p.cg + k];
+                const float d = v.x - a;
+                b += v.y + d * d * (float)rows;
+            }
+            if (MODE == 0) reinterpret_cast<float2*>(t.part)[((int64_t)q.n * t.chunks + q.chunk) * p.groups + q.g0 + g] = make_float2(a, b);
+            else cs[g] = make_float2(a, 1.f / sqrtf(b / (float)((int64_t)rows * p.cg) + p.eps));
+        }
+        if (MODE == 0) return;
+        __syncthreads();
+    } else {
+        ov_gn_gather<true>(p, t, q, cs);
+    }
+    if (q.chunk == 0)
+        for (int g = tid; g < q.ng; g += 256) {
+            mean[(int64_t)q.n * p.groups + q.g0 + g] = cs[g].x;
+            rstd[(int64_t)q.n * p.groups + q.g0 + g] = cs[g].y;
+        }
+    if (cnt <= 0) return;
+    float mu[E], rw[E], b[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = min(tx * E + k, q.cb - 1);
+        const float2 v = cs[c / p.cg];
+        mu[k] = v.x;
+        rw[k] = v.y * ov_gn_param(p.w, p.wtype, q.c0 + c, 1.f);
+        b[k] = ov_gn_param(p.b, p.wtype, q.c0 + c, 0.f);
+    }
+    constexpr int RA = 4;
+    for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
+        float v[RA][E];
+#pragma unroll
+        for (int i = 0; i < RA; ++i) ov_gn_load<T>(xc + (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C, cnt, v[i]);
+#pragma unroll
+        for (int i = 0; i < RA; ++i) {
+            const int rr = r + i * t.ty;
+            if (rr >= q.r1) break;
+#pragma unroll
+            for (int k = 0; k < E; ++k) v[i][k] = (v[i][k] - mu[k]) * rw[k] + b[k];
+            ov_act<E>(v[i], p.act);
+            ov_gn_drop<E>(p, row0 + rr, q.c0 + tx * E, v[i]);
+            ov_gn_store<T>(y + (row0 + rr) * p.C + q.c0 + tx * E, cnt, v[i]);
+        }
+    }
+}
+
+// chan: [2][N chunks][C]: the tiles' sums of dv xhat, then of dv, per channel
+template <typename T, int MODE>
+__global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p, const OvGnTile t,
+                                                             const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
+                                                             float* __restrict__ chan) {
+    constexpr int E = OvVec<T>::N, RA = 4;
+    __shared__ float2 cs[OV_GN_MAX_CB(E)];
+    __shared__ float2 st[OV_GN_MAX_CB(E)];
+    const OvGnPlace q = ov_gn_place(p, t, MODE == 1);
+    const int tid = threadIdx.x, ty = tid / t.tx, tx = tid - ty * t.tx;
+    const bool on = ty < t.ty;
+    const int cnt = on ? min(q.cb - tx * E, E) : 0;
+    const int64_t row0 = (int64_t)q.n * p.S;
+    const T* xc = x + q.c0 + tx * E;
+    const T* dc = dy + q.c0 + tx * E;
+    float mu[E], rr_[E], w[E], b[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const int c = max(min(tx * E + k, q.cb - 1), 0);
+        const int64_t gi = (int64_t)q.n * p.groups + q.g0 + c / p.cg;
+        mu[k] = mean[gi];
+        rr_[k] = rstd[gi];
+        w[k] = ov_gn_param(p.w, p.wtype, q.c0 + c, 1.f);
+        b[k] = ov_gn_param(p.b, p.wtype, q.c0 + c, 0.f);
+    }
+    // xhat and dv of one row
+    auto grad = [&](int64_t row, float (&v)[E], float (&d)[E]) {
+        ov_gn_drop<E>(p, row, q.c0 + tx * E, d);
+        float a[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            v[k] = (v[k] - mu[k]) * rr_[k];
+            a[k] = v[k] * w[k] + b[k];
+        }
+        ov_act_grad<E>(a, p.act);
+#pragma unroll
+        for (int k = 0; k < E; ++k) d[k] = d[k] == 0.f ? 0.f : d[k] * a[k];
+    };
+    if (MODE != 1) {
+        float sb[E], sw[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) sb[k] = sw[k] = 0.f;
+        if (cnt > 0)
+            for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
+                float v[RA][E], d[RA][E];
+#pragma unroll
+                for (int i = 0; i < RA; ++i) {
+                    const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C;
+                    ov_gn_load<T>(xc + o, cnt, v[i]);
+                    ov_gn_load<T>(dc + o, cnt, d[i]);
+                }
+#pragma unroll
+                for (int i = 0; i < RA; ++i) {
+                    if (r + i * t.ty >= q.r1) break;
+                    grad(row0 + r + i * t.ty, v[i], d[i]);
+#pragma unroll
+                    for (int k = 0; k < E; ++k) {
+                        sb[k] += d[i][k];
+                        sw[k] += d[i][k] * v[i][k];
+                    }
+                }
+            }
+        if (on)
+#pragma unroll
+            for (int k = 0; k < E; ++k) cs[ty * t.tx * E + tx * E + k] = make_float2(sb[k], sw[k]);
+        __syncthreads();
+        const int64_t R = (int64_t)p.N * t.chunks, ro = (int64_t)q.n * t.chunks + q.chunk;
+        for (int c = tid; c < q.cb; c += 256) {
+            float a = 0.f, e = 0.f;
+            for (int k = 0; k < t.ty; ++k) {
+                const float2 v = cs[k * t.tx * E + c];
+                a += v.x;
+                e += v.y;
+            }
+            if (chan) {
+                chan[ro * p.C + q.c0 + c] = e;
+                chan[(R + ro) * p.C + q.c0 + c] = a;
+            }
+            const float wc = ov_gn_param(p.w, p.wtype, q.c0 + c, 1.f);
+            st[c] = make_float2(a * wc, e * wc);
+        }
+        __syncthreads();
+        for (int g = tid; g < q.ng; g += 256) {
+            float a = 0.f, e = 0.f;
+            for (int k = 0; k < p.cg; ++k) {
+                const float2 v = st[g * p.cg + k];
+                a += v.x;
+                e += v.y;
+            }
+            if (MODE == 0) reinterpret_cast<float2*>(t.part)[ro * p.groups + q.g0 + g] = make_float2(a, e);
+            else {
+                const float total = (float)((int64_t)p.S * p.cg);
+                cs[g] = make_float2(a / total, e / total);
+            }
+        }
+        if (MODE == 0) return;
+        __syncthreads();
+    } else {
+        ov_gn_gather<false>(p, t, q, cs);
+    }
+    if (cnt <= 0) return;
+    float s1[E], s2[E];
+#pragma unroll
+    for (int k = 0; k < E; ++k) {
+        const float2 v = cs[min(tx * E + k, q.cb - 1) / p.cg];
+        s1[k] = v.x;
+        s2[k] = v.y;
+    }
+    for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
+        float v[RA][E], d[RA][E];
+#pragma unroll
+        for (int i = 0; i < RA; ++i) {
+            const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C;
+            ov_gn_load<T>(xc + o, cnt, v[i]);
+            ov_gn_load<T>(dc + o, cnt, d[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < RA; ++i) {
+            const int rr = r + i * t.ty;
+            if (rr >= q.r1) break;
+            grad(row0 + rr, v[i], d[i]);
+#pragma unroll
+            for (int k = 0; k < E; ++k) d[i][k] = rr_[k] * (d[i][k] * w[k] - s1[k] - v[i][k] * s2[k]);
+            ov_gn_store<T>(dx + (row0 + rr) * p.C + q.c0 + tx * E, cnt, d[i]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------- any shape: groups too wide for the forms above
+// one workgroup per (sample, group), everything re-read from the cache
+template <typename T>
+__global__ __launch_bounds__(1024) void ov_gn_any_fwd_kernel(const T* __restrict__ x, const OvGn p, T* __restrict__ y, float* __restrict__ mean,
+                                                             float* __restrict__ rstd) {
     __shared__ float red[16];
     const int64_t n = blockIdx.x / p.groups;
     const int g = blockIdx.x % p.groups;
-    const int64_t cnt = (int64_t)p.S * p.cg;
-    const T* xb = x + n * p.S * p.C + g * p.cg;
+    const float cnt = (float)((int64_t)p.S * p.cg);
+    const int64_t base = n * p.S * p.C + (int64_t)g * p.cg;
     float s = 0.f;
-    for (int64_t i = threadIdx.x; i < cnt; i += 256) s += ov_to_f<T>(xb[i / p.cg * p.C + i % p.cg]);
-    const float mu = ov_block_sum(s, red) / (float)cnt;
+    for (int r = 0; r < p.S; ++r)
+        for (int c = threadIdx.x; c < p.cg; c += 1024) s += ov_to_f<T>(x[base + (int64_t)r * p.C + c]);
+    const float mu = ov_block_sum(s, red) / cnt;
     s = 0.f;
-    for (int64_t i = threadIdx.x; i < cnt; i += 256) {
-        const float d = ov_to_f<T>(xb[i / p.cg * p.C + i % p.cg]) - mu;
-        s += d * d;
-    }
-    const float r = 1.f / sqrtf(ov_block_sum(s, red) / (float)cnt + p.eps);
-    for (int64_t i = threadIdx.x; i < cnt; i += 256) {
-        const int64_t row = n * p.S + i / p.cg;
-        const int c = g * p.cg + (int)(i % p.cg);
-        const float v = (ov_to_f<T>(x[row * p.C + c]) - mu) * r * ov_gn_param(p.w, p.wtype, c, 1.f) + ov_gn_param(p.b, p.wtype, c, 0.f);
-        y[row * p.C + c] = ov_from_f<T>(ov_gn_kept(p, row, c) ? ov_act(v, p.act) * p.drop.scale : 0.f);
-    }
-    if (threadIdx.x == 0) { mean[blockIdx.x] = mu; rstd[blockIdx.x] = r; }
+    for (int r = 0; r < p.S; ++r)
+        for (int c = threadIdx.x; c < p.cg; c += 1024) {
+            const float d = ov_to_f<T>(x[base + (int64_t)r * p.C + c]) - mu;
+            s += d * d;
+        }
+    const float rs = 1.f / sqrtf(ov_block_sum(s, red) / cnt + p.eps);
+    for (int r = 0; r < p.S; ++r)
+        for (int c = threadIdx.x; c < p.cg; c += 1024) {
+            const int64_t o = base + (int64_t)r * p.C + c;
+            const int ch = g * p.cg + c;
+            float v[1] = {(ov_to_f<T>(x[o]) - mu) * rs * ov_gn_param(p.w, p.wtype, ch, 1.f) + ov_gn_param(p.b, p.wtype, ch, 0.f)};
+            ov_act<1>(v, p.act);
+            ov_gn_drop<1>(p, n * p.S + r, ch, v);
+            y[o] = ov_from_f<T>(v[0]);
+        }
+    if (threadIdx.x == 0) { mean[blockIdx.x] = mu; rstd[blockIdx.x] = rs; }
 }
 
 template <typename T>
-__device__ __forceinline__ float ov_gn_dv(const OvGn& p, const T* x, const T* dy, int64_t row, int c, float mu, float r, float* xhat) {
-    *xhat = (ov_to_f<T>(x[row * p.C + c]) - mu) * r;
-    if (!ov_gn_kept(p, row, c)) return 0.f;
-    const float v = *xhat * ov_gn_param(p.w, p.wtype, c, 1.f) + ov_gn_param(p.b, p.wtype, c, 0.f);
-    return ov_to_f<T>(dy[row * p.C + c]) * p.drop.scale * ov_act_grad(v, p.act);
+__device__ __forceinline__ float ov_gn_any_dv(const OvGn& p, const T* x, const T* dy, int64_t row, int c, float mu, float r, float* xhat) {
+    const int64_t o = row * p.C + c;
+    *xhat = (ov_to_f<T>(x[o]) - mu) * r;
+    float d[1] = {ov_to_f<T>(dy[o])}, a[1] = {*xhat * ov_gn_param(p.w, p.wtype, c, 1.f) + ov_gn_param(p.b, p.wtype, c, 0.f)};
+    ov_gn_drop<1>(p, row, c, d);
+    ov_act_grad<1>(a, p.act);
+    return d[0] == 0.f ? 0.f : d[0] * a[0];
 }
 
 template <typename T>
-__global__ __launch_bounds__(256) void ov_gn_bwd_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p,
-                                                           const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx) {
+__global__ __launch_bounds__(1024) void ov_gn_any_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p,
+                                                            const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx) {
     __shared__ float red[16];
     const int64_t n = blockIdx.x / p.groups;
     const int g = blockIdx.x % p.groups;
-    const int64_t cnt = (int64_t)p.S * p.cg;
-    const float mu = mean[blockIdx.x], r = rstd[blockIdx.x];
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t i = threadIdx.x; i < cnt; i += 256) {
-        const int c = g * p.cg + (int)(i % p.cg);
-        float xh;
-        const float e = ov_gn_dv(p, x, dy, n * p.S + i / p.cg, c, mu, r, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
-        s1 += e;
-        s2 += e * xh;
-    }
-    s1 = ov_block_sum(s1, red) / (float)cnt;
-    s2 = ov_block_sum(s2, red) / (float)cnt;
-    for (int64_t i = threadIdx.x; i < cnt; i += 256) {
-        const int64_t row = n * p.S + i / p.cg;
-        const int c = g * p.cg + (int)(i % p.cg);
-        float xh;
-        const float e = ov_gn_dv(p, x, dy, row, c, mu, r, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
-        dx[row * p.C + c] = ov_from_f<T>(r * (e - s1 - xh * s2));
-    }
+    const float cnt = (float)((int64_t)p.S * p.cg);
+    const float mu = mean[blockIdx.x], rs = rstd[blockIdx.x];
+    float s1 = 0.f, s2 = 0.f, xh;
+    for (int r = 0; r < p.S; ++r)
+        for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) {
+            const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
+            s1 += e;
+            s2 += e * xh;
+        }
+    s1 = ov_block_sum(s1, red) / cnt;
+    s2 = ov_block_sum(s2, red) / cnt;
+    for (int r = 0; r < p.S; ++r)
+        for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) {
+            const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
+            dx[(n * p.S + r) * p.C + c] = ov_from_f<T>(rs * (e - s1 - xh * s2));
+        }
 }
 
-// one workgroup per channel
+// sums over the rows for 64 channels: a wave's lanes along the channels, 16 waves along the rows
 template <typename T>
-__global__ __launch_bounds__(256) void ov_gn_bwd_param_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p,
-                                                              const float* __restrict__ mean, const float* __restrict__ rstd, float* __restrict__ dw,
-                                                              float* __restrict__ db) {
-    __shared__ float red[16];
-    const int c = blockIdx.x, g = c / p.cg;
-    float s1 = 0.f, s2 = 0.f;
-    for (int64_t row = threadIdx.x; row < (int64_t)p.N * p.S; row += 256) {
-        const int64_t k = row / p.S * p.groups + g;
-        float xh;
-        const float dv = ov_gn_dv(p, x, dy, row, c, mean[k], rstd[k], &xh);
-        s1 += dv;
-        s2 += dv * xh;
-    }
-    s1 = ov_block_sum(s1, red);
-    s2 = ov_block_sum(s2, red);
-    if (threadIdx.x == 0) {
-        if (dw) dw[c] = s2;
-        if (db) db[c] = s1;
+__global__ __launch_bounds__(1024) void ov_gn_any_param_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p,
+                                                               const float* __restrict__ mean, const float* __restrict__ rstd,
+                                                               float* __restrict__ dw, float* __restrict__ db) {
+    __shared__ float2 red[16][64];
+    const int lane = ov_lane(), wave = ov_wave_id(), c = blockIdx.x * 64 + lane;
+    float2 s = {0.f, 0.f};
+    if (c < p.C)
+        for (int64_t row = wave; row < (int64_t)p.N * p.S; row += 16) {
+            const int64_t k = row / p.S * p.groups + c / p.cg;
+            float xh;
+            const float dv = ov_gn_any_dv(p, x, dy, row, c, mean[k], rstd[k], &xh);
+            s.x += dv * xh;
+            s.y += dv;
+        }
+    red[wave][lane] = s;
+    __syncthreads();
+    if (wave == 0 && c < p.C) {
+        for (int k = 1; k < 16; ++k) { s.x += red[k][lane].x; s.y += red[k][lane].y; }
+        if (dw) dw[c] = s.x;
+        if (db) db[c] = s.y;
     }
 }
 
@@ -154,9 +714,119 @@ static int ov_gn_check(const char* what, int32_t dtype, int32_t N, int32_t S, in
     return ONTOVAE_OK;
 }
 
+// ---------------------------------------------------------------- host
+enum { OV_GN_ROW, OV_GN_TILE, OV_GN_TILE1, OV_GN_ANY };
+struct OvGnPlan {
+    int form;
+    int lpg, nv, RS;         // OV_GN_ROW
+    OvGnTile t;              // OV_GN_TILE (two launches), OV_GN_TILE1 (one)
+    int64_t part_floats, chan_floats, chan_rows;
+};
+
+static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool backward) {
+    OvGnPlan q{};
+    const int E = dtype == ONTOVAE_F32 ? 4 : 8, cg = C / groups;
+    const int pieces = (cg + E - 1) / E;
+    if (S == 1 && pieces <= 1024 * (16 / E)) {
+        q.form = OV_GN_ROW;
+        if (pieces <= 64) {
+            q.nv = 1;
+            q.lpg = 8;
+            while (q.lpg < pieces) q.lpg *= 2;
+        } else {
+            q.lpg = pieces <= 64 * (16 / E) ? 64 : pieces <= 256 * (16 / E) ? 256 : 1024;
+            q.nv = 16 / E;
+        }
+        // enough slots for four workgroups of 256 threads per CU; the gradient sums of a slot are a row of C floats to write and
+        // read again, so a slot takes at least 8 samples there
+        const int64_t want = std::max<int64_t>(262144 / ((int64_t)groups * q.lpg), 1);
+        q.RS = (int)std::min<int64_t>(want, backward ? std::max((N + 7) / 8, std::min(N, 16)) : N);
+        q.chan_rows = q.RS;
+        q.chan_floats = backward ? 2LL * q.RS * C : 0;
+        return q;
+    }
+    const int max_cb = 256 * E;
+    if (S > 1 && cg <= max_cb) {
+        OvGnTile& t = q.t;
+        t.gb = std::min(groups, max_cb / cg);
+        t.nblk = (groups + t.gb - 1) / t.gb;
+        t.gb = (groups + t.nblk - 1) / t.nblk;
+        t.nblk = (groups + t.gb - 1) / t.gb;
+        t.tx = (t.gb * cg + E - 1) / E;
+        t.ty = std::min(256 / t.tx, S);
+        const int64_t bytes = (int64_t)S * t.gb * cg * (dtype == ONTOVAE_F32 ? 4 : 2);
+        const int64_t wg = (int64_t)N * t.nblk;
+        if (bytes <= 65536) {
+            q.form = OV_GN_TILE1;
+            t.chunks = 1;
+            t.rows = S;
+        } else {
+            q.form = OV_GN_TILE;
+            const int most = (S + t.ty * 8 - 1) / (t.ty * 8);
+            t.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, (2048 + wg - 1) / wg));
+            t.rows = (S + t.chunks - 1) / t.chunks;
+            t.chunks = (S + t.rows - 1) / t.rows;
+            q.part_floats = 2LL * N * t.chunks * groups;
+        }
+        q.chan_rows = (int64_t)N * t.chunks;
+        q.chan_floats = backward ? 2 * q.chan_rows * C : 0;
+        return q;
+    }
+    q.form = OV_GN_ANY;
+    return q;
+}
+
+static int64_t ov_gn_ws(const OvGnPlan& q) { return ((q.part_floats + 63) / 64 * 64 + q.chan_floats) * 4; }
+
 extern "C" int64_t ontovae_group_norm_act_workspace_bytes(int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, int32_t backward) {
-    (void)dtype; (void)N; (void)S; (void)C; (void)groups; (void)backward;
-    return 0;
+    if (N < 1 || S < 1 || C < 1 || groups < 1 || C % groups || dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) return 0;
+    return ov_gn_ws(ov_gn_plan(dtype, N, S, C, groups, backward != 0));
+}
+
+static int ov_gn_ready(const char* what, const OvGn& p, const OvGnPlan& q, const void* ws, int64_t bytes) {
+    const int64_t need = ov_gn_ws(q);
+    if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255))) {
+        ontovae_set_error("%s: workspace of %lld bytes, 256-B aligned, needed", what, (long long)need);
+        return ONTOVAE_EINVAL;
+    }
+    const int64_t wg = q.form == OV_GN_ROW ? ((int64_t)q.RS * p.groups * q.lpg + 255) / 256
+                       : q.form == OV_GN_ANY ? (int64_t)p.N * p.groups : (int64_t)p.N * q.t.chunks * q.t.nblk;
+    if (wg > INT32_MAX) { ontovae_set_error("%s: N = %d with %d groups: too many workgroups", what, p.N, p.groups); return ONTOVAE_EINVAL; }
+    return ONTOVAE_OK;
+}
+
+#define OV_GN_ROW_SWITCH(GO)                                                                   \
+    switch (q.lpg) {                                                                           \
+        case 8: GO(8, 1); break;                                                               \
+        case 16: GO(16, 1); break;                                                             \
+        case 32: GO(32, 1); break;                                                             \
+        case 64: if (q.nv == 1) { GO(64, 1); } else { GO(64, NVX); } break;                    \
+        case 256: GO(256, NVX); break;                                                         \
+        default: GO(1024, NVX); break;                                                         \
+    }
+
+template <typename T>
+static void ov_gn_fwd_launch(const void* x, const OvGn& p, OvGnPlan q, void* y, float* mean, float* rstd, void* ws, hipStream_t st) {
+    const T* xt = static_cast<const T*>(x);
+    T* yt = static_cast<T*>(y);
+    q.t.part = static_cast<float*>(ws);
+    constexpr int NVX = 16 / OvVec<T>::N;
+    if (q.form == OV_GN_ROW) {
+#define OV_GO(L, V)                                                                                                                              \
+    hipLaunchKernelGGL((ov_gn_row_fwd_kernel<T, L, V>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
+                       dim3(L < 256 ? 256 : L), 0, st, xt, p, q.RS, yt, mean, rstd)
+        OV_GN_ROW_SWITCH(OV_GO)
+#undef OV_GO
+    } else if (q.form == OV_GN_ANY) {
+        hipLaunchKernelGGL(ov_gn_any_fwd_kernel<T>, dim3((unsigned)((int64_t)p.N * p.groups)), dim3(1024), 0, st, xt, p, yt, mean, rstd);
+    } else {
+        const dim3 grid((unsigned)((int64_t)p.N * q.t.chunks * q.t.nblk));
+        if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 2>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+        else {
+            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 0>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 1>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+        }
+    }
 }
 
 extern "C" int ontovae_group_norm_act(const void* x, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, const void* weight,
@@ -167,24 +837,54 @@ extern "C" int ontovae_group_norm_act(const void* x, int32_t dtype, int32_t N, i
     if (rc) return rc;
     if (N == 0 || S == 0 || C == 0) return ONTOVAE_OK;
     if (!x || !y || !mean || !rstd) { ontovae_set_error("group_norm_act: NULL argument"); return ONTOVAE_EINVAL; }
-    (void)workspace; (void)workspace_bytes;
+    const OvGnPlan q = ov_gn_plan(dtype, N, S, C, groups, false);
+    if ((rc = ov_gn_ready("group_norm_act", p, q, workspace, workspace_bytes))) return rc;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    const dim3 grid((unsigned)(N * groups));
     switch (dtype) {
-        case ONTOVAE_F32: hipLaunchKernelGGL(ov_gn_fwd_kernel<float>, grid, dim3(256), 0, st, (const float*)x, p, (float*)y, mean, rstd); break;
-        case ONTOVAE_BF16: hipLaunchKernelGGL(ov_gn_fwd_kernel<ov_bf>, grid, dim3(256), 0, st, (const ov_bf*)x, p, (ov_bf*)y, mean, rstd); break;
-        default: hipLaunchKernelGGL(ov_gn_fwd_kernel<ov_hf>, grid, dim3(256), 0, st, (const ov_hf*)x, p, (ov_hf*)y, mean, rstd); break;
+        case ONTOVAE_F32: ov_gn_fwd_launch<float>(x, p, q, y, mean, rstd, workspace, st); break;
+        case ONTOVAE_BF16: ov_gn_fwd_launch<ov_bf>(x, p, q, y, mean, rstd, workspace, st); break;
+        default: ov_gn_fwd_launch<ov_hf>(x, p, q, y, mean, rstd, workspace, st); break;
     }
     OV_OPS_LAUNCH_CHECK("group_norm_act");
     return ONTOVAE_OK;
 }
 
 template <typename T>
-static void ov_gn_bwd_launch(const void* dy, const void* x, const OvGn& p, const float* mean, const float* rstd, void* dx, float* dw, float* db,
-                             hipStream_t st) {
-    if (p.N > 0)
-        hipLaunchKernelGGL(ov_gn_bwd_dx_kernel<T>, dim3((unsigned)(p.N * p.groups)), dim3(256), 0, st, (const T*)dy, (const T*)x, p, mean, rstd, (T*)dx);
-    if (dw || db) hipLaunchKernelGGL(ov_gn_bwd_param_kernel<T>, dim3(p.C), dim3(256), 0, st, (const T*)dy, (const T*)x, p, mean, rstd, dw, db);
+static void ov_gn_bwd_launch(const void* dy, const void* x, const OvGn& p, OvGnPlan q, const float* mean, const float* rstd, void* dx, float* dw,
+                             float* db, void* ws, hipStream_t st) {
+    const T* xt = static_cast<const T*>(x);
+    const T* dt = static_cast<const T*>(dy);
+    T* dxt = static_cast<T*>(dx);
+    q.t.part = static_cast<float*>(ws);
+    float* chan = dw || db ? static_cast<float*>(ws) + (q.part_floats + 63) / 64 * 64 : nullptr;
+    constexpr int NVX = 16 / OvVec<T>::N;
+    if (q.form == OV_GN_ANY) {
+        hipLaunchKernelGGL(ov_gn_any_dx_kernel<T>, dim3((unsigned)((int64_t)p.N * p.groups)), dim3(1024), 0, st, dt, xt, p, mean, rstd, dxt);
+        if (dw || db) hipLaunchKernelGGL(ov_gn_any_param_kernel<T>, dim3((p.C + 63) / 64), dim3(1024), 0, st, dt, xt, p, mean, rstd, dw, db);
+        return;
+    }
+    if (q.form == OV_GN_ROW) {
+#define OV_GO(L, V)                                                                                                                              \
+    hipLaunchKernelGGL((ov_gn_row_bwd_kernel<T, L, V>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
+                       dim3(L < 256 ? 256 : L), 0, st, dt, xt, p, q.RS, mean, rstd, dxt, chan)
+        OV_GN_ROW_SWITCH(OV_GO)
+#undef OV_GO
+    } else {
+        const dim3 grid((unsigned)((int64_t)p.N * q.t.chunks * q.t.nblk));
+        if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 2>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
+        else {
+            hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 0>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
+            hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 1>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
+        }
+    }
+    if (chan) hipLaunchKernelGGL(ov_gn_param_kernel, dim3((p.C + 15) / 16, 2), dim3(256), 0, st, chan, q.chan_rows, p.C, dw, db);
+}
+
+__global__ __launch_bounds__(256) void ov_gn_zero_kernel(float* dw, float* db, int C) {
+    for (int c = blockIdx.x * 256 + threadIdx.x; c < C; c += gridDim.x * 256) {
+        if (dw) dw[c] = 0.f;
+        if (db) db[c] = 0.f;
+    }
 }
 
 extern "C" int ontovae_group_norm_act_backward(const void* dy, const void* x, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups,
@@ -195,15 +895,19 @@ extern "C" int ontovae_group_norm_act_backward(const void* dy, const void* x, in
     int rc = ov_gn_check("group_norm_act_backward", dtype, N, S, C, groups, weight, bias, wdtype, 0.f, act, drop, seed, offset, &p);
     if (rc) return rc;
     if (C == 0) return ONTOVAE_OK;
-    const bool none = N == 0 || S == 0;
-    if (!none && (!dy || !x || !mean || !rstd || !dx)) { ontovae_set_error("group_norm_act_backward: NULL argument"); return ONTOVAE_EINVAL; }
-    (void)workspace; (void)workspace_bytes;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
-    if (none) p.N = 0;
+    if (N == 0 || S == 0) {
+        if (dweight || dbias) hipLaunchKernelGGL(ov_gn_zero_kernel, dim3(std::min((C + 255) / 256, 256)), dim3(256), 0, st, dweight, dbias, C);
+        OV_OPS_LAUNCH_CHECK("group_norm_act_backward");
+        return ONTOVAE_OK;
+    }
+    if (!dy || !x || !mean || !rstd || !dx) { ontovae_set_error("group_norm_act_backward: NULL argument"); return ONTOVAE_EINVAL; }
+    const OvGnPlan q = ov_gn_plan(dtype, N, S, C, groups, true);
+    if ((rc = ov_gn_ready("group_norm_act_backward", p, q, workspace, workspace_bytes))) return rc;
     switch (dtype) {
-        case ONTOVAE_F32: ov_gn_bwd_launch<float>(dy, x, p, mean, rstd, dx, dweight, dbias, st); break;
-        case ONTOVAE_BF16: ov_gn_bwd_launch<ov_bf>(dy, x, p, mean, rstd, dx, dweight, dbias, st); break;
-        default: ov_gn_bwd_launch<ov_hf>(dy, x, p, mean, rstd, dx, dweight, dbias, st); break;
+        case ONTOVAE_F32: ov_gn_bwd_launch<float>(dy, x, p, q, mean, rstd, dx, dweight, dbias, workspace, st); break;
+        case ONTOVAE_BF16: ov_gn_bwd_launch<ov_bf>(dy, x, p, q, mean, rstd, dx, dweight, dbias, workspace, st); break;
+        default: ov_gn_bwd_launch<ov_hf>(dy, x, p, q, mean, rstd, dx, dweight, dbias, workspace, st); break;
     }
     OV_OPS_LAUNCH_CHECK("group_norm_act_backward");
     return ONTOVAE_OK;
