@@ -28,6 +28,24 @@ __device__ __forceinline__ float ov_gn_param(const void* p, int wtype, int c, fl
     return (float)static_cast<const ov_hf*>(p)[c];
 }
 
+// E neighbours of a parameter vector from channel c on, cnt of them valid (the rest 0)
+template <int E>
+__device__ __forceinline__ void ov_gn_params(const void* p, int wtype, int c, int cnt, float none, float (&f)[E]) {
+#pragma unroll
+    for (int j = 0; j < E; ++j) f[j] = j < cnt ? none : 0.f;
+    if (!p) return;
+    if (wtype == ONTOVAE_F32) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[j] = static_cast<const float*>(p)[c + min(j, max(cnt - 1, 0))];
+    } else if (wtype == ONTOVAE_BF16) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[j] = (float)static_cast<const ov_bf*>(p)[c + min(j, max(cnt - 1, 0))];
+    } else {
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[j] = (float)static_cast<const ov_hf*>(p)[c + min(j, max(cnt - 1, 0))];
+    }
+}
+
 // sigma(v) and what silu and gelu and their slopes need of exp and erf
 __device__ __forceinline__ float ov_sigmoid(float v) { return __builtin_amdgcn_rcpf(1.f + __expf(-v)); }
 
@@ -61,17 +79,16 @@ __device__ __forceinline__ void ov_act_grad(float (&v)[E], int act) {
             const float s = ov_sigmoid(v[j]);
             v[j] = s * (1.f + v[j] * (1.f - s));
         }
-    } else {
+    } else if (act == ONTOVAE_ACT_GELU) {
 #pragma unroll
         for (int j = 0; j < E; ++j)
             v[j] = 0.5f * (1.f + erff(v[j] * 0.70710678118654752f)) + v[j] * __expf(-0.5f * v[j] * v[j]) * 0.39894228040143268f;
     }
 }
 
-// dropout of E neighbours of a row from column c on (E <= 8: at most two of the row's blocks of eight): f[j] v[j], f = 0 or scale
+// the kept ones of E neighbours of a row from column c on (E <= 8: at most two of the row's blocks of eight), bit j = element j
 template <int E>
-__device__ __forceinline__ void ov_gn_drop(const OvGn& p, int64_t row, int c, float (&v)[E]) {
-    if (p.drop.t == 0) return;
+__device__ __forceinline__ uint32_t ov_gn_kept(const OvGn& p, int64_t row, int c) {
     const uint64_t block = (uint64_t)row * ((p.C + 7) / 8) + (c >> 3);
     const int o = c & 7;
     OvPhilox r = ov_drop_draw(p.drop, block);
@@ -83,22 +100,41 @@ __device__ __forceinline__ void ov_gn_drop(const OvGn& p, int64_t row, int c, fl
 #pragma unroll
         for (int j = 0; j < 8; ++j) m |= (ov_drop_kept(p.drop, r, j) ? 1u : 0u) << (8 + j);
     }
+    return m >> o;
+}
+template <int E>
+__device__ __forceinline__ void ov_gn_drop(const OvGn& p, int64_t row, int c, float (&v)[E]) {
+    if (p.drop.t == 0) return;
+    const uint32_t m = ov_gn_kept<E>(p, row, c);
 #pragma unroll
-    for (int j = 0; j < E; ++j) v[j] = (m >> (o + j)) & 1 ? v[j] * p.drop.scale : 0.f;
+    for (int j = 0; j < E; ++j) v[j] = (m >> j) & 1 ? v[j] * p.drop.scale : 0.f;
+}
+// dv = dy D act'(v): v comes in, dv goes out; a dropped place gives 0 whatever dy and act' are
+template <int E>
+__device__ __forceinline__ void ov_gn_dv(const OvGn& p, int64_t row, int c, const float (&dy)[E], float (&v)[E]) {
+    ov_act_grad<E>(v, p.act);
+#pragma unroll
+    for (int j = 0; j < E; ++j) v[j] *= dy[j];
+    ov_gn_drop<E>(p, row, c, v);
 }
 
-// 16 bytes of a row (cnt of them valid: a group's or a row's last piece), as floats; nothing is read behind cnt
+// 16 bytes from element `off` of x [total], whatever of them belongs to the reader: a piece that ends inside its 16 bytes reads
+// on into its neighbour.  The load is unconditional (a branch around it would make the compiler wait for every load by itself);
+// the last pieces of the tensor, which have no neighbour, are read from further in front, and ov_gn_floats fetches their
+// elements one by one.
 template <typename T>
-__device__ __forceinline__ void ov_gn_load(const T* x, int cnt, float (&f)[OvVec<T>::N]) {
+__device__ __forceinline__ void ov_gn_raw(const T* x, int64_t total, int64_t off, OvVec<T>& v) {
+    v.load(x + min(off, total - OvVec<T>::N));
+}
+template <typename T>
+__device__ __forceinline__ void ov_gn_floats(const T* x, int64_t total, int64_t off, const OvVec<T>& v, float (&f)[OvVec<T>::N]) {
     constexpr int E = OvVec<T>::N;
-    OvVec<T> v;
-    if (cnt >= E) v.load(x);
-    else {
-#pragma unroll
-        for (int j = 0; j < E; ++j) v.e[j] = j < cnt ? x[j] : (T)0.f;
-    }
 #pragma unroll
     for (int j = 0; j < E; ++j) f[j] = ov_to_f<T>(v.e[j]);
+    if (off > total - E) {
+#pragma unroll
+        for (int j = 0; j < E; ++j) f[j] = off + j < total ? ov_to_f<T>(x[off + j]) : 0.f;
+    }
 }
 template <typename T>
 __device__ __forceinline__ void ov_gn_store(T* y, int cnt, const float (&f)[OvVec<T>::N]) {
@@ -121,60 +157,90 @@ __device__ __forceinline__ void ov_gn_store_f(float* y, int cnt, const float (&f
         if (j < cnt) y[j] = f[j];
 }
 
-// sum over the LPG threads of a group: lanes of a wave, or the workgroup
+// LIGHT kernels: no dropout and no gelu, whose code (two Philox draws, erff) sets the register count of the others
+template <bool LIGHT>
+__device__ __forceinline__ OvGn ov_gn_light(OvGn p) {
+    if (LIGHT) {
+        p.drop.t = 0;
+        p.act = min(p.act, (int)ONTOVAE_ACT_SILU);
+    }
+    return p;
+}
+
+// sum over the LPG threads of a group, in every one of them: lanes of a wave (DPP moves inside 16 lanes), or the workgroup
 template <int LPG>
 __device__ __forceinline__ float ov_gn_sum(float v, float* red) {
-    if (LPG <= 64) {
-#pragma unroll
-        for (int o = LPG / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
-        return v;
-    }
-    return ov_block_sum(v, red);
+    if (LPG > 64) return ov_block_sum(v, red);
+    v += ov_dpp<0xB1, 0xF>(v);                           // quad_perm [1,0,3,2]
+    v += ov_dpp<0x4E, 0xF>(v);                           // quad_perm [2,3,0,1]
+    v += ov_dpp<0x141, 0xF>(v);                          // row_half_mirror: 8 lanes
+    if (LPG >= 16) v += ov_dpp<0x140, 0xF>(v);           // row_mirror: 16 lanes
+    if (LPG >= 32) v += __shfl_xor(v, 16, 64);
+    if (LPG >= 64) v += __shfl_xor(v, 32, 64);
+    return v;
 }
 
 // ---------------------------------------------------------------- S = 1: a group is one contiguous run of cg elements
 // LPG threads hold a group in registers, NV pieces of 16 bytes each; a slot of LPG threads keeps its group and walks the
 // samples rs, rs + RS, ...: weight and bias (and the sums of their gradients) stay in registers.  Neighbouring slots take
 // neighbouring groups, so a workgroup reads contiguous memory.  One read of x (and dy), one write: bound by memory.
-template <typename T, int LPG, int NV>
-__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(const T* __restrict__ x, const OvGn p, int RS, T* __restrict__ y,
+// The next sample is requested before the current one is reduced.
+template <typename T, int LPG, int NV, bool LIGHT>
+__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(const T* __restrict__ x, const OvGn p_, int RS, T* __restrict__ y,
                                                                              float* __restrict__ mean, float* __restrict__ rstd) {
+    const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvVec<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
     __shared__ float red[16];
     const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
-    const int j = threadIdx.x % LPG, g = (int)(slot % p.groups), rs = (int)(slot / p.groups);
+    const int j = threadIdx.x % LPG, rs = (int)(slot / p.groups), g = (int)(slot - (int64_t)rs * p.groups);
     if (rs >= RS) return;
-    float w[NV][E], b[NV][E];
+    const int64_t gc = (int64_t)g * p.cg, step = (int64_t)RS * p.C;
+    const int64_t total = (int64_t)p.N * p.C;
+    const bool ragged = p.cg % E != 0;
+    int64_t at = (int64_t)rs * p.C + gc;
+    OvVec<T> raw[NV];
     int cnt[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int o = (j + i * LPG) * E;
         cnt[i] = min(p.cg - o, E);
-#pragma unroll
-        for (int k = 0; k < E; ++k) {
-            w[i][k] = k < cnt[i] ? ov_gn_param(p.w, p.wtype, g * p.cg + o + k, 1.f) : 0.f;
-            b[i][k] = k < cnt[i] ? ov_gn_param(p.b, p.wtype, g * p.cg + o + k, 0.f) : 0.f;
-        }
+        ov_gn_raw<T>(x, total, at + o, raw[i]);
     }
+    float w[NV][E], b[NV][E];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if (cnt[i] > 0) {
+            ov_gn_params<E>(p.w, p.wtype, (int)gc + (j + i * LPG) * E, cnt[i], 1.f, w[i]);
+            ov_gn_params<E>(p.b, p.wtype, (int)gc + (j + i * LPG) * E, cnt[i], 0.f, b[i]);
+        }
     const float len = (float)p.cg;
     for (int n = rs; n < p.N; n += RS) {
-        const int64_t base = (int64_t)n * p.C + g * p.cg;
         float v[NV][E];
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) ov_gn_load<T>(x + base + (j + i * LPG) * E, cnt[i], v[i]);
+        for (int i = 0; i < NV; ++i) {
+            ov_gn_floats<T>(x, total, at + (j + i * LPG) * E, raw[i], v[i]);
+            if (ragged || NV > 1 || LPG * E > p.cg) {     // not every piece is whole
 #pragma unroll
-        for (int i = 0; i < NV; ++i)
+                for (int k = 0; k < E; ++k) v[i][k] = k < cnt[i] ? v[i][k] : 0.f;
+            }
 #pragma unroll
             for (int k = 0; k < E; ++k) s += v[i][k];
+        }
+        const int64_t here = at;
+        at += step;
+        if (n + RS < p.N) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) ov_gn_raw<T>(x, total, at + (j + i * LPG) * E, raw[i]);
+        }
         const float mu = ov_gn_sum<LPG>(s, red) / len;
         s = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                const float d = v[i][k] - mu;
-                s += k < cnt[i] ? d * d : 0.f;
+                v[i][k] = k < cnt[i] ? v[i][k] - mu : 0.f;
+                s += v[i][k] * v[i][k];
             }
         const float r = 1.f / sqrtf(ov_gn_sum<LPG>(s, red) / len + p.eps);
 #pragma unroll
@@ -182,10 +248,10 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(co
             if (cnt[i] <= 0) continue;
             const int o = (j + i * LPG) * E;
 #pragma unroll
-            for (int k = 0; k < E; ++k) v[i][k] = (v[i][k] - mu) * r * w[i][k] + b[i][k];
+            for (int k = 0; k < E; ++k) v[i][k] = v[i][k] * r * w[i][k] + b[i][k];
             ov_act<E>(v[i], p.act);
-            ov_gn_drop<E>(p, n, g * p.cg + o, v[i]);
-            ov_gn_store<T>(y + base + o, cnt[i], v[i]);
+            ov_gn_drop<E>(p, n, (int)gc + o, v[i]);
+            ov_gn_store<T>(y + here + o, cnt[i], v[i]);
         }
         if (j == 0) {
             mean[(int64_t)n * p.groups + g] = mu;
@@ -195,57 +261,75 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(co
 }
 
 // part: [2][RS][C]: the slots' sums of dv xhat, then of dv (written for every slot, also one without a sample)
-template <typename T, int LPG, int NV>
-__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p, int RS,
+template <typename T, int LPG, int NV, bool LIGHT>
+__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p_, int RS,
                                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                              T* __restrict__ dx, float* __restrict__ part) {
+    const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvVec<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
     __shared__ float red[16];
     const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
-    const int j = threadIdx.x % LPG, g = (int)(slot % p.groups), rs = (int)(slot / p.groups);
+    const int j = threadIdx.x % LPG, rs = (int)(slot / p.groups), g = (int)(slot - (int64_t)rs * p.groups);
     if (rs >= RS) return;
-    float w[NV][E], b[NV][E], sw[NV][E], sb[NV][E];
+    const int64_t gc = (int64_t)g * p.cg, step = (int64_t)RS * p.C;
+    const int64_t total = (int64_t)p.N * p.C;
+    int64_t at = (int64_t)rs * p.C + gc;
+    OvVec<T> rx[NV], rd[NV];
     int cnt[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
         const int o = (j + i * LPG) * E;
         cnt[i] = min(p.cg - o, E);
+        ov_gn_raw<T>(x, total, at + o, rx[i]);
+        ov_gn_raw<T>(dy, total, at + o, rd[i]);
+    }
+    float mu = mean[(int64_t)rs * p.groups + g], r = rstd[(int64_t)rs * p.groups + g];
+    float w[NV][E], b[NV][E], sw[NV][E], sb[NV][E];
 #pragma unroll
-        for (int k = 0; k < E; ++k) {
-            w[i][k] = k < cnt[i] ? ov_gn_param(p.w, p.wtype, g * p.cg + o + k, 1.f) : 0.f;
-            b[i][k] = k < cnt[i] ? ov_gn_param(p.b, p.wtype, g * p.cg + o + k, 0.f) : 0.f;
-            sw[i][k] = sb[i][k] = 0.f;
+    for (int i = 0; i < NV; ++i) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) w[i][k] = b[i][k] = sw[i][k] = sb[i][k] = 0.f;
+        if (cnt[i] > 0) {
+            ov_gn_params<E>(p.w, p.wtype, (int)gc + (j + i * LPG) * E, cnt[i], 1.f, w[i]);
+            ov_gn_params<E>(p.b, p.wtype, (int)gc + (j + i * LPG) * E, cnt[i], 0.f, b[i]);
         }
     }
     const float len = (float)p.cg;
     for (int n = rs; n < p.N; n += RS) {
-        const int64_t base = (int64_t)n * p.C + g * p.cg;
-        const float mu = mean[(int64_t)n * p.groups + g], r = rstd[(int64_t)n * p.groups + g];
+        const int64_t here = at;
+        const float mu0 = mu, r0 = r;
         float v[NV][E], d[NV][E];
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            ov_gn_load<T>(x + base + (j + i * LPG) * E, cnt[i], v[i]);
-            ov_gn_load<T>(dy + base + (j + i * LPG) * E, cnt[i], d[i]);
+            ov_gn_floats<T>(x, total, at + (j + i * LPG) * E, rx[i], v[i]);
+            ov_gn_floats<T>(dy, total, at + (j + i * LPG) * E, rd[i], d[i]);
+        }
+        at += step;
+        if (n + RS < p.N) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i) {
+                ov_gn_raw<T>(x, total, at + (j + i * LPG) * E, rx[i]);
+                ov_gn_raw<T>(dy, total, at + (j + i * LPG) * E, rd[i]);
+            }
+            mu = mean[(int64_t)(n + RS) * p.groups + g];
+            r = rstd[(int64_t)(n + RS) * p.groups + g];
         }
         float s1 = 0.f, s2 = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
-            if (cnt[i] <= 0) continue;
-            ov_gn_drop<E>(p, n, g * p.cg + (j + i * LPG) * E, d[i]);
             float a[E];
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                v[i][k] = (v[i][k] - mu) * r;
+                v[i][k] = (v[i][k] - mu0) * r0;
                 a[k] = v[i][k] * w[i][k] + b[i][k];
             }
-            ov_act_grad<E>(a, p.act);
+            ov_gn_dv<E>(p, n, (int)gc + (j + i * LPG) * E, d[i], a);
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                if (k >= cnt[i]) { v[i][k] = 0.f; a[k] = 0.f; }
-                const float dv = d[i][k] == 0.f ? 0.f : d[i][k] * a[k];        // a dropped place: 0 whatever act' is
-                sw[i][k] += dv * v[i][k];
-                sb[i][k] += dv;
-                d[i][k] = dv * w[i][k];
+                if (k >= cnt[i]) a[k] = v[i][k] = 0.f;
+                sw[i][k] += a[k] * v[i][k];
+                sb[i][k] += a[k];
+                d[i][k] = a[k] * w[i][k];
                 s1 += d[i][k];
                 s2 += d[i][k] * v[i][k];
             }
@@ -256,14 +340,14 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
         for (int i = 0; i < NV; ++i) {
             if (cnt[i] <= 0) continue;
 #pragma unroll
-            for (int k = 0; k < E; ++k) d[i][k] = r * (d[i][k] - s1 - v[i][k] * s2);
-            ov_gn_store<T>(dx + base + (j + i * LPG) * E, cnt[i], d[i]);
+            for (int k = 0; k < E; ++k) d[i][k] = r0 * (d[i][k] - s1 - v[i][k] * s2);
+            ov_gn_store<T>(dx + here + (j + i * LPG) * E, cnt[i], d[i]);
         }
     }
     if (!part) return;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int64_t o = (int64_t)rs * p.C + g * p.cg + (j + i * LPG) * E;
+        const int64_t o = (int64_t)rs * p.C + gc + (j + i * LPG) * E;
         ov_gn_store_f<E>(part + o, cnt[i], sw[i]);
         ov_gn_store_f<E>(part + (int64_t)RS * p.C + o, cnt[i], sb[i]);
     }
@@ -300,7 +384,7 @@ __global__ __launch_bounds__(256) void ov_gn_param_kernel(const float* __restric
 }
 
 // ---------------------------------------------------------------- S > 1: tiles of rows x channels
-// A workgroup takes rows [r0, r1) of a sample and a block of whole groups (all channels if they fit): 256 threads as TX pieces
+// A workgroup takes a run of a sample's rows and a block of whole groups (all channels if they fit): 256 threads as TX pieces
 // of 16 bytes x TY rows, a thread's channels fixed, so that weight, bias and the per-channel sums stay in registers; channel
 // sums meet in LDS, group sums are sums of channel sums (a piece may hold parts of several groups).
 //   MODE 0: sums of the tile only      MODE 1: the output, from the sums of the sample's tiles
@@ -315,6 +399,10 @@ struct OvGnTile {
 };
 
 struct OvGnPlace { int n, chunk, c0, cb, g0, ng, r0, r1; };
+// rows of tile k
+__device__ __forceinline__ int ov_gn_tile_rows(const OvGn& p, const OvGnTile& t, int k) { return min(t.rows, p.S - k * t.rows); }
+// of these, the rows of thread row ty
+__device__ __forceinline__ int ov_gn_thread_rows(const OvGnTile& t, int rows, int ty) { return (rows - ty + t.ty - 1) / t.ty; }
 __device__ __forceinline__ OvGnPlace ov_gn_place(const OvGn& p, const OvGnTile& t, bool reverse) {
     OvGnPlace q;
     int id = reverse ? gridDim.x - 1 - blockIdx.x : blockIdx.x;
@@ -327,7 +415,7 @@ __device__ __forceinline__ OvGnPlace ov_gn_place(const OvGn& p, const OvGnTile& 
     q.c0 = q.g0 * p.cg;
     q.cb = q.ng * p.cg;
     q.r0 = q.chunk * t.rows;
-    q.r1 = min(q.r0 + t.rows, p.S);
+    q.r1 = q.r0 + ov_gn_tile_rows(p, t, q.chunk);
     return q;
 }
 
@@ -343,7 +431,7 @@ __device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, c
         float a = 0.f, b = 0.f;
         for (int k = l; k < t.chunks; k += lg) {
             const float2 v = src[(int64_t)k * p.groups];
-            a += FWD ? v.x * (float)(min(t.rows, p.S - k * t.rows) * p.cg) : v.x;
+            a += FWD ? v.x * (float)(ov_gn_tile_rows(p, t, k) * p.cg) : v.x;
             b += v.y;
         }
         for (int o = lg / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
@@ -353,7 +441,7 @@ __device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, c
             float d2 = 0.f;
             for (int k = l; k < t.chunks; k += lg) {
                 const float d = src[(int64_t)k * p.groups].x - mu;
-                d2 += d * d * (float)(min(t.rows, p.S - k * t.rows) * p.cg);
+                d2 += d * d * (float)(ov_gn_tile_rows(p, t, k) * p.cg);
             }
             for (int o = lg / 2; o > 0; o >>= 1) d2 += __shfl_xor(d2, o, 64);
             if (l == 0) st[g] = make_float2(mu, 1.f / sqrtf((b + d2) / total + p.eps));
@@ -366,9 +454,10 @@ __device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, c
 
 #define OV_GN_MAX_CB(E) (256 * (E))
 
-template <typename T, int MODE>
-__global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict__ x, const OvGn p, const OvGnTile t, T* __restrict__ y,
+template <typename T, int MODE, bool LIGHT>
+__global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict__ x, const OvGn p_, const OvGnTile t, T* __restrict__ y,
                                                              float* __restrict__ mean, float* __restrict__ rstd) {
+    const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvVec<T>::N, RB = 8;
     __shared__ float2 cs[OV_GN_MAX_CB(E)];               // (mean, M2) of a thread's rows of a channel
     __shared__ float2 st[OV_GN_MAX_CB(E)];               // per group: (mean, M2), then (mu, r)
@@ -376,8 +465,13 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
     const int tid = threadIdx.x, ty = tid / t.tx, tx = tid - ty * t.tx;
     const bool on = ty < t.ty;
     const int cnt = on ? min(q.cb - tx * E, E) : 0;      // <= 0: no channel of the block
-    const int64_t row0 = (int64_t)q.n * p.S;
-    const T* xc = x + q.c0 + tx * E;
+    const int64_t row0 = (int64_t)q.n * p.S, col = q.c0 + tx * E, total = (int64_t)p.N * p.S * p.C;
+    constexpr int RA = 8;
+    OvVec<T> raw[RA];
+    auto fetch = [&](int r) {
+#pragma unroll
+        for (int i = 0; i < RA; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, raw[i]);
+    };
     if (MODE != 1) {
         float m[E], m2[E];
 #pragma unroll
@@ -385,21 +479,31 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
         int have = 0;
         if (cnt > 0)
             for (int r = q.r0 + ty; r < q.r1; r += RB * t.ty) {
-                float v[RB][E];
-                const int nb = min((q.r1 - r + t.ty - 1) / t.ty, RB);
+                OvVec<T> v[RB];
+                const int nb = min(ov_gn_thread_rows(t, q.r1 - r, 0), RB);
 #pragma unroll
-                for (int i = 0; i < RB; ++i) ov_gn_load<T>(xc + (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C, cnt, v[i]);
+                for (int i = 0; i < RB; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, v[i]);
+                if ((row0 + min(r + (RB - 1) * t.ty, q.r1 - 1)) * p.C + col > total - E) {      // the tensor's last pieces
+#pragma unroll
+                    for (int i = 0; i < RB; ++i) {
+                        const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col;
+                        float f[E];
+                        ov_gn_floats<T>(x, total, o, v[i], f);
+#pragma unroll
+                        for (int k = 0; k < E; ++k) v[i].e[k] = ov_from_f<T>(f[k]);
+                    }
+                }
                 // mean and second moment of these rows, then Chan's combination with the ones before
                 const float fb = (float)nb, ft = (float)(have + nb), wgt = fb / ft, cross = (float)have * wgt;
 #pragma unroll
                 for (int k = 0; k < E; ++k) {
                     float s = 0.f, s2 = 0.f;
 #pragma unroll
-                    for (int i = 0; i < RB; ++i) s += i < nb ? v[i][k] : 0.f;
+                    for (int i = 0; i < RB; ++i) s += i < nb ? ov_to_f<T>(v[i].e[k]) : 0.f;
                     const float mb = s / fb;
 #pragma unroll
                     for (int i = 0; i < RB; ++i) {
-                        const float d = v[i][k] - mb;
+                        const float d = ov_to_f<T>(v[i].e[k]) - mb;
                         s2 += i < nb ? d * d : 0.f;
                     }
                     const float d = mb - m[k];
@@ -416,12 +520,12 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
         const int rows = q.r1 - q.r0;
         for (int c = tid; c < q.cb; c += 256) {
             float a = 0.f, b = 0.f;
-            for (int k = 0; k < t.ty; ++k) a += cs[k * t.tx * E + c].x * (float)((rows - k + t.ty - 1) / t.ty);
+            for (int k = 0; k < t.ty; ++k) a += cs[k * t.tx * E + c].x * (float)ov_gn_thread_rows(t, rows, k);
             a /= (float)rows;
             for (int k = 0; k < t.ty; ++k) {
                 const float2 v = cs[k * t.tx * E + c];
                 const float d = v.x - a;
-                b += v.y + d * d * (float)((rows - k + t.ty - 1) / t.ty);
+                b += v.y + d * d * (float)ov_gn_thread_rows(t, rows, k);
             }
             st[c] = make_float2(a, b);
         }
@@ -441,6 +545,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
         if (MODE == 0) return;
         __syncthreads();
     } else {
+        if (cnt > 0) fetch(q.r0 + ty);                    // under the gather's latency
         ov_gn_gather<true>(p, t, q, cs);
     }
     if (q.chunk == 0)
@@ -449,38 +554,39 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
             rstd[(int64_t)q.n * p.groups + q.g0 + g] = cs[g].y;
         }
     if (cnt <= 0) return;
+    if (MODE == 2) fetch(q.r0 + ty);
     float mu[E], rw[E], b[E];
+    ov_gn_params<E>(p.w, p.wtype, q.c0 + tx * E, cnt, 1.f, rw);
+    ov_gn_params<E>(p.b, p.wtype, q.c0 + tx * E, cnt, 0.f, b);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-        const int c = min(tx * E + k, q.cb - 1);
-        const float2 v = cs[c / p.cg];
+        const float2 v = cs[min(tx * E + k, q.cb - 1) / p.cg];
         mu[k] = v.x;
-        rw[k] = v.y * ov_gn_param(p.w, p.wtype, q.c0 + c, 1.f);
-        b[k] = ov_gn_param(p.b, p.wtype, q.c0 + c, 0.f);
+        rw[k] *= v.y;
     }
-    constexpr int RA = 4;
     for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
-        float v[RA][E];
-#pragma unroll
-        for (int i = 0; i < RA; ++i) ov_gn_load<T>(xc + (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C, cnt, v[i]);
+        if (r > q.r0 + ty) fetch(r);
 #pragma unroll
         for (int i = 0; i < RA; ++i) {
             const int rr = r + i * t.ty;
             if (rr >= q.r1) break;
+            float v[E];
+            ov_gn_floats<T>(x, total, (row0 + rr) * p.C + col, raw[i], v);
 #pragma unroll
-            for (int k = 0; k < E; ++k) v[i][k] = (v[i][k] - mu[k]) * rw[k] + b[k];
-            ov_act<E>(v[i], p.act);
-            ov_gn_drop<E>(p, row0 + rr, q.c0 + tx * E, v[i]);
-            ov_gn_store<T>(y + (row0 + rr) * p.C + q.c0 + tx * E, cnt, v[i]);
+            for (int k = 0; k < E; ++k) v[k] = (v[k] - mu[k]) * rw[k] + b[k];
+            ov_act<E>(v, p.act);
+            ov_gn_drop<E>(p, row0 + rr, q.c0 + tx * E, v);
+            ov_gn_store<T>(y + (row0 + rr) * p.C + col, cnt, v);
         }
     }
 }
 
 // chan: [2][N chunks][C]: the tiles' sums of dv xhat, then of dv, per channel
-template <typename T, int MODE>
-__global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p, const OvGnTile t,
+template <typename T, int MODE, bool LIGHT>
+__global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p_, const OvGnTile t,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                                                              float* __restrict__ chan) {
+    const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvVec<T>::N, RA = 4;
     __shared__ float2 cs[OV_GN_MAX_CB(E)];
     __shared__ float2 st[OV_GN_MAX_CB(E)];
@@ -488,56 +594,61 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
     const int tid = threadIdx.x, ty = tid / t.tx, tx = tid - ty * t.tx;
     const bool on = ty < t.ty;
     const int cnt = on ? min(q.cb - tx * E, E) : 0;
-    const int64_t row0 = (int64_t)q.n * p.S;
-    const T* xc = x + q.c0 + tx * E;
-    const T* dc = dy + q.c0 + tx * E;
-    float mu[E], rr_[E], w[E], b[E];
+    const int64_t row0 = (int64_t)q.n * p.S, col = q.c0 + tx * E, total = (int64_t)p.N * p.S * p.C;
+    // x - mu, then v = (x - mu) (r gamma) + beta
+    float mu[E], rw[E], b[E];
+    OvVec<T> rx[RA], rd[RA];
+    auto fetch = [&](int r) {
 #pragma unroll
-    for (int k = 0; k < E; ++k) {
-        const int c = max(min(tx * E + k, q.cb - 1), 0);
-        const int64_t gi = (int64_t)q.n * p.groups + q.g0 + c / p.cg;
-        mu[k] = mean[gi];
-        rr_[k] = rstd[gi];
-        w[k] = ov_gn_param(p.w, p.wtype, q.c0 + c, 1.f);
-        b[k] = ov_gn_param(p.b, p.wtype, q.c0 + c, 0.f);
-    }
-    // xhat and dv of one row
-    auto grad = [&](int64_t row, float (&v)[E], float (&d)[E]) {
-        ov_gn_drop<E>(p, row, q.c0 + tx * E, d);
-        float a[E];
+        for (int i = 0; i < RA; ++i) {
+            const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col;
+            ov_gn_raw<T>(x, total, o, rx[i]);
+            ov_gn_raw<T>(dy, total, o, rd[i]);
+        }
+    };
+    if (cnt > 0) {
+        ov_gn_params<E>(p.w, p.wtype, q.c0 + tx * E, cnt, 1.f, rw);
+        ov_gn_params<E>(p.b, p.wtype, q.c0 + tx * E, cnt, 0.f, b);
 #pragma unroll
         for (int k = 0; k < E; ++k) {
-            v[k] = (v[k] - mu[k]) * rr_[k];
-            a[k] = v[k] * w[k] + b[k];
+            const int64_t gi = (int64_t)q.n * p.groups + q.g0 + min(tx * E + k, q.cb - 1) / p.cg;
+            mu[k] = mean[gi];
+            rw[k] *= rstd[gi];
         }
-        ov_act_grad<E>(a, p.act);
+    }
+    auto grad = [&](int64_t row, const OvVec<T>& vx, const OvVec<T>& vd, float (&xm)[E], float (&dv)[E]) {
+        float d[E];
+        ov_gn_floats<T>(x, total, row * p.C + col, vx, xm);
+        ov_gn_floats<T>(dy, total, row * p.C + col, vd, d);
 #pragma unroll
-        for (int k = 0; k < E; ++k) d[k] = d[k] == 0.f ? 0.f : d[k] * a[k];
+        for (int k = 0; k < E; ++k) {
+            xm[k] -= mu[k];
+            dv[k] = xm[k] * rw[k] + b[k];
+        }
+        ov_gn_dv<E>(p, row, q.c0 + tx * E, d, dv);
     };
     if (MODE != 1) {
         float sb[E], sw[E];
 #pragma unroll
         for (int k = 0; k < E; ++k) sb[k] = sw[k] = 0.f;
-        if (cnt > 0)
+        if (cnt > 0) {
             for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
-                float v[RA][E], d[RA][E];
-#pragma unroll
-                for (int i = 0; i < RA; ++i) {
-                    const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C;
-                    ov_gn_load<T>(xc + o, cnt, v[i]);
-                    ov_gn_load<T>(dc + o, cnt, d[i]);
-                }
+                fetch(r);
 #pragma unroll
                 for (int i = 0; i < RA; ++i) {
                     if (r + i * t.ty >= q.r1) break;
-                    grad(row0 + r + i * t.ty, v[i], d[i]);
+                    float xm[E], dv[E];
+                    grad(row0 + r + i * t.ty, rx[i], rd[i], xm, dv);
 #pragma unroll
                     for (int k = 0; k < E; ++k) {
-                        sb[k] += d[i][k];
-                        sw[k] += d[i][k] * v[i][k];
+                        sb[k] += dv[k];
+                        sw[k] += dv[k] * xm[k];
                     }
                 }
             }
+#pragma unroll
+            for (int k = 0; k < E; ++k) sw[k] *= rstd[(int64_t)q.n * p.groups + q.g0 + min(tx * E + k, q.cb - 1) / p.cg];
+        }
         if (on)
 #pragma unroll
             for (int k = 0; k < E; ++k) cs[ty * t.tx * E + tx * E + k] = make_float2(sb[k], sw[k]);
@@ -577,29 +688,26 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
         ov_gn_gather<false>(p, t, q, cs);
     }
     if (cnt <= 0) return;
-    float s1[E], s2[E];
+    // dx = r (dv gamma - s1 - xhat s2) = dv (r gamma) - r s1 - (x - mu) r^2 s2
+    float k1[E], k2[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) {
         const float2 v = cs[min(tx * E + k, q.cb - 1) / p.cg];
-        s1[k] = v.x;
-        s2[k] = v.y;
+        const float rs = rstd[(int64_t)q.n * p.groups + q.g0 + min(tx * E + k, q.cb - 1) / p.cg];
+        k1[k] = rs * v.x;
+        k2[k] = rs * rs * v.y;
     }
     for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
-        float v[RA][E], d[RA][E];
-#pragma unroll
-        for (int i = 0; i < RA; ++i) {
-            const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C;
-            ov_gn_load<T>(xc + o, cnt, v[i]);
-            ov_gn_load<T>(dc + o, cnt, d[i]);
-        }
+        fetch(r);
 #pragma unroll
         for (int i = 0; i < RA; ++i) {
             const int rr = r + i * t.ty;
             if (rr >= q.r1) break;
-            grad(row0 + rr, v[i], d[i]);
+            float xm[E], dv[E];
+            grad(row0 + rr, rx[i], rd[i], xm, dv);
 #pragma unroll
-            for (int k = 0; k < E; ++k) d[i][k] = rr_[k] * (d[i][k] * w[k] - s1[k] - v[i][k] * s2[k]);
-            ov_gn_store<T>(dx + (row0 + rr) * p.C + q.c0 + tx * E, cnt, d[i]);
+            for (int k = 0; k < E; ++k) dv[k] = dv[k] * rw[k] - k1[k] - xm[k] * k2[k];
+            ov_gn_store<T>(dx + (row0 + rr) * p.C + col, cnt, dv);
         }
     }
 }
@@ -642,9 +750,8 @@ __device__ __forceinline__ float ov_gn_any_dv(const OvGn& p, const T* x, const T
     const int64_t o = row * p.C + c;
     *xhat = (ov_to_f<T>(x[o]) - mu) * r;
     float d[1] = {ov_to_f<T>(dy[o])}, a[1] = {*xhat * ov_gn_param(p.w, p.wtype, c, 1.f) + ov_gn_param(p.b, p.wtype, c, 0.f)};
-    ov_gn_drop<1>(p, row, c, d);
-    ov_act_grad<1>(a, p.act);
-    return d[0] == 0.f ? 0.f : d[0] * a[0];
+    ov_gn_dv<1>(p, row, c, d, a);
+    return a[0];
 }
 
 template <typename T>
@@ -727,7 +834,11 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
     OvGnPlan q{};
     const int E = dtype == ONTOVAE_F32 ? 4 : 8, cg = C / groups;
     const int pieces = (cg + E - 1) / E;
-    if (S == 1 && pieces <= 1024 * (16 / E)) {
+    if ((int64_t)N * S * C < E) {                         // not one 16-byte piece
+        q.form = OV_GN_ANY;
+        return q;
+    }
+    if (S == 1 && pieces <= 1024 * (8 / E)) {
         q.form = OV_GN_ROW;
         if (pieces <= 64) {
             q.nv = 1;
@@ -735,7 +846,7 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
             while (q.lpg < pieces) q.lpg *= 2;
         } else {
             q.lpg = pieces <= 64 * (16 / E) ? 64 : pieces <= 256 * (16 / E) ? 256 : 1024;
-            q.nv = 16 / E;
+            q.nv = 16 / E;                                // 1024 threads: half of it, 128 registers are all there are
         }
         // enough slots for four workgroups of 256 threads per CU; the gradient sums of a slot are a row of C floats to write and
         // read again, so a slot takes at least 8 samples there
@@ -756,14 +867,13 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         t.ty = std::min(256 / t.tx, S);
         const int64_t bytes = (int64_t)S * t.gb * cg * (dtype == ONTOVAE_F32 ? 4 : 2);
         const int64_t wg = (int64_t)N * t.nblk;
-        if (bytes <= 65536) {
-            q.form = OV_GN_TILE1;
-            t.chunks = 1;
-            t.rows = S;
-        } else {
+        t.chunks = 1;
+        t.rows = S;
+        q.form = OV_GN_TILE1;
+        if (bytes > 65536) {
             q.form = OV_GN_TILE;
-            const int most = (S + t.ty * 8 - 1) / (t.ty * 8);
-            t.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, (2048 + wg - 1) / wg));
+            const int most = (S + t.ty * 16 - 1) / (t.ty * 16);
+            t.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, (1024 + wg - 1) / wg));
             t.rows = (S + t.chunks - 1) / t.chunks;
             t.chunks = (S + t.rows - 1) / t.rows;
             q.part_floats = 2LL * N * t.chunks * groups;
@@ -802,18 +912,18 @@ static int ov_gn_ready(const char* what, const OvGn& p, const OvGnPlan& q, const
         case 32: GO(32, 1); break;                                                             \
         case 64: if (q.nv == 1) { GO(64, 1); } else { GO(64, NVX); } break;                    \
         case 256: GO(256, NVX); break;                                                         \
-        default: GO(1024, NVX); break;                                                         \
+        default: GO(1024, NVX / 2); break;                                                         \
     }
 
-template <typename T>
-static void ov_gn_fwd_launch(const void* x, const OvGn& p, OvGnPlan q, void* y, float* mean, float* rstd, void* ws, hipStream_t st) {
+template <typename T, bool LIGHT>
+static void ov_gn_fwd_go(const void* x, const OvGn& p, OvGnPlan q, void* y, float* mean, float* rstd, void* ws, hipStream_t st) {
     const T* xt = static_cast<const T*>(x);
     T* yt = static_cast<T*>(y);
     q.t.part = static_cast<float*>(ws);
     constexpr int NVX = 16 / OvVec<T>::N;
     if (q.form == OV_GN_ROW) {
 #define OV_GO(L, V)                                                                                                                              \
-    hipLaunchKernelGGL((ov_gn_row_fwd_kernel<T, L, V>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
+    hipLaunchKernelGGL((ov_gn_row_fwd_kernel<T, L, V, LIGHT>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
                        dim3(L < 256 ? 256 : L), 0, st, xt, p, q.RS, yt, mean, rstd)
         OV_GN_ROW_SWITCH(OV_GO)
 #undef OV_GO
@@ -821,12 +931,19 @@ static void ov_gn_fwd_launch(const void* x, const OvGn& p, OvGnPlan q, void* y, 
         hipLaunchKernelGGL(ov_gn_any_fwd_kernel<T>, dim3((unsigned)((int64_t)p.N * p.groups)), dim3(1024), 0, st, xt, p, yt, mean, rstd);
     } else {
         const dim3 grid((unsigned)((int64_t)p.N * q.t.chunks * q.t.nblk));
-        if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 2>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+        if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 2, LIGHT>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
         else {
-            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 0>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
-            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 1>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 0, LIGHT>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 1, LIGHT>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
         }
     }
+}
+
+static bool ov_gn_is_light(const OvGn& p) { return p.drop.t == 0 && p.act <= ONTOVAE_ACT_SILU; }
+template <typename T>
+static void ov_gn_fwd_launch(const void* x, const OvGn& p, const OvGnPlan& q, void* y, float* mean, float* rstd, void* ws, hipStream_t st) {
+    if (ov_gn_is_light(p)) ov_gn_fwd_go<T, true>(x, p, q, y, mean, rstd, ws, st);
+    else ov_gn_fwd_go<T, false>(x, p, q, y, mean, rstd, ws, st);
 }
 
 extern "C" int ontovae_group_norm_act(const void* x, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, const void* weight,
@@ -849,8 +966,8 @@ extern "C" int ontovae_group_norm_act(const void* x, int32_t dtype, int32_t N, i
     return ONTOVAE_OK;
 }
 
-template <typename T>
-static void ov_gn_bwd_launch(const void* dy, const void* x, const OvGn& p, OvGnPlan q, const float* mean, const float* rstd, void* dx, float* dw,
+template <typename T, bool LIGHT>
+static void ov_gn_bwd_go(const void* dy, const void* x, const OvGn& p, OvGnPlan q, const float* mean, const float* rstd, void* dx, float* dw,
                              float* db, void* ws, hipStream_t st) {
     const T* xt = static_cast<const T*>(x);
     const T* dt = static_cast<const T*>(dy);
@@ -865,19 +982,26 @@ static void ov_gn_bwd_launch(const void* dy, const void* x, const OvGn& p, OvGnP
     }
     if (q.form == OV_GN_ROW) {
 #define OV_GO(L, V)                                                                                                                              \
-    hipLaunchKernelGGL((ov_gn_row_bwd_kernel<T, L, V>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
+    hipLaunchKernelGGL((ov_gn_row_bwd_kernel<T, L, V, LIGHT>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
                        dim3(L < 256 ? 256 : L), 0, st, dt, xt, p, q.RS, mean, rstd, dxt, chan)
         OV_GN_ROW_SWITCH(OV_GO)
 #undef OV_GO
     } else {
         const dim3 grid((unsigned)((int64_t)p.N * q.t.chunks * q.t.nblk));
-        if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 2>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
+        if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 2, LIGHT>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
         else {
-            hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 0>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
-            hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 1>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
+            hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 0, LIGHT>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
+            hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 1, LIGHT>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
         }
     }
     if (chan) hipLaunchKernelGGL(ov_gn_param_kernel, dim3((p.C + 15) / 16, 2), dim3(256), 0, st, chan, q.chan_rows, p.C, dw, db);
+}
+
+template <typename T>
+static void ov_gn_bwd_launch(const void* dy, const void* x, const OvGn& p, const OvGnPlan& q, const float* mean, const float* rstd, void* dx, float* dw,
+                             float* db, void* ws, hipStream_t st) {
+    if (ov_gn_is_light(p)) ov_gn_bwd_go<T, true>(dy, x, p, q, mean, rstd, dx, dw, db, ws, st);
+    else ov_gn_bwd_go<T, false>(dy, x, p, q, mean, rstd, dx, dw, db, ws, st);
 }
 
 __global__ __launch_bounds__(256) void ov_gn_zero_kernel(float* dw, float* db, int C) {
