@@ -11,6 +11,15 @@
 
 #include "ontovae_dropout.h"
 
+// 8 neighbours of a row: one Philox block of dropout where they start on a multiple of 8, else two
+template <typename T>
+struct OvGnPiece {
+    static constexpr int N = 8;
+    T e[8];
+    __device__ __forceinline__ void load(const T* p) { __builtin_memcpy(e, p, sizeof(e)); }
+    __device__ __forceinline__ void store(T* p) const { __builtin_memcpy(p, e, sizeof(e)); }
+};
+
 struct OvGn {
     int N, S, C, groups, cg;
     const void* w;
@@ -118,17 +127,17 @@ __device__ __forceinline__ void ov_gn_dv(const OvGn& p, int64_t row, int c, cons
     ov_gn_drop<E>(p, row, c, v);
 }
 
-// 16 bytes from element `off` of x [total], whatever of them belongs to the reader: a piece that ends inside its 16 bytes reads
+// 8 elements from `off` on of x [total], whatever of them belongs to the reader: a piece that ends inside the 8 reads
 // on into its neighbour.  The load is unconditional (a branch around it would make the compiler wait for every load by itself);
 // the last pieces of the tensor, which have no neighbour, are read from further in front, and ov_gn_floats fetches their
 // elements one by one.
 template <typename T>
-__device__ __forceinline__ void ov_gn_raw(const T* x, int64_t total, int64_t off, OvVec<T>& v) {
-    v.load(x + min(off, total - OvVec<T>::N));
+__device__ __forceinline__ void ov_gn_raw(const T* x, int64_t total, int64_t off, OvGnPiece<T>& v) {
+    v.load(x + min(off, total - OvGnPiece<T>::N));
 }
 template <typename T>
-__device__ __forceinline__ void ov_gn_floats(const T* x, int64_t total, int64_t off, const OvVec<T>& v, float (&f)[OvVec<T>::N]) {
-    constexpr int E = OvVec<T>::N;
+__device__ __forceinline__ void ov_gn_floats(const T* x, int64_t total, int64_t off, const OvGnPiece<T>& v, float (&f)[OvGnPiece<T>::N]) {
+    constexpr int E = OvGnPiece<T>::N;
 #pragma unroll
     for (int j = 0; j < E; ++j) f[j] = ov_to_f<T>(v.e[j]);
     if (off > total - E) {
@@ -137,9 +146,9 @@ __device__ __forceinline__ void ov_gn_floats(const T* x, int64_t total, int64_t 
     }
 }
 template <typename T>
-__device__ __forceinline__ void ov_gn_store(T* y, int cnt, const float (&f)[OvVec<T>::N]) {
-    constexpr int E = OvVec<T>::N;
-    OvVec<T> v;
+__device__ __forceinline__ void ov_gn_store(T* y, int cnt, const float (&f)[OvGnPiece<T>::N]) {
+    constexpr int E = OvGnPiece<T>::N;
+    OvGnPiece<T> v;
 #pragma unroll
     for (int j = 0; j < E; ++j) v.e[j] = ov_from_f<T>(f[j]);
     if (cnt >= E) v.store(y);
@@ -181,7 +190,7 @@ __device__ __forceinline__ float ov_gn_sum(float v, float* red) {
 }
 
 // ---------------------------------------------------------------- S = 1: a group is one contiguous run of cg elements
-// LPG threads hold a group in registers, NV pieces of 16 bytes each; a slot of LPG threads keeps its group and walks the
+// LPG threads hold a group in registers, NV pieces of 8 elements each; a slot of LPG threads keeps its group and walks the
 // samples rs, rs + RS, ...: weight and bias (and the sums of their gradients) stay in registers.  Neighbouring slots take
 // neighbouring groups, so a workgroup reads contiguous memory.  One read of x (and dy), one write: bound by memory.
 // The next sample is requested before the current one is reduced.
@@ -189,7 +198,7 @@ template <typename T, int LPG, int NV, bool LIGHT>
 __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(const T* __restrict__ x, const OvGn p_, int RS, T* __restrict__ y,
                                                                              float* __restrict__ mean, float* __restrict__ rstd) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
-    constexpr int E = OvVec<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
+    constexpr int E = OvGnPiece<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
     __shared__ float red[16];
     const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
     const int j = threadIdx.x % LPG, rs = (int)(slot / p.groups), g = (int)(slot - (int64_t)rs * p.groups);
@@ -198,7 +207,7 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(co
     const int64_t total = (int64_t)p.N * p.C;
     const bool ragged = p.cg % E != 0;
     int64_t at = (int64_t)rs * p.C + gc;
-    OvVec<T> raw[NV];
+    OvGnPiece<T> raw[NV];
     int cnt[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -260,21 +269,23 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(co
     }
 }
 
-// part: [2][RS][C]: the slots' sums of dv xhat, then of dv (written for every slot, also one without a sample)
+// part: [2][R][C]: sums of dv xhat, then of dv.  A slot's sums, or, where whole samples fit a workgroup (wgs of them at a time), the
+// workgroup's: fewer rows to write and to add up again.
 template <typename T, int LPG, int NV, bool LIGHT>
-__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p_, int RS,
+__global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p_, int RS, int wgs,
                                                                              const float* __restrict__ mean, const float* __restrict__ rstd,
                                                                              T* __restrict__ dx, float* __restrict__ part) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
-    constexpr int E = OvVec<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
+    constexpr int E = OvGnPiece<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
     __shared__ float red[16];
+    __shared__ float sums[LPG < 256 ? 256 * 8 : 8];
     const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
     const int j = threadIdx.x % LPG, rs = (int)(slot / p.groups), g = (int)(slot - (int64_t)rs * p.groups);
-    if (rs >= RS) return;
     const int64_t gc = (int64_t)g * p.cg, step = (int64_t)RS * p.C;
     const int64_t total = (int64_t)p.N * p.C;
-    int64_t at = (int64_t)rs * p.C + gc;
-    OvVec<T> rx[NV], rd[NV];
+    const int first = min(rs, p.N - 1);                  // a slot past the last (rs >= RS) walks no sample
+    int64_t at = (int64_t)first * p.C + gc;
+    OvGnPiece<T> rx[NV], rd[NV];
     int cnt[NV];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -283,7 +294,7 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
         ov_gn_raw<T>(x, total, at + o, rx[i]);
         ov_gn_raw<T>(dy, total, at + o, rd[i]);
     }
-    float mu = mean[(int64_t)rs * p.groups + g], r = rstd[(int64_t)rs * p.groups + g];
+    float mu = mean[(int64_t)first * p.groups + g], r = rstd[(int64_t)first * p.groups + g];
     float w[NV][E], b[NV][E], sw[NV][E], sb[NV][E];
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
@@ -295,7 +306,7 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
         }
     }
     const float len = (float)p.cg;
-    for (int n = rs; n < p.N; n += RS) {
+    for (int n = rs < RS ? rs : p.N; n < p.N; n += RS) {
         const int64_t here = at;
         const float mu0 = mu, r0 = r;
         float v[NV][E], d[NV][E];
@@ -345,11 +356,30 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
         }
     }
     if (!part) return;
+    const int64_t R = wgs > 1 ? gridDim.x : RS, row = wgs > 1 ? blockIdx.x : rs;
 #pragma unroll
     for (int i = 0; i < NV; ++i) {
-        const int64_t o = (int64_t)rs * p.C + gc + (j + i * LPG) * E;
+        if (LPG < 256 && wgs > 1) {                      // uniform; 256 = wgs * groups * LPG
+            const int lane = threadIdx.x, per = p.groups * LPG;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                __syncthreads();
+#pragma unroll
+                for (int k = 0; k < E; ++k) sums[k * 256 + lane] = h ? sb[i][k] : sw[i][k];
+                __syncthreads();
+                if (lane < per)
+                    for (int o = per; o < 256; o += per) {
+#pragma unroll
+                        for (int k = 0; k < E; ++k) (h ? sb[i][k] : sw[i][k]) += sums[k * 256 + lane + o];
+                    }
+            }
+            if (lane >= per) continue;
+        } else if (rs >= RS) {
+            continue;
+        }
+        const int64_t o = row * p.C + gc + (j + i * LPG) * E;
         ov_gn_store_f<E>(part + o, cnt[i], sw[i]);
-        ov_gn_store_f<E>(part + (int64_t)RS * p.C + o, cnt[i], sb[i]);
+        ov_gn_store_f<E>(part + R * p.C + o, cnt[i], sb[i]);
     }
 }
 
@@ -385,7 +415,7 @@ __global__ __launch_bounds__(256) void ov_gn_param_kernel(const float* __restric
 
 // ---------------------------------------------------------------- S > 1: tiles of rows x channels
 // A workgroup takes a run of a sample's rows and a block of whole groups (all channels if they fit): 256 threads as TX pieces
-// of 16 bytes x TY rows, a thread's channels fixed, so that weight, bias and the per-channel sums stay in registers; channel
+// of 8 channels x TY rows, a thread's channels fixed, so that weight, bias and the per-channel sums stay in registers; channel
 // sums meet in LDS, group sums are sums of channel sums (a piece may hold parts of several groups).
 //   MODE 0: sums of the tile only      MODE 1: the output, from the sums of the sample's tiles
 //   MODE 2: the tile is the whole sample; both in one launch, the second read from the cache
@@ -458,7 +488,7 @@ template <typename T, int MODE, bool LIGHT>
 __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict__ x, const OvGn p_, const OvGnTile t, T* __restrict__ y,
                                                              float* __restrict__ mean, float* __restrict__ rstd) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
-    constexpr int E = OvVec<T>::N, RB = 8;
+    constexpr int E = OvGnPiece<T>::N, RB = 16 / (int)sizeof(T);
     __shared__ float2 cs[OV_GN_MAX_CB(E)];               // (mean, M2) of a thread's rows of a channel
     __shared__ float2 st[OV_GN_MAX_CB(E)];               // per group: (mean, M2), then (mu, r)
     const OvGnPlace q = ov_gn_place(p, t, MODE == 1);
@@ -467,7 +497,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
     const int cnt = on ? min(q.cb - tx * E, E) : 0;      // <= 0: no channel of the block
     const int64_t row0 = (int64_t)q.n * p.S, col = q.c0 + tx * E, total = (int64_t)p.N * p.S * p.C;
     constexpr int RA = 8;
-    OvVec<T> raw[RA];
+    OvGnPiece<T> raw[RA];
     auto fetch = [&](int r) {
 #pragma unroll
         for (int i = 0; i < RA; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, raw[i]);
@@ -479,7 +509,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
         int have = 0;
         if (cnt > 0)
             for (int r = q.r0 + ty; r < q.r1; r += RB * t.ty) {
-                OvVec<T> v[RB];
+                OvGnPiece<T> v[RB];
                 const int nb = min(ov_gn_thread_rows(t, q.r1 - r, 0), RB);
 #pragma unroll
                 for (int i = 0; i < RB; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, v[i]);
@@ -494,22 +524,26 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
                     }
                 }
                 // mean and second moment of these rows, then Chan's combination with the ones before
-                const float fb = (float)nb, ft = (float)(have + nb), wgt = fb / ft, cross = (float)have * wgt;
+                const float fb = (float)nb, ft = (float)(have + nb), wgt = fb / ft, cross = (float)have * wgt, rb = 1.f / fb;
+                auto merge = [&](auto whole) {
 #pragma unroll
-                for (int k = 0; k < E; ++k) {
-                    float s = 0.f, s2 = 0.f;
+                    for (int k = 0; k < E; ++k) {
+                        float s = 0.f, s2 = 0.f;
 #pragma unroll
-                    for (int i = 0; i < RB; ++i) s += i < nb ? ov_to_f<T>(v[i].e[k]) : 0.f;
-                    const float mb = s / fb;
+                        for (int i = 0; i < RB; ++i) s += whole || i < nb ? ov_to_f<T>(v[i].e[k]) : 0.f;
+                        const float mb = s * rb;
 #pragma unroll
-                    for (int i = 0; i < RB; ++i) {
-                        const float d = ov_to_f<T>(v[i].e[k]) - mb;
-                        s2 += i < nb ? d * d : 0.f;
+                        for (int i = 0; i < RB; ++i) {
+                            const float d = ov_to_f<T>(v[i].e[k]) - mb;
+                            s2 += whole || i < nb ? d * d : 0.f;
+                        }
+                        const float d = mb - m[k];
+                        m[k] += d * wgt;
+                        m2[k] += s2 + d * d * cross;
                     }
-                    const float d = mb - m[k];
-                    m[k] += d * wgt;
-                    m2[k] += s2 + d * d * cross;
-                }
+                };
+                if (nb == RB) merge(std::true_type{});
+                else merge(std::false_type{});
                 have += nb;
             }
         if (on)
@@ -587,7 +621,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
                                                              const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
                                                              float* __restrict__ chan) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
-    constexpr int E = OvVec<T>::N, RA = 4;
+    constexpr int E = OvGnPiece<T>::N, RA = 8 / (int)sizeof(T);
     __shared__ float2 cs[OV_GN_MAX_CB(E)];
     __shared__ float2 st[OV_GN_MAX_CB(E)];
     const OvGnPlace q = ov_gn_place(p, t, MODE == 1);
@@ -597,7 +631,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
     const int64_t row0 = (int64_t)q.n * p.S, col = q.c0 + tx * E, total = (int64_t)p.N * p.S * p.C;
     // x - mu, then v = (x - mu) (r gamma) + beta
     float mu[E], rw[E], b[E];
-    OvVec<T> rx[RA], rd[RA];
+    OvGnPiece<T> rx[RA], rd[RA];
     auto fetch = [&](int r) {
 #pragma unroll
         for (int i = 0; i < RA; ++i) {
@@ -616,7 +650,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
             rw[k] *= rstd[gi];
         }
     }
-    auto grad = [&](int64_t row, const OvVec<T>& vx, const OvVec<T>& vd, float (&xm)[E], float (&dv)[E]) {
+    auto grad = [&](int64_t row, const OvGnPiece<T>& vx, const OvGnPiece<T>& vd, float (&xm)[E], float (&dv)[E]) {
         float d[E];
         ov_gn_floats<T>(x, total, row * p.C + col, vx, xm);
         ov_gn_floats<T>(dy, total, row * p.C + col, vd, d);
@@ -825,16 +859,16 @@ static int ov_gn_check(const char* what, int32_t dtype, int32_t N, int32_t S, in
 enum { OV_GN_ROW, OV_GN_TILE, OV_GN_TILE1, OV_GN_ANY };
 struct OvGnPlan {
     int form;
-    int lpg, nv, RS;         // OV_GN_ROW
+    int lpg, nv, RS, wgs;    // OV_GN_ROW
     OvGnTile t;              // OV_GN_TILE (two launches), OV_GN_TILE1 (one)
     int64_t part_floats, chan_floats, chan_rows;
 };
 
 static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool backward) {
     OvGnPlan q{};
-    const int E = dtype == ONTOVAE_F32 ? 4 : 8, cg = C / groups;
+    const int E = 8, cg = C / groups;
     const int pieces = (cg + E - 1) / E;
-    if ((int64_t)N * S * C < E) {                         // not one 16-byte piece
+    if ((int64_t)N * S * C < E) {                         // not one piece
         q.form = OV_GN_ANY;
         return q;
     }
@@ -848,12 +882,15 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
             q.lpg = pieces <= 64 * (16 / E) ? 64 : pieces <= 256 * (16 / E) ? 256 : 1024;
             q.nv = 16 / E;                                // 1024 threads: half of it, 128 registers are all there are
         }
-        // enough slots for four workgroups of 256 threads per CU; the gradient sums of a slot are a row of C floats to write and
-        // read again, so a slot takes at least 8 samples there
-        const int64_t want = std::max<int64_t>(262144 / ((int64_t)groups * q.lpg), 1);
-        q.RS = (int)std::min<int64_t>(want, backward ? std::max((N + 7) / 8, std::min(N, 16)) : N);
-        q.chan_rows = q.RS;
-        q.chan_floats = backward ? 2LL * q.RS * C : 0;
+        // enough slots for four workgroups of 256 threads per CU.  Each row of gradient sums (a workgroup's where whole samples
+        // fit it, else a slot's) is written and read once more: at most one to 8 samples
+        const int per = groups * q.lpg;
+        q.wgs = q.lpg < 256 && per <= 128 && 256 % per == 0 ? 256 / per : 1;
+        const int64_t want = std::max<int64_t>(262144 / ((int64_t)per), 1);
+        const int64_t most = (int64_t)std::max((N + 7) / 8, std::min(N, 16)) * q.wgs;
+        q.RS = (int)std::min<int64_t>(want, backward ? std::min<int64_t>(most, N) : N);
+        q.chan_rows = q.wgs > 1 ? (q.RS + q.wgs - 1) / q.wgs : q.RS;
+        q.chan_floats = backward ? 2 * q.chan_rows * C : 0;
         return q;
     }
     const int max_cb = 256 * E;
@@ -920,7 +957,7 @@ static void ov_gn_fwd_go(const void* x, const OvGn& p, OvGnPlan q, void* y, floa
     const T* xt = static_cast<const T*>(x);
     T* yt = static_cast<T*>(y);
     q.t.part = static_cast<float*>(ws);
-    constexpr int NVX = 16 / OvVec<T>::N;
+    constexpr int NVX = 16 / OvGnPiece<T>::N;
     if (q.form == OV_GN_ROW) {
 #define OV_GO(L, V)                                                                                                                              \
     hipLaunchKernelGGL((ov_gn_row_fwd_kernel<T, L, V, LIGHT>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
@@ -974,7 +1011,7 @@ static void ov_gn_bwd_go(const void* dy, const void* x, const OvGn& p, OvGnPlan 
     T* dxt = static_cast<T*>(dx);
     q.t.part = static_cast<float*>(ws);
     float* chan = dw || db ? static_cast<float*>(ws) + (q.part_floats + 63) / 64 * 64 : nullptr;
-    constexpr int NVX = 16 / OvVec<T>::N;
+    constexpr int NVX = 16 / OvGnPiece<T>::N;
     if (q.form == OV_GN_ANY) {
         hipLaunchKernelGGL(ov_gn_any_dx_kernel<T>, dim3((unsigned)((int64_t)p.N * p.groups)), dim3(1024), 0, st, dt, xt, p, mean, rstd, dxt);
         if (dw || db) hipLaunchKernelGGL(ov_gn_any_param_kernel<T>, dim3((p.C + 63) / 64), dim3(1024), 0, st, dt, xt, p, mean, rstd, dw, db);
@@ -983,7 +1020,7 @@ static void ov_gn_bwd_go(const void* dy, const void* x, const OvGn& p, OvGnPlan 
     if (q.form == OV_GN_ROW) {
 #define OV_GO(L, V)                                                                                                                              \
     hipLaunchKernelGGL((ov_gn_row_bwd_kernel<T, L, V, LIGHT>), dim3((unsigned)(((int64_t)q.RS * p.groups * L + (L < 256 ? 256 : L) - 1) / (L < 256 ? 256 : L))), \
-                       dim3(L < 256 ? 256 : L), 0, st, dt, xt, p, q.RS, mean, rstd, dxt, chan)
+                       dim3(L < 256 ? 256 : L), 0, st, dt, xt, p, q.RS, q.wgs, mean, rstd, dxt, chan)
         OV_GN_ROW_SWITCH(OV_GO)
 #undef OV_GO
     } else {

@@ -3,6 +3,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "ontovae_ops.h"
 #include "ontovae_dropout.h"
