@@ -43,7 +43,9 @@ __device__ __forceinline__ void ov_gn_params(const void* p, int wtype, int c, in
 #pragma unroll
     for (int j = 0; j < E; ++j) f[j] = j < cnt ? none : 0.f;
     if (!p) return;
-    if (wtype == ONTOVAE_F32) {
+    if (wtype == ONTOVAE_F32 && cnt >= E) {
+        __builtin_memcpy(f, static_cast<const float*>(p) + c, sizeof(f));
+    } else if (wtype == ONTOVAE_F32) {
 #pragma unroll
         for (int j = 0; j < E; ++j) f[j] = static_cast<const float*>(p)[c + min(j, max(cnt - 1, 0))];
     } else if (wtype == ONTOVAE_BF16) {
@@ -886,7 +888,7 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         // fit it, else a slot's) is written and read once more: at most one to 8 samples
         const int per = groups * q.lpg;
         q.wgs = q.lpg < 256 && per <= 128 && 256 % per == 0 ? 256 / per : 1;
-        const int64_t want = std::max<int64_t>(262144 / ((int64_t)per), 1);
+        const int64_t want = std::max<int64_t>(262144 / (int64_t)per, 1);
         const int64_t most = (int64_t)std::max((N + 7) / 8, std::min(N, 16)) * q.wgs;
         q.RS = (int)std::min<int64_t>(want, backward ? std::min<int64_t>(most, N) : N);
         q.chan_rows = q.wgs > 1 ? (q.RS + q.wgs - 1) / q.wgs : q.RS;

@@ -33,11 +33,11 @@ struct OvVec {
     }
 };
 
-// waits until at most N vector-memory operations of the wave are outstanding
+// waits until at most N vector-memory operations of the wave are outstanding, and its LDS operations are done
 template <int N>
 __device__ __forceinline__ void ov_wait_vm() {
     static_assert(N < 64, "the counter holds 63");
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
 __device__ __forceinline__ uint32_t ov_wave_max_u(uint32_t v) {

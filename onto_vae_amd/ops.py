@@ -111,6 +111,8 @@ def quantize_rows(x, rows=None):
     M = xm.shape[0] if rows is None else rows.shape[0]
     lead = tuple(x.shape[:-1]) if rows is None else (M,)
     ldq = max((K + 63) // 64 * 64, 64)
+    if ldq % 1024 == 0:          # rows a multiple of 1024 bytes apart meet in the same memory channels
+        ldq += 128
     with _on(x.device):
         q = torch.empty(M, ldq, dtype=torch.int8, device=x.device)
         scale = torch.empty(M, dtype=torch.float32, device=x.device)
