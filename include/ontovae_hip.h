@@ -223,8 +223,8 @@ typedef struct ontovae_ctx {
     uint32_t flags;            /* ONTOVAE_FLAG_*: force the general-purpose kernel variants (tests) */
     ontovae_sell_t sell_fwd;   /* n_slices == 0: not provided, the per-level kernels run instead */
     ontovae_sell_t sell_bwd;
-    /* operand copies of the bf16-MFMA variant (ONTOVAE_FLAG_BF16_GEMM): ontovae_bf16_workspace_bytes(dims, max_batch) bytes of
-     * device memory, 256-B aligned; NULL / 0 otherwise */
+    /* operand copies of the reduced-precision variants, 256-B aligned device memory: ontovae_bf16_workspace_bytes(dims, max_batch)
+     * bytes with ONTOVAE_FLAG_BF16_GEMM, ontovae_int8_workspace_bytes with ONTOVAE_FLAG_INT8_ENCODER; NULL / 0 otherwise */
     void* bf16_ws;
     int64_t bf16_ws_bytes;
     ontovae_gsell_t gsell;     /* n_slices == 0: not provided */
@@ -250,6 +250,11 @@ typedef struct ontovae_ctx {
                                            gene kernel without its LDS accumulators, the term layers' weight gradient from riders of the latent backward
                                            instead of the per-level backward kernels (the path of an ontology whose tiles do not fit the accumulators;
                                            tests compare the two) */
+/* Inference passes (ontovae_forward with train == 0, ontovae_eval_step, ontovae_pass_data, ontovae_encode_pre) take the encoder's first
+ * product x W0^T in 8-bit integers, one scale per row of x and of W0, sums exact (ontovae_int8_linear; W0 is quantised in every pass).
+ * Training passes stay float32.  Each operand is off by at most half a step of its row's max / 127.  Needs ctx->bf16_ws of
+ * ontovae_int8_workspace_bytes; excludes ONTOVAE_FLAG_BF16_GEMM. */
+#define ONTOVAE_FLAG_INT8_ENCODER 256u
 #define ONTOVAE_FLAG_NO_RIDERS     16u  /* weight gradient of the gene rows as its own launch instead of inside the backward chain's */
 #define ONTOVAE_FLAG_SIDE_STREAM    4u  /* run the decoder weight gradient and dWh on a library-owned second stream, forked from
                                            and joined into the caller's stream with events (off by default: on this pool the event
@@ -263,6 +268,7 @@ int64_t ontovae_workspace_bytes(const ontovae_dims_t* dims, int32_t max_batch);
  * ontovae_forward with train != 0) refuse more rows. */
 int64_t ontovae_workspace_bytes_split(const ontovae_dims_t* dims, int32_t max_batch, int32_t max_train_batch);
 int64_t ontovae_bf16_workspace_bytes(const ontovae_dims_t* dims, int32_t max_batch);
+int64_t ontovae_int8_workspace_bytes(const ontovae_dims_t* dims, int32_t max_batch);
 
 /* AdamW hyper-parameters of one step, pre-folded on the host in double like torch does
  * (torch.optim.AdamW defaults at onto_vae/vae_model.py:251). */
@@ -549,6 +555,29 @@ int ontovae_vae_decode_forward(const ontovae_vae_ctx_t* ctx, const float* heads,
 int ontovae_vae_decode_step(const ontovae_vae_ctx_t* ctx, const float* heads, const float* x, const int32_t* xidx, int32_t B,
                             const float* eps, uint64_t rng_offset, float kl_coeff, const ontovae_adamw_t* opt, int32_t apply_update,
                             float* dheads_out, float* loss_out, void* stream);
+/* The same two entry points for blocks of another kind; no counterpart in the reference, whose blocks are
+ * [Linear, BatchNorm1d, Dropout, ReLU] (modules.py:43-64, 116-133):
+ *   groups > 0: group norm over the block's units in place of BatchNorm1d (groups divides every width; gamma and beta are the
+ *     block's, bn_state and bn_nbt are not touched): ontovae_group_norm_act with its activation and dropout.  The rows of a batch
+ *     are then independent: a batch may have one row, training and inference normalise alike.
+ *   input_drop > 0: training passes feed the encoder the batch's rows after ontovae_dropout (denoising); the loss still compares with x.
+ *   ONTOVAE_VAE_FLAG_INT8_INPUT: inference passes take the first layer's product in 8 bits (ontovae_int8_linear).
+ * workspace: ontovae_vae_ext_workspace_bytes(dims, ext, max_batch), 256-B aligned.  ext == NULL: the plain entry points. */
+#define ONTOVAE_VAE_FLAG_INT8_INPUT 1u
+typedef struct ontovae_vae_ext {
+    int32_t groups;
+    float input_drop;
+    uint32_t flags;
+    int32_t reserved;          /* 0 */
+    void* workspace; int64_t workspace_bytes;
+} ontovae_vae_ext_t;
+int64_t ontovae_vae_ext_workspace_bytes(const ontovae_vae_dims_t* dims, const ontovae_vae_ext_t* ext, int32_t max_batch);
+int ontovae_vae_train_step_ext(const ontovae_vae_ctx_t* ctx, const ontovae_vae_ext_t* ext, const float* x, const int32_t* xidx, int32_t B,
+                               const float* eps, uint64_t rng_offset, float kl_coeff, const ontovae_adamw_t* opt, int32_t apply_update,
+                               float* loss_out, void* stream);
+int ontovae_vae_forward_ext(const ontovae_vae_ctx_t* ctx, const ontovae_vae_ext_t* ext, const float* x, const int32_t* xidx, int32_t B,
+                            const float* eps, uint64_t rng_offset, int32_t train, float kl_coeff, float* recon, float* mu, float* log_var,
+                            float* z_out, float* loss_out, void* stream);
 /* torch.optim.AdamW.step over the flat buffers with gradients from ctx->Gr (after apply_update == 0). */
 int ontovae_vae_adamw_apply(const ontovae_vae_ctx_t* ctx, const ontovae_adamw_t* opt, void* stream);
 

@@ -80,6 +80,11 @@ class AdamW(C.Structure):
     _fields_ = [(n, C.c_float) for n in ("decay_mul", "one_m_beta1", "beta2", "one_m_beta2", "step_size", "bc2_sqrt", "eps")]
 
 
+class VaeExt(C.Structure):
+    _fields_ = [("groups", C.c_int32), ("input_drop", C.c_float), ("flags", C.c_uint32), ("reserved", C.c_int32), ("workspace", C.c_void_p),
+                ("workspace_bytes", C.c_int64)]
+
+
 class OntoVAEHipError(RuntimeError):
     pass
 
@@ -145,6 +150,8 @@ def lib():
         "ontovae_vae_layout": [C.POINTER(VaeDims), C.POINTER(VaeLayout)],
         "ontovae_vae_train_step": [C.POINTER(VaeCtx), vp, vp, i32, vp, u64, f32, C.POINTER(AdamW), i32, vp, vp],
         "ontovae_vae_forward": [C.POINTER(VaeCtx), vp, vp, i32, vp, u64, i32, f32, vp, vp, vp, vp, vp, vp],
+        "ontovae_vae_train_step_ext": [C.POINTER(VaeCtx), C.POINTER(VaeExt), vp, vp, i32, vp, u64, f32, C.POINTER(AdamW), i32, vp, vp],
+        "ontovae_vae_forward_ext": [C.POINTER(VaeCtx), C.POINTER(VaeExt), vp, vp, i32, vp, u64, i32, f32, vp, vp, vp, vp, vp, vp],
         "ontovae_vae_adamw_apply": [C.POINTER(VaeCtx), C.POINTER(AdamW), vp],
         "ontovae_vae_decode_forward": [C.POINTER(VaeCtx), vp, vp, vp, i32, vp, u64, i32, f32, vp, vp, vp, vp, vp, vp],
         "ontovae_vae_decode_step": [C.POINTER(VaeCtx), vp, vp, vp, i32, vp, u64, f32, C.POINTER(AdamW), i32, vp, vp, vp],
@@ -167,13 +174,15 @@ def lib():
         fn.restype = C.c_int
     L.ontovae_plan_destroy.argtypes = [vp]
     L.ontovae_plan_destroy.restype = None
-    for name in ("ontovae_workspace_bytes", "ontovae_bf16_workspace_bytes"):
+    for name in ("ontovae_workspace_bytes", "ontovae_bf16_workspace_bytes", "ontovae_int8_workspace_bytes"):
         getattr(L, name).argtypes = [C.POINTER(Dims), i32]
         getattr(L, name).restype = C.c_int64
     L.ontovae_workspace_bytes_split.argtypes = [C.POINTER(Dims), i32, i32]
     L.ontovae_workspace_bytes_split.restype = C.c_int64
     L.ontovae_vae_workspace_bytes.argtypes = [C.POINTER(VaeDims), i32]
     L.ontovae_vae_workspace_bytes.restype = C.c_int64
+    L.ontovae_vae_ext_workspace_bytes.argtypes = [C.POINTER(VaeDims), C.POINTER(VaeExt), i32]
+    L.ontovae_vae_ext_workspace_bytes.restype = C.c_int64
     for name in ("ontovae_wilcoxon_workspace_bytes", "ontovae_fdr_workspace_bytes"):
         getattr(L, name).argtypes = [i32, i32]
         getattr(L, name).restype = C.c_int64
@@ -189,13 +198,14 @@ def lib():
 EXPORTED = ["ontovae_last_error", "ontovae_abi_version", "ontovae_plan_create", "ontovae_plan_create_from_links",
             "ontovae_plan_destroy", "ontovae_plan_dims", "ontovae_plan_levels", "ontovae_plan_export",
             "ontovae_plan_entry_coords", "ontovae_plan_csc_split", "ontovae_plan_row_k", "ontovae_plan_sell_sizes", "ontovae_plan_sell_export", "ontovae_plan_gsell_sizes", "ontovae_plan_gsell_export", "ontovae_plan_tile_info", "ontovae_plan_layer_node0", "ontovae_plan_unpack_mask", "ontovae_param_layout",
-            "ontovae_workspace_bytes", "ontovae_workspace_bytes_split", "ontovae_bf16_workspace_bytes", "ontovae_forward", "ontovae_train_step", "ontovae_train_step_dp",
+            "ontovae_workspace_bytes", "ontovae_workspace_bytes_split", "ontovae_bf16_workspace_bytes", "ontovae_int8_workspace_bytes", "ontovae_forward", "ontovae_train_step", "ontovae_train_step_dp",
             "ontovae_adamw_apply", "ontovae_adamw_apply_range", "ontovae_dp_bn_bwd", "ontovae_dw0_rows", "ontovae_dw0_global", "ontovae_dp_pack_dy", "ontovae_dp_dh_global", "ontovae_eval_step", "ontovae_pass_data", "ontovae_decoder_forward",
             "ontovae_encode_pre", "ontovae_pass_data_perturbed",
             "ontovae_compose_order", "ontovae_gather_rows", "ontovae_vals_to_dense", "ontovae_dense_to_vals",
             "ontovae_wilcoxon_workspace_bytes", "ontovae_wilcoxon_zsplit", "ontovae_fdr_workspace_bytes", "ontovae_fdr_bh", "ontovae_fdr_bh_static",
             "ontovae_to_feature_major",
             "ontovae_vae_layout", "ontovae_vae_workspace_bytes", "ontovae_vae_train_step", "ontovae_vae_forward", "ontovae_vae_adamw_apply",
+            "ontovae_vae_ext_workspace_bytes", "ontovae_vae_train_step_ext", "ontovae_vae_forward_ext",
             "ontovae_vae_decode_forward", "ontovae_vae_decode_step", "ontovae_decoder_backward", "ontovae_decoder_forward_train",
             "ontovae_quantize_rows", "ontovae_int8_matmul_workspace_bytes", "ontovae_int8_matmul", "ontovae_int8_linear_workspace_bytes",
             "ontovae_int8_linear", "ontovae_group_norm_act_workspace_bytes",
@@ -203,6 +213,8 @@ EXPORTED = ["ontovae_last_error", "ontovae_abi_version", "ontovae_plan_create", 
             "ontovae_profile_begin", "ontovae_profile_read", "ontovae_profile_end", "ontovae_profile_overhead"]
 
 FLAG_BF16_GEMM = 32
+FLAG_INT8_ENCODER = 256      # inference passes: x W0^T in 8-bit integers (ontovae_int8_linear)
+VAE_FLAG_INT8_INPUT = 1      # the same for the plain VAE's first layer (VaeExt.flags)
 FLAG_PER_BLOCK_WGRAD = 64    # decoder weight-gradient partials per column block everywhere (no LDS accumulators, no level-kernel weight gradient)
 FLAG_CB_GENE_FWD = 128       # training forward of the gene layer on 32-column blocks instead of the LDS-panel kernel (tests compare the two)
 

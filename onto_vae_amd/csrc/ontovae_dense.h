@@ -206,6 +206,86 @@ __global__ __launch_bounds__(256) void ov_vae_slabsum_kernel(const float* __rest
     }
 }
 
+// ---- blocks with group norm, input dropout, a first layer in 8 bits (ontovae_vae_ext_t)
+struct OvVaeExtWs {
+    float *xin, *row, *drow, *dpar;                  // [B, G]; a block's rows [B, F] (activations, gradients); its gradient sums [2, F]
+    float *h[2 * OV_VAE_MAXL], *mean[2 * OV_VAE_MAXL], *rstd[2 * OV_VAE_MAXL];     // by bn_index: what the norm read, its statistics
+    void *gn, *i8;
+    int64_t gn_bytes, i8_bytes;
+};
+static int64_t ov_vae_ext_carve(const OvVaeNet& n, const ontovae_vae_ext_t& e, int max_batch, void* base, OvVaeExtWs* out) {
+    int64_t off = 0;
+    auto take = [&](int64_t bytes) {
+        char* p = base ? static_cast<char*>(base) + off : nullptr;
+        off += (bytes + 255) / 256 * 256;
+        return reinterpret_cast<float*>(p);
+    };
+    OvVaeExtWs w{};
+    if (e.input_drop > 0.f) w.xin = take(4LL * max_batch * n.G);
+    if (e.groups > 0) {
+        w.row = take(4LL * max_batch * n.fmax);
+        w.drow = take(4LL * max_batch * n.fmax);
+        w.dpar = take(8LL * n.fmax);
+        auto per = [&](const OvVaeLayer& l) {
+            w.h[l.bn_index] = take(4LL * max_batch * l.out);
+            w.mean[l.bn_index] = take(4LL * max_batch * e.groups);
+            w.rstd[l.bn_index] = take(4LL * max_batch * e.groups);
+            // S = 1: grows with the batch
+            w.gn_bytes = std::max(w.gn_bytes, ontovae_group_norm_act_workspace_bytes(ONTOVAE_F32, max_batch, 1, l.out, e.groups, 1));
+        };
+        for (int i = 0; i < n.ne; ++i) per(n.enc[i]);
+        for (int i = 0; i < n.nd; ++i) per(n.dec[i]);
+        w.gn = take(w.gn_bytes);
+    }
+    if (e.flags & ONTOVAE_VAE_FLAG_INT8_INPUT) {
+        w.i8_bytes = ov_int8_need_upto(n.enc[0].out, n.G, max_batch);
+        w.i8 = take(w.i8_bytes);
+    }
+    if (out) *out = w;
+    return off;
+}
+
+static int ov_vae_ext_check(const OvVaeNet& n, const ontovae_vae_ext_t* e) {
+    if (e->groups < 0 || !(e->input_drop >= 0.f && e->input_drop < 1.f) || (e->flags & ~ONTOVAE_VAE_FLAG_INT8_INPUT) || e->reserved) {
+        ontovae_set_error("vae ext: groups = %d, input_drop = %g, flags = 0x%x, reserved = %d", e->groups, (double)e->input_drop, e->flags, e->reserved);
+        return ONTOVAE_EINVAL;
+    }
+    for (int i = 0; e->groups > 0 && i < n.ne + n.nd; ++i) {
+        const int w = i < n.ne ? n.enc[i].out : n.dec[i - n.ne].out;
+        if (w % e->groups) { ontovae_set_error("vae ext: %d groups do not divide a block of %d units", e->groups, w); return ONTOVAE_EINVAL; }
+    }
+    return ONTOVAE_OK;
+}
+
+extern "C" int64_t ontovae_vae_ext_workspace_bytes(const ontovae_vae_dims_t* dims, const ontovae_vae_ext_t* ext, int32_t max_batch) {
+    if (!dims || !ext || max_batch < 1) return -1;
+    OvVaeNet n;
+    if (ov_vae_net(*dims, &n) || ov_vae_ext_check(n, ext)) return -1;
+    return ov_vae_ext_carve(n, *ext, max_batch, nullptr, nullptr);
+}
+
+// sum of split-K slabs [S][F, ldb] + bias -> rows [B, F]: 32 x 32 tiles turned through LDS
+__global__ __launch_bounds__(256) void ov_vae_slab_rows_kernel(const float* __restrict__ slab, int S, int64_t stride, const float* __restrict__ bias,
+                                                              int F, int B, int ldb, float* __restrict__ rows) {
+    __shared__ float tile[32][33];
+    const int f0 = blockIdx.x * 32, b0 = blockIdx.y * 32;
+    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
+    for (int j = ty; j < 32; j += 8) {
+        const int f = f0 + j, b = b0 + tx;
+        float v = 0.f;
+        if (f < F && b < B) {
+            for (int q = 0; q < S; ++q) v += slab[q * stride + (int64_t)f * ldb + b];
+            if (bias) v += bias[f];
+        }
+        tile[j][tx] = v;
+    }
+    __syncthreads();
+    for (int j = ty; j < 32; j += 8) {
+        const int b = b0 + j, f = f0 + tx;
+        if (f < F && b < B) rows[(int64_t)b * F + f] = tile[tx][j];
+    }
+}
+
 struct OvVaeStep {
     const ontovae_vae_ctx_t* c;
     OvVaeNet n;
@@ -215,9 +295,15 @@ struct OvVaeStep {
     const float* x; const int32_t* xidx;
     OvAdam adam; int apply;
     uint64_t rng_off;
+    const float* xin; const int32_t* xin_idx;        // what the encoder reads: x, or its rows after dropout
+    int groups;                                      // group norm in place of BatchNorm; 0: BatchNorm
+    float input_drop;
+    bool int8;                                       // the first layer of inference passes in 8 bits
+    OvVaeExtWs ext;
 };
 
-static int ov_vae_check(const ontovae_vae_ctx_t* c, int B, bool need_opt, OvVaeStep* s, const float* x, const int32_t* xidx, void* stream) {
+static int ov_vae_check(const ontovae_vae_ctx_t* c, int B, bool need_opt, OvVaeStep* s, const float* x, const int32_t* xidx, void* stream,
+                        const ontovae_vae_ext_t* ext = nullptr) {
     if (!c || !c->P || !c->bn_state || !c->bn_nbt || !c->workspace) { ontovae_set_error("vae ctx: a required pointer is NULL"); return ONTOVAE_EINVAL; }
     int rc = ov_vae_net(c->dims, &s->n);
     if (rc) return rc;
@@ -233,7 +319,27 @@ static int ov_vae_check(const ontovae_vae_ctx_t* c, int B, bool need_opt, OvVaeS
     ov_vae_carve(s->n, c->max_batch, c->workspace, &s->ws);
     s->c = c; s->B = B; s->ldb = ov_ldb(B); s->st = reinterpret_cast<hipStream_t>(stream); s->x = x; s->xidx = xidx;
     s->adam = OvAdam{}; s->apply = 0; s->rng_off = 0;
+    s->xin = x; s->xin_idx = xidx;
+    s->groups = 0; s->input_drop = 0.f; s->int8 = false; s->ext = OvVaeExtWs{};
+    if (ext) {
+        if ((rc = ov_vae_ext_check(s->n, ext))) return rc;
+        const int64_t need = ov_vae_ext_carve(s->n, *ext, c->max_batch, nullptr, nullptr);
+        if (need > 0 && (!ext->workspace || ext->workspace_bytes < need || (reinterpret_cast<uintptr_t>(ext->workspace) & 255))) {
+            ontovae_set_error("vae ext: workspace of %lld bytes, 256-B aligned, required", (long long)need);
+            return ONTOVAE_EINVAL;
+        }
+        ov_vae_ext_carve(s->n, *ext, c->max_batch, ext->workspace, &s->ext);
+        s->groups = ext->groups; s->input_drop = ext->input_drop; s->int8 = (ext->flags & ONTOVAE_VAE_FLAG_INT8_INPUT) != 0;
+    }
     return ONTOVAE_OK;
+}
+
+// the rows the encoder of a training pass reads: the batch after dropout
+static int ov_vae_input(OvVaeStep& s) {
+    if (s.input_drop <= 0.f) return ONTOVAE_OK;
+    int rc = ontovae_dropout(s.x, ONTOVAE_F32, s.n.G, s.xidx, s.xidx ? INT32_MAX : s.B, s.B, s.n.G, s.input_drop, s.c->seed, s.rng_off, s.ext.xin, s.st);
+    s.xin = s.ext.xin; s.xin_idx = nullptr;
+    return rc;
 }
 
 static inline uint64_t ov_vae_layer_off(uint64_t rng_off, int bn_index) { return rng_off ^ ((uint64_t)(bn_index + 1) << 48); }
@@ -246,7 +352,7 @@ static int ov_vae_linear_fwd(OvVaeStep& s, const OvVaeLayer& l, const float* W, 
     g.C = s.ws.slab; g.ldc = s.ldb; g.slab_stride = (int64_t)l.out * s.ldb;
     int S;
     if (!prev) {
-        g.B = s.x; g.ldb = l.in; g.bgather = s.xidx;
+        g.B = s.xin; g.ldb = l.in; g.bgather = s.xin_idx;
         const int tiles = ((l.out + 95) / 96) * ((s.B + 127) / 128);
         S = ov_vae_split(tiles, l.in, 512);
         S = (int)std::min<int64_t>(S, std::max<int64_t>(1, s.ws.slab_floats / g.slab_stride));
@@ -269,8 +375,23 @@ static int ov_vae_linear_fwd(OvVaeStep& s, const OvVaeLayer& l, const float* W, 
 static int ov_vae_block_fwd(OvVaeStep& s, const OvVaeLayer& l, const float* prev, int train) {
     const ontovae_vae_ctx_t* c = s.c;
     int S = 1, rc;
-    if ((rc = ov_vae_linear_fwd(s, l, c->P + l.W, prev, &S))) return rc;
+    if (!prev && s.int8 && !train) {
+        if ((rc = ov_int8_first_layer(c->P + l.W, l.out, l.in, s.xin, l.in, s.xin_idx, s.B, s.ldb, s.ext.i8, s.ext.i8_bytes, s.ws.slab, s.st))) return rc;
+    } else if ((rc = ov_vae_linear_fwd(s, l, c->P + l.W, prev, &S))) return rc;
     const int k = l.bn_index;
+    if (s.groups > 0) {
+        // rows in sample-major form for the operator: relu and dropout commute, so the order [norm, dropout, relu] is kept
+        const dim3 grid((l.out + 31) / 32, (s.B + 31) / 32);
+        hipLaunchKernelGGL(ov_vae_slab_rows_kernel, grid, dim3(256), 0, s.st, s.ws.slab, S, (int64_t)l.out * s.ldb, c->P + l.b, l.out, s.B, s.ldb, s.ext.h[k]);
+        OV_LAUNCH_CHECK();
+        if ((rc = ontovae_group_norm_act(s.ext.h[k], ONTOVAE_F32, s.B, 1, l.out, s.groups, c->P + l.gamma, c->P + l.beta, ONTOVAE_F32, 1e-5f,
+                                         ONTOVAE_ACT_RELU, train ? c->drop : 0.f, c->seed, ov_vae_layer_off(s.rng_off, k), s.ext.row, s.ext.mean[k],
+                                         s.ext.rstd[k], s.ext.gn, s.ext.gn_bytes, s.st)))
+            return rc;
+        hipLaunchKernelGGL(ov_transpose_in_kernel, dim3((l.out + 31) / 32, (s.ldb + 31) / 32), dim3(256), 0, s.st, s.ext.row, l.out, s.B, s.ldb, s.ws.a[k]);
+        OV_LAUNCH_CHECK();
+        return ONTOVAE_OK;
+    }
     hipLaunchKernelGGL(ov_bn_fwd_kernel, dim3(l.out), dim3(256), 0, s.st, s.ws.slab, S, (int64_t)l.out * s.ldb, c->P + l.b, c->P + l.gamma,
                        c->P + l.beta, c->bn_state + l.bn, c->bn_state + l.bn + l.out, c->bn_nbt + k, s.ws.xhat[k], s.ws.a[k], s.ws.mean[k],
                        s.ws.invstd[k], (float*)nullptr, l.out, s.B, s.B, s.ldb, train ? 1 : 0, c->drop, c->seed, ov_vae_layer_off(s.rng_off, k));
@@ -379,7 +500,7 @@ static int ov_vae_dw(OvVaeStep& s, int64_t Woff, int out, int in, const float* d
     if (s.apply) { g.C = c->P + Woff; g.Pm = c->M + Woff; g.Pv = c->V + Woff; }
     else g.C = c->Gr + Woff;
     if (!prev) {
-        g.B = s.x; g.ldb = in; g.bgather = s.xidx;          // B(k = b, n = g) = X[row(b) * G + g]
+        g.B = s.xin; g.ldb = in; g.bgather = s.xin_idx;     // B(k = b, n = g) = X[row(b) * G + g]
         if (s.apply) return ov_launch_gemm<1, 4, 1, 2, true, false, OV_EPI_ADAMW>(g, 1, true, s.st);
         return ov_launch_gemm<1, 4, 1, 2, true, false, OV_EPI_STORE>(g, 1, true, s.st);
     }
@@ -395,15 +516,40 @@ static int ov_vae_block_bwd(OvVaeStep& s, const OvVaeLayer& l, const float* ga, 
     const ontovae_vae_ctx_t* c = s.c;
     const int k = l.bn_index;
     float* Gr = c->Gr;
-    const OvBnBwdArgs bn{ga, s.ws.a[k], s.ws.xhat[k], s.ws.invstd[k], c->P + l.gamma, c->P + l.beta, c->P + l.b,
+    int rc;
+    if (s.groups > 0) {
+        const dim3 grid((l.out + 31) / 32, (s.B + 31) / 32);
+        hipLaunchKernelGGL(ov_vae_slab_rows_kernel, grid, dim3(256), 0, s.st, ga, daS, (int64_t)l.out * s.ldb, (const float*)nullptr, l.out, s.B, s.ldb,
+                           s.ext.drow);
+        OV_LAUNCH_CHECK();
+        float* dw = s.apply ? s.ext.dpar : Gr + l.gamma;
+        float* db = s.apply ? s.ext.dpar + l.out : Gr + l.beta;
+        if ((rc = ontovae_group_norm_act_backward(s.ext.drow, s.ext.h[k], ONTOVAE_F32, s.B, 1, l.out, s.groups, c->P + l.gamma, c->P + l.beta,
+                                                  ONTOVAE_F32, s.ext.mean[k], s.ext.rstd[k], ONTOVAE_ACT_RELU, c->drop, c->seed,
+                                                  ov_vae_layer_off(s.rng_off, k), s.ext.row, dw, db, s.ext.gn, s.ext.gn_bytes, s.st)))
+            return rc;
+        hipLaunchKernelGGL(ov_transpose_in_kernel, dim3((l.out + 31) / 32, (s.ldb + 31) / 32), dim3(256), 0, s.st, s.ext.row, l.out, s.B, s.ldb, s.ws.dh);
+        OV_LAUNCH_CHECK();
+        if (s.apply)
+            for (int h = 0; h < 2; ++h) {
+                const int64_t o = h ? l.beta : l.gamma;
+                hipLaunchKernelGGL(ov_adamw_flat_kernel, dim3((l.out + 255) / 256), dim3(256), 0, s.st, c->P + o, c->M + o, c->V + o,
+                                   s.ext.dpar + h * l.out, (int64_t)l.out, (int64_t)-1, (int64_t)-1, s.adam);
+                OV_LAUNCH_CHECK();
+            }
+        hipLaunchKernelGGL(ov_vae_rowsum_kernel, dim3((l.out + 3) / 4), dim3(256), 0, s.st, s.ws.dh, l.out, s.B, s.ldb, c->P + l.b,
+                           c->M ? c->M + l.b : nullptr, c->V ? c->V + l.b : nullptr, Gr ? Gr + l.b : nullptr, s.apply, s.adam);
+        OV_LAUNCH_CHECK();
+    } else {
+        const OvBnBwdArgs bn{ga, s.ws.a[k], s.ws.xhat[k], s.ws.invstd[k], c->P + l.gamma, c->P + l.beta, c->P + l.b,
                          c->M ? c->M + l.gamma : nullptr, c->M ? c->M + l.beta : nullptr, c->M ? c->M + l.b : nullptr,
                          c->V ? c->V + l.gamma : nullptr, c->V ? c->V + l.beta : nullptr, c->V ? c->V + l.b : nullptr,
                          Gr ? Gr + l.gamma : nullptr, Gr ? Gr + l.beta : nullptr, Gr ? Gr + l.b : nullptr, s.ws.dh, s.ws.bwd_local,
                          (float*)nullptr, l.out, s.B, s.B, s.ldb, 1, s.apply, s.adam, c->drop, c->seed, ov_vae_layer_off(s.rng_off, k), daS,
                          (int64_t)l.out * s.ldb, nullptr, 0};
-    hipLaunchKernelGGL(ov_bn_bwd_kernel, dim3(l.out), dim3(256), 0, s.st, bn);
-    OV_LAUNCH_CHECK();
-    int rc;
+        hipLaunchKernelGGL(ov_bn_bwd_kernel, dim3(l.out), dim3(256), 0, s.st, bn);
+        OV_LAUNCH_CHECK();
+    }
     if (dprev && (rc = ov_vae_da(s, c->P + l.W, l.out, l.in, s.ws.dh, dprev, S_out, keep_slabs))) return rc;    // before W is updated
     return ov_vae_dw(s, l.W, l.out, l.in, s.ws.dh, prev);
 }
@@ -438,16 +584,23 @@ static int ov_vae_decoder_bwd(OvVaeStep& s, int* nrec) {
 extern "C" int ontovae_vae_train_step(const ontovae_vae_ctx_t* ctx, const float* x, const int32_t* xidx, int32_t B, const float* eps,
                                       uint64_t rng_offset, float kl_coeff, const ontovae_adamw_t* opt, int32_t apply_update,
                                       float* loss_out, void* stream) {
+    return ontovae_vae_train_step_ext(ctx, nullptr, x, xidx, B, eps, rng_offset, kl_coeff, opt, apply_update, loss_out, stream);
+}
+
+extern "C" int ontovae_vae_train_step_ext(const ontovae_vae_ctx_t* ctx, const ontovae_vae_ext_t* ext, const float* x, const int32_t* xidx, int32_t B,
+                                          const float* eps, uint64_t rng_offset, float kl_coeff, const ontovae_adamw_t* opt, int32_t apply_update,
+                                          float* loss_out, void* stream) {
     OvVaeStep s;
-    int rc = ov_vae_check(ctx, B, apply_update != 0, &s, x, xidx, stream);
+    int rc = ov_vae_check(ctx, B, apply_update != 0, &s, x, xidx, stream, ext);
     if (rc) return rc;
     if (!loss_out) { ontovae_set_error("vae_train_step: loss_out is NULL"); return ONTOVAE_EINVAL; }
     if (apply_update && !opt) { ontovae_set_error("vae_train_step: opt is NULL"); return ONTOVAE_EINVAL; }
     if (!apply_update && !ctx->Gr) { ontovae_set_error("vae_train_step: gradient buffer Gr is NULL"); return ONTOVAE_EINVAL; }
-    if (B < 2) { ontovae_set_error("vae_train_step: BatchNorm in train mode needs more than 1 sample per batch"); return ONTOVAE_EINVAL; }
+    if (B < 2 && s.groups == 0) { ontovae_set_error("vae_train_step: BatchNorm in train mode needs more than 1 sample per batch"); return ONTOVAE_EINVAL; }
     s.adam = ov_adam_from(opt); s.apply = apply_update ? 1 : 0; s.rng_off = rng_offset;
     const OvVaeNet& n = s.n;
     int nkl = 0, nrec = 0;
+    if ((rc = ov_vae_input(s))) return rc;
     if ((rc = ov_vae_forward_core(s, eps, 1, 1, &nkl))) return rc;
     if ((rc = ov_vae_decoder_bwd(s, &nrec))) return rc;
     int daS = 1;
@@ -479,13 +632,20 @@ extern "C" int ontovae_vae_train_step(const ontovae_vae_ctx_t* ctx, const float*
 extern "C" int ontovae_vae_forward(const ontovae_vae_ctx_t* ctx, const float* x, const int32_t* xidx, int32_t B, const float* eps,
                                    uint64_t rng_offset, int32_t train, float kl_coeff, float* recon, float* mu, float* log_var,
                                    float* z_out, float* loss_out, void* stream) {
+    return ontovae_vae_forward_ext(ctx, nullptr, x, xidx, B, eps, rng_offset, train, kl_coeff, recon, mu, log_var, z_out, loss_out, stream);
+}
+
+extern "C" int ontovae_vae_forward_ext(const ontovae_vae_ctx_t* ctx, const ontovae_vae_ext_t* ext, const float* x, const int32_t* xidx, int32_t B,
+                                       const float* eps, uint64_t rng_offset, int32_t train, float kl_coeff, float* recon, float* mu, float* log_var,
+                                       float* z_out, float* loss_out, void* stream) {
     OvVaeStep s;
-    int rc = ov_vae_check(ctx, B, false, &s, x, xidx, stream);
+    int rc = ov_vae_check(ctx, B, false, &s, x, xidx, stream, ext);
     if (rc) return rc;
-    if (train && B < 2) { ontovae_set_error("vae_forward: BatchNorm in train mode needs more than 1 sample per batch"); return ONTOVAE_EINVAL; }
+    if (train && B < 2 && s.groups == 0) { ontovae_set_error("vae_forward: BatchNorm in train mode needs more than 1 sample per batch"); return ONTOVAE_EINVAL; }
     s.rng_off = rng_offset;
     const OvVaeNet& n = s.n;
     int nkl = 0, nrec = 0;
+    if (train && (rc = ov_vae_input(s))) return rc;
     if ((rc = ov_vae_forward_core(s, eps, train ? 1 : 0, loss_out ? 1 : 0, &nkl, !recon && !loss_out))) return rc;
     OvStep t{};
     t.B = B; t.ldb = s.ldb; t.st = s.st;

@@ -605,7 +605,7 @@ static int ov_q8_gemm_launch(OvQ8Gemm g, const OvQ8Plan& p, bool direct, hipStre
         case OV_Q8_T32: return ov_q8_gemm_go<32, 128, 32, 32, 128, 4, true, T>(g, p.splits, st);
         case OV_Q8_T64: return ov_q8_gemm_go<64, 64, 32, 32, 128, 4, true, T>(g, p.splits, st);
         case OV_Q8_T128: return ov_q8_gemm_go<128, 128, 64, 64, 64, 4, true, T>(g, p.splits, st);
-        case OV_Q8_T192: return ov_q8_gemm_go<128, 192, 64, 96, 64, 7, true, T>(g, p.splits, st);
+        case OV_Q8_T192: return ov_q8_gemm_go<128, 192, 32, 96, 128, 3, true, T>(g, p.splits, st);
         default: return ov_q8_gemm_go<256, 256, 128, 64, 64, 4, true, T>(g, p.splits, st);
     }
 }
@@ -679,6 +679,18 @@ extern "C" int64_t ontovae_int8_linear_workspace_bytes(int32_t M, int32_t N, int
     if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K || ov_q8_few(M, K)) return 0;
     const int64_t head = (M * ov_q8_blocks(K) * 128 + 255) / 256 * 256 + ((int64_t)M * 4 + 255) / 256 * 256;
     return head + ontovae_int8_matmul_workspace_bytes(M, N, K);
+}
+
+// K is cut only where a form has t < 256 tiles, into at most 256 / t + 1 slabs of at most t whole tiles, and never below 4 steps
+int64_t ov_int8_linear_bytes_upto(int max_M, int N, int K) {
+    int64_t slabs = 0;
+    for (int c = 0; c < 5; ++c) {
+        const int64_t t = std::min<int64_t>((int64_t)((max_M + ov_q8_bm[c] - 1) / ov_q8_bm[c]) * ((N + ov_q8_bn[c] - 1) / ov_q8_bn[c]), 255);
+        slabs = std::max(slabs, (256 + t) * ov_q8_bm[c] * ov_q8_bn[c]);
+    }
+    const int64_t cuts = std::min<int64_t>(256, std::max((K + 127) / 128 / 4, 1));
+    slabs = std::min(slabs, cuts * max_M * N);
+    return (max_M * ov_q8_blocks(K) * 128 + 255) / 256 * 256 + ((int64_t)max_M * 4 + 255) / 256 * 256 + slabs * 4;
 }
 
 template <typename T, int MT>

@@ -25,7 +25,7 @@
 
 #define OV_LAUNCH_CHECK() OV_HIP_CHECK(hipGetLastError())
 
-#define OV_KNOWN_FLAGS (ONTOVAE_FLAG_LEVEL_LAUNCHES | ONTOVAE_FLAG_ROW_GENE_LAYER | ONTOVAE_FLAG_SIDE_STREAM | ONTOVAE_FLAG_WIDE_GENE_TILES | ONTOVAE_FLAG_NO_RIDERS | ONTOVAE_FLAG_BF16_GEMM | ONTOVAE_FLAG_CB_GENE_FWD | ONTOVAE_FLAG_PER_BLOCK_WGRAD)
+#define OV_KNOWN_FLAGS (ONTOVAE_FLAG_LEVEL_LAUNCHES | ONTOVAE_FLAG_ROW_GENE_LAYER | ONTOVAE_FLAG_SIDE_STREAM | ONTOVAE_FLAG_WIDE_GENE_TILES | ONTOVAE_FLAG_NO_RIDERS | ONTOVAE_FLAG_BF16_GEMM | ONTOVAE_FLAG_CB_GENE_FWD | ONTOVAE_FLAG_PER_BLOCK_WGRAD | ONTOVAE_FLAG_INT8_ENCODER)
 
 // batch columns per wave pass (64 lanes x VEC) and the padded row length, a multiple of it
 // -------------------------------------------------------------------------------------------------
@@ -176,6 +176,34 @@ static inline int ov_ldb(int B) {
     // gene layer 2250 -> 1290 us at B = 8192, whole step 9.8 -> 8.5 ms).  At most 6 % of padding columns.
     if (ldb >= 4096 && ((ldb >> 8) & 1) == 0) ldb += 256;
     return ldb;
+}
+
+// Workspace of a first layer in 8 bits (W [L, G], up to max_batch rows): the weight's rows and scales, the product sample-major,
+// and what ontovae_int8_linear asks for.
+struct OvI8Ws { int8_t* qw; float *sw, *h; void* lin; int64_t ldw, head; };
+static OvI8Ws ov_int8_carve(int L, int G, int B, void* base) {
+    OvI8Ws w{};
+    w.ldw = ((int64_t)G + 63) / 64 * 64;
+    if (w.ldw % 1024 == 0) w.ldw += 128;          // rows a multiple of 1024 bytes apart meet in the same memory channels
+    auto up = [](int64_t n) { return (n + 255) / 256 * 256; };
+    char* p = static_cast<char*>(base);
+    int64_t off = 0;
+    w.qw = reinterpret_cast<int8_t*>(p + off); off += up(L * w.ldw);
+    w.sw = reinterpret_cast<float*>(p + off); off += up(4LL * L);
+    w.h = reinterpret_cast<float*>(p + off); off += up(4LL * L * B);
+    w.lin = p + off;
+    w.head = off;
+    return w;
+}
+static int64_t ov_int8_need(int L, int G, int B) { return ov_int8_carve(L, G, B, nullptr).head + ontovae_int8_linear_workspace_bytes(B, L, G); }
+// for every batch up to max_batch
+static int64_t ov_int8_need_upto(int L, int G, int max_batch) {
+    return ov_int8_carve(L, G, max_batch, nullptr).head + ov_int8_linear_bytes_upto(max_batch, L, G);
+}
+
+extern "C" int64_t ontovae_int8_workspace_bytes(const ontovae_dims_t* dims, int32_t max_batch) {
+    if (!dims || max_batch < 1 || dims->L < 1 || dims->G < 1) return -1;
+    return ov_int8_need_upto(dims->L, dims->G, max_batch);
 }
 
 // =================================================================================================
@@ -2940,6 +2968,14 @@ static int ov_check_ctx(const ontovae_ctx_t* c, int B, bool need_opt, bool train
                           (long long)ov_carve(d, c->max_batch, ov_train_cap(c), nullptr, nullptr));
         return ONTOVAE_EINVAL;
     }
+    if (c->flags & ONTOVAE_FLAG_INT8_ENCODER) {
+        if (c->flags & ONTOVAE_FLAG_BF16_GEMM) { ontovae_set_error("ctx: ONTOVAE_FLAG_INT8_ENCODER and ONTOVAE_FLAG_BF16_GEMM exclude each other"); return ONTOVAE_EINVAL; }
+        if (!c->bf16_ws || (reinterpret_cast<uintptr_t>(c->bf16_ws) & 255) || c->bf16_ws_bytes < ov_int8_need(d.L, d.G, B)) {
+            ontovae_set_error("ctx: ONTOVAE_FLAG_INT8_ENCODER needs bf16_ws of ontovae_int8_workspace_bytes, 256-B aligned (%lld bytes for this batch)",
+                              (long long)ov_int8_need(d.L, d.G, B));
+            return ONTOVAE_EINVAL;
+        }
+    }
     if (c->flags & ONTOVAE_FLAG_BF16_GEMM) {
         if (d.G % 8) { ontovae_set_error("ctx: the bf16 variant needs a gene count that is a multiple of 8 (G = %d)", d.G); return ONTOVAE_EINVAL; }
         if (!c->bf16_ws || (reinterpret_cast<uintptr_t>(c->bf16_ws) & 255) || c->bf16_ws_bytes < ov_bf16_carve(d, c->max_batch, nullptr, nullptr)) {
@@ -3219,6 +3255,30 @@ static int ov_enc_gemm(OvStep& s, int* S_out) {
     if (nt == 2) return ov_launch_gemm<3, 2, 4, 1, true, true, OV_EPI_STORE>(g, Seff, vec, s.st);
     if (OV_DBG((s.c->flags >> 14) & 1)) return ov_launch_gemm<3, 4, 4, 2, true, true, OV_EPI_STORE>(g, Seff, vec, s.st);
     return ov_launch_gemm<3, 4, 4, 1, true, true, OV_EPI_STORE>(g, Seff, vec, s.st);
+}
+
+// h = W x^T of a batch in 8 bits, feature-major [L, ldb] (columns >= B zero): the weight's rows are quantised in every pass, so that a
+// weight that moved is never met in an old form
+static int ov_int8_first_layer(const float* W, int L, int G, const float* x, int64_t xld, const int32_t* xidx, int B, int ldb, void* ws, int64_t bytes,
+                               float* h, hipStream_t st) {
+    const OvI8Ws w = ov_int8_carve(L, G, B, ws);
+    int rc = ontovae_quantize_rows(W, ONTOVAE_F32, G, nullptr, L, L, G, w.qw, w.ldw, w.sw, st);
+    if (rc) return rc;
+    if ((rc = ontovae_int8_linear(x, ONTOVAE_F32, xld, xidx, xidx ? INT32_MAX : B, w.qw, w.ldw, w.sw, nullptr, B, L, G, w.h, ONTOVAE_F32, L, w.lin,
+                                  bytes - w.head, st)))
+        return rc;
+    hipLaunchKernelGGL(ov_transpose_in_kernel, dim3((L + 31) / 32, (ldb + 31) / 32), dim3(256), 0, st, w.h, L, B, ldb, h);
+    OV_LAUNCH_CHECK();
+    return ONTOVAE_OK;
+}
+
+// the encoder's first product of a pass: inference passes take it in 8 bits where the context says so
+static int ov_enc_product(OvStep& s, int train, int* S_out) {
+    const ontovae_ctx_t* c = s.c;
+    if (train || !(c->flags & ONTOVAE_FLAG_INT8_ENCODER)) return ov_enc_gemm(s, S_out);
+    OvProfScope prof(ONTOVAE_PHASE_ENC_GEMM, s.st);
+    *S_out = 1;
+    return ov_int8_first_layer(c->P + c->lay.W0, c->dims.L, c->dims.G, s.x, s.xld, s.xidx, s.B, s.ldb, c->bf16_ws, c->bf16_ws_bytes, s.ws.slab, s.st);
 }
 
 // mode 5: S = number of rank blocks in `stats`, each 2 L + 1 floats
@@ -3719,7 +3779,7 @@ static int ov_make_step(const ontovae_ctx_t* ctx, const float* x, const int32_t*
 // encoder (eval or fused-train) + heads + reparam: leaves mu/lv in ws.mulv, z in the panel
 static int ov_encode(OvStep& s, const float* eps, int train, uint64_t rng_off, uint32_t eps_stream, int write_kl, int* nkl) {
     int S = 1, rc;
-    if ((rc = ov_enc_gemm(s, &S))) return rc;
+    if ((rc = ov_enc_product(s, train, &S))) return rc;
     if ((rc = ov_bn_fwd(s, S, train ? 1 : 0, s.B, nullptr, rng_off))) return rc;
     if ((rc = ov_heads_fwd(s))) return rc;
     return ov_reparam(s, eps, train, rng_off, eps_stream, write_kl, nkl, true);     // also refreshes the packed term-layer weights
@@ -3902,7 +3962,7 @@ extern "C" int ontovae_encode_pre(const ontovae_ctx_t* ctx, const float* x, cons
     OvStep s;
     ov_make_step(ctx, x, xidx, B, stream, &s);
     int S = 1;
-    if ((rc = ov_enc_gemm(s, &S))) return rc;
+    if ((rc = ov_enc_product(s, 0, &S))) return rc;
     const ontovae_dims_t& d = ctx->dims;
     hipLaunchKernelGGL(ov_slab_sum_kernel, dim3((B + 255) / 256, d.L), dim3(256), 0, s.st, s.ws.slab, S, (int64_t)d.L * s.ldb, B, s.ldb, hpre, ldh);
     OV_LAUNCH_CHECK();

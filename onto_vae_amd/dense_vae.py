@@ -24,10 +24,15 @@ except Exception:  # pragma: no cover
 class DenseEngine:
     """Device state of one dense VAE: flat parameters / moments / gradients, BatchNorm statistics, workspace, ontovae_vae_ctx_t."""
 
-    def __init__(self, in_features, layer_dims_enc, layer_dims_dec, latent_dim, device, drop=0.0, z_drop=0.0):
+    def __init__(self, in_features, layer_dims_enc, layer_dims_dec, latent_dim, device, drop=0.0, z_drop=0.0, groups=0, input_drop=0.0):
         enc, dec = [int(v) for v in layer_dims_enc], [int(v) for v in layer_dims_dec]
         if not 1 <= len(enc) <= _lib.VAE_MAXL or not 1 <= len(dec) <= _lib.VAE_MAXL:
             raise ValueError(f"layer_dims_enc / layer_dims_dec need between 1 and {_lib.VAE_MAXL} entries")
+        self.groups, self.input_drop, self.int8 = int(groups), float(input_drop), False
+        if self.groups < 0 or any(w % self.groups for w in enc + dec if self.groups):
+            raise ValueError(f"groups = {groups} must divide every width of layer_dims_enc / layer_dims_dec")
+        if not 0.0 <= self.input_drop < 1.0:
+            raise ValueError(f"input_drop = {input_drop} outside [0, 1)")
         d = _lib.VaeDims()
         d.G, d.Z, d.n_enc, d.n_dec = int(in_features), int(latent_dim), len(enc), len(dec)
         for i, v in enumerate(enc):
@@ -49,6 +54,7 @@ class DenseEngine:
             for i, w in enumerate(widths):
                 self.bn_view(side, i)[1].fill_(1.0)
         self._ws, self.max_batch, self._ctx = None, 0, None
+        self._ext, self._ext_ws = None, None
         self.seed = int(torch.initial_seed()) & 0xFFFFFFFFFFFFFFFF
         self.rng_offset = 0
 
@@ -98,6 +104,7 @@ class DenseEngine:
                 if v is not None:
                     setattr(self, n, v.to(device))
             self._ws, self.max_batch, self._ctx = None, 0, None
+            self._ext, self._ext_ws = None, None
         return self
 
     def ensure_opt_state(self):
@@ -128,6 +135,7 @@ class DenseEngine:
             self._ws = None
             self._ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=self.device)
             self.max_batch, self._ctx = mb, None
+            self._ext, self._ext_ws = None, None
         if self._ctx is None:
             c = _lib.VaeCtx()
             c.dims = self.dims
@@ -139,6 +147,31 @@ class DenseEngine:
             c.max_batch, c.drop, c.z_drop, c.seed = self.max_batch, self.drop, self.z_drop, self.seed
             self._ctx = c
         return self._ctx
+
+    def set_precision(self, mfma_dtype):
+        """'f32' or 'int8': inference passes take the first layer's product in 8-bit integers (training stays float32)."""
+        if mfma_dtype not in ("f32", "int8"):
+            raise ValueError("mfma_dtype must be 'f32' or 'int8'")
+        if mfma_dtype == "int8" and self.G > 131071:
+            raise ValueError(f"the int8 variant sums exactly up to 131071 genes, got {self.G}")
+        self.int8 = mfma_dtype == "int8"
+        self._ext, self._ext_ws = None, None
+
+    def ext(self):
+        """ontovae_vae_ext_t of the model's blocks (None: the reference's), after ctx()."""
+        if not (self.groups or self.input_drop > 0 or self.int8):
+            return None
+        if self._ext is None:
+            e = _lib.VaeExt(groups=self.groups, input_drop=self.input_drop, flags=_lib.VAE_FLAG_INT8_INPUT if self.int8 else 0)
+            nbytes = _lib.lib().ontovae_vae_ext_workspace_bytes(C.byref(self.dims), C.byref(e), self.max_batch)
+            if nbytes < 0:
+                raise _lib.OntoVAEHipError("vae ext workspace sizing failed")
+            self._ext_ws = torch.empty(nbytes + 256, dtype=torch.uint8, device=self.device)
+            base = self._ext_ws.data_ptr()
+            aligned = (base + 255) // 256 * 256
+            e.workspace, e.workspace_bytes = aligned, self._ext_ws.numel() - (aligned - base)
+            self._ext = e
+        return C.byref(self._ext)
 
     def _x(self, x, xidx):
         if xidx is None:
@@ -167,8 +200,8 @@ class DenseEngine:
         width = dict(recon=self.G, mu=self.Z, log_var=self.Z, z=self.Z)
         out = {k: (torch.empty(B, width[k], dtype=torch.float32, device=self.device) if k in want else None) for k in width}
         ctx = self.ctx(B)
-        _lib.check(_lib.lib().ontovae_vae_forward(C.byref(ctx), _ptr(x), _ptr(xidx), B, _ptr(eps), self.next_offset(), 1 if train else 0,
-                                                  float(kl_coeff), _ptr(out["recon"]), _ptr(out["mu"]), _ptr(out["log_var"]), _ptr(out["z"]),
+        _lib.check(_lib.lib().ontovae_vae_forward_ext(C.byref(ctx), self.ext(), _ptr(x), _ptr(xidx), B, _ptr(eps), self.next_offset(),
+                                                      1 if train else 0, float(kl_coeff), _ptr(out["recon"]), _ptr(out["mu"]), _ptr(out["log_var"]), _ptr(out["z"]),
                                                   _ptr(loss_out), self.stream()), "vae_forward")
         return out
 
@@ -181,8 +214,8 @@ class DenseEngine:
         else:
             self.ensure_grad_buffer()
         ctx = self.ctx(B)
-        _lib.check(_lib.lib().ontovae_vae_train_step(C.byref(ctx), _ptr(x), _ptr(xidx), B, _ptr(eps), self.next_offset(), float(kl_coeff),
-                                                     C.byref(adam) if adam is not None else None, 1 if apply_update else 0, _ptr(loss_out),
+        _lib.check(_lib.lib().ontovae_vae_train_step_ext(C.byref(ctx), self.ext(), _ptr(x), _ptr(xidx), B, _ptr(eps), self.next_offset(), float(kl_coeff),
+                                                         C.byref(adam) if adam is not None else None, 1 if apply_update else 0, _ptr(loss_out),
                                                      self.stream()), "vae_train_step")
 
     def eval_step(self, x, xidx, eps, kl_coeff, loss_out):
@@ -234,8 +267,8 @@ class DenseEngine:
         _lib.check(_lib.lib().ontovae_vae_adamw_apply(C.byref(ctx), C.byref(adam), self.stream()), "vae_adamw_apply")
 
 
-def _block(cin, cout, drop):
-    return nn.Sequential(nn.Linear(cin, cout), nn.BatchNorm1d(cout), nn.Dropout(p=drop), nn.ReLU())
+def _block(cin, cout, drop, groups=0):
+    return nn.Sequential(nn.Linear(cin, cout), nn.GroupNorm(groups, cout) if groups else nn.BatchNorm1d(cout), nn.Dropout(p=drop), nn.ReLU())
 
 
 def _adopt(engine, seq, views, bn=None, nbt=None):
@@ -250,8 +283,9 @@ def _rebind(seq, views, bn=None, nbt=None):
     _bind(seq[0], "weight", views[0]); _bind(seq[0], "bias", views[1])
     if len(views) == 4:
         _bind(seq[1], "weight", views[2]); _bind(seq[1], "bias", views[3])
-        seq[1]._buffers["running_mean"], seq[1]._buffers["running_var"] = bn
-        seq[1]._buffers["num_batches_tracked"] = nbt
+        if isinstance(seq[1], nn.BatchNorm1d):
+            seq[1]._buffers["running_mean"], seq[1]._buffers["running_var"] = bn
+            seq[1]._buffers["num_batches_tracked"] = nbt
 
 
 class DenseEncoder(nn.Module):
@@ -263,7 +297,7 @@ class DenseEncoder(nn.Module):
         e = engine
         self.in_features, self.layer_dims, self.latent_dim, self.drop, self.z_drop = e.G, list(e.enc), e.Z, e.drop, e.z_drop
         self.layer_nums = [self.layer_dims[i:i + 2] for i in range(len(self.layer_dims) - 1)]
-        self.encoder = nn.ModuleList([_block(*reversed(e.block_shape("enc", i)), e.drop) for i in range(len(e.enc))])
+        self.encoder = nn.ModuleList([_block(*reversed(e.block_shape("enc", i)), e.drop, e.groups) for i in range(len(e.enc))])
         self.mu = nn.Sequential(nn.Linear(e.enc[-1], e.Z), nn.Dropout(p=e.z_drop))
         self.logvar = nn.Sequential(nn.Linear(e.enc[-1], e.Z), nn.Dropout(p=e.z_drop))
         for i, seq in enumerate(self.encoder):
@@ -296,7 +330,7 @@ class Decoder(nn.Module):
         e = engine
         self.in_features, self.layer_dims, self.latent_dim, self.drop = e.G, list(e.dec), e.Z, e.drop
         self.layer_nums = [self.layer_dims[i:i + 2] for i in range(len(self.layer_dims) - 1)]
-        self.decoder = nn.ModuleList([_block(*reversed(e.block_shape("dec", i)), e.drop) for i in range(len(e.dec))] +
+        self.decoder = nn.ModuleList([_block(*reversed(e.block_shape("dec", i)), e.drop, e.groups) for i in range(len(e.dec))] +
                                      [nn.Sequential(nn.Linear(e.dec[-1], e.G))])
         for i in range(len(e.dec)):
             _adopt(e, self.decoder[i], e.block_views("dec", i))
@@ -319,10 +353,17 @@ class VAE(nn.Module):
     """A standard VAE without ontology (reference vae_model.py:913-955).
 
     Parameters as in the reference: data (2D numpy array, samples in rows), layer_dims_enc, layer_dims_dec, latent_dim,
-    drop, z_drop."""
+    drop, z_drop.  Not in the reference: norm='group' normalises every block over `groups` groups of its units, sample by sample
+    (onto_vae_amd.ops.group_norm_act), in place of BatchNorm1d; input_drop feeds the encoder the batch after dropout in
+    training (onto_vae_amd.ops.dropout; the loss still compares with the batch itself)."""
 
-    def __init__(self, data, layer_dims_enc=[1000], layer_dims_dec=[1000], latent_dim=128, drop=0.2, z_drop=0.5):
+    def __init__(self, data, layer_dims_enc=[1000], layer_dims_dec=[1000], latent_dim=128, drop=0.2, z_drop=0.5, norm='batch', groups=8,
+                 input_drop=0.0):
         super().__init__()
+        if norm not in ('batch', 'group'):
+            raise ValueError("norm must be 'batch' or 'group'")
+        if norm == 'group' and int(groups) < 1:
+            raise ValueError(f"groups = {groups} must be positive")
         self.X = data
         self.in_features = self.X.shape[1]
         self.layer_dims_enc = layer_dims_enc
@@ -330,8 +371,10 @@ class VAE(nn.Module):
         self.latent_dim = latent_dim
         self.drop = drop
         self.z_drop = z_drop
+        self.norm, self.groups, self.input_drop = norm, groups, input_drop
         self.device = 'cuda' if torch.cuda.is_available() else 'cpu'
-        object.__setattr__(self, "_engine", DenseEngine(self.in_features, layer_dims_enc, layer_dims_dec, latent_dim, self.device, drop, z_drop))
+        object.__setattr__(self, "_engine", DenseEngine(self.in_features, layer_dims_enc, layer_dims_dec, latent_dim, self.device, drop, z_drop,
+                                                        int(groups) if norm == 'group' else 0, input_drop))
         self.encoder = DenseEncoder(self._engine)
         self.decoder = Decoder(self._engine)
         self.eps_source = None        # test hook: callable(B) -> eps [B, latent_dim]; None = Philox stream inside the kernels
@@ -354,6 +397,11 @@ class VAE(nn.Module):
 
     def _eps(self, B):
         return None if self.eps_source is None else self.eps_source(B)
+
+    def set_precision(self, mfma_dtype):
+        """'f32' (default) or 'int8' (not in the reference): inference passes take the encoder's first product in 8-bit integers."""
+        self._engine.set_precision(mfma_dtype)
+        return self
 
     # ------------------------------------------------------------------ reference methods
     def reparameterize(self, mu, log_var):

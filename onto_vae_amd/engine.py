@@ -223,6 +223,10 @@ class Engine:
             self._bf16_ws = torch.zeros(nb16 + 256, dtype=torch.uint8, device=self.device)
             self.ensure_grad_buffer()          # the bf16 dW0 product is staged in the gradient buffer
             self._ctx = None
+        if (self.flags & _lib.FLAG_INT8_ENCODER) and getattr(self, "_bf16_ws", None) is None:
+            nb8 = L.ontovae_int8_workspace_bytes(C.byref(self.plan.dims), self.max_batch)
+            self._bf16_ws = torch.empty(nb8 + 256, dtype=torch.uint8, device=self.device)
+            self._ctx = None
         if self._ctx is None:
             c = _lib.Ctx()
             c.dims = self.plan.dims
@@ -258,7 +262,7 @@ class Engine:
             c.max_train_batch = self.max_train_batch
             c.drop, c.z_drop, c.seed = self.drop, self.z_drop, self.seed
             c.flags = self.flags
-            if self.flags & _lib.FLAG_BF16_GEMM:
+            if self.flags & (_lib.FLAG_BF16_GEMM | _lib.FLAG_INT8_ENCODER):
                 b16 = self._bf16_ws.data_ptr()
                 a16 = (b16 + 255) // 256 * 256
                 c.bf16_ws = C.c_void_p(a16)
@@ -271,15 +275,20 @@ class Engine:
 
     def set_precision(self, mfma_dtype):
         """'f32' (default: everything in float32, the reference's precision) or 'bf16' (the two
-        large dense products x W0^T and dW0 = dh x on bf16 MFMA with fp32 accumulation; weights and AdamW stay fp32)."""
-        if mfma_dtype not in ("f32", "bf16"):
-            raise ValueError("mfma_dtype must be 'f32' or 'bf16'")
+        large dense products x W0^T and dW0 = dh x on bf16 MFMA with fp32 accumulation; weights and AdamW stay fp32) or 'int8'
+        (inference passes take x W0^T in 8-bit integers, one scale per row of x and of W0; training passes stay float32)."""
+        if mfma_dtype not in ("f32", "bf16", "int8"):
+            raise ValueError("mfma_dtype must be 'f32', 'bf16' or 'int8'")
+        if mfma_dtype == "int8" and self.plan.G > 131071:
+            raise ValueError(f"the int8 variant sums exactly up to 131071 genes, got {self.plan.G}")
         if mfma_dtype == "bf16":
             if self.plan.G % 8:
                 raise ValueError(f"the bf16 variant needs a gene count that is a multiple of 8, got {self.plan.G}")
-            self.flags |= _lib.FLAG_BF16_GEMM
-        else:
-            self.flags &= ~_lib.FLAG_BF16_GEMM
+        was = self.flags
+        self.flags &= ~(_lib.FLAG_BF16_GEMM | _lib.FLAG_INT8_ENCODER)
+        self.flags |= {"f32": 0, "bf16": _lib.FLAG_BF16_GEMM, "int8": _lib.FLAG_INT8_ENCODER}[mfma_dtype]
+        if self.flags != was:
+            self._bf16_ws = None       # the variants size it differently
         self._ctx = None
 
     def stream(self):

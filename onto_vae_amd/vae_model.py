@@ -137,9 +137,11 @@ class OntoVAE(nn.Module):
 
     # ------------------------------------------------------------------ plumbing
     def set_precision(self, mfma_dtype):
-        """Not in the reference.  'f32' (default) or 'bf16': BASELINE.json configs[4], the two large dense products of a pass
-        (x W0^T and its weight gradient) on bf16 MFMA with fp32 accumulation; parameters, optimizer and everything else stay
-        float32.  Stated tolerance against the float32 path: loss 2e-2 relative per step, activities cosine >= 0.999."""
+        """Not in the reference.  'f32' (default); 'bf16': the two large dense products of a pass (x W0^T and its weight
+        gradient) on bf16 MFMA with fp32 accumulation, parameters, optimizer and everything else float32 (stated tolerance
+        against the float32 path: loss 2e-2 relative per step, activities cosine >= 0.999); 'int8': inference passes take
+        x W0^T in 8-bit integers with one scale per sample and per hidden unit (onto_vae_amd.ops.int8_linear; activities
+        cosine >= 0.999), training passes stay float32."""
         self._engine.set_precision(mfma_dtype)
         return self
 

@@ -150,3 +150,31 @@ def test_python_entry_points_refuse_host_tensors():
                lambda: ops.int8_matmul(x.to(torch.int8), x[:, 0], x.to(torch.int8), x[:, 0])):
         with pytest.raises(_lib.OntoVAEHipError, match="no CPU path"):
             fn()
+
+
+def test_vae_ext_sizing_and_refusals(L):
+    from onto_vae_amd import _lib
+    d = _lib.VaeDims()
+    d.G, d.Z, d.n_enc, d.n_dec = 500, 8, 1, 1
+    d.enc[0], d.dec[0] = 96, 64
+    size = lambda **kw: L.ontovae_vae_ext_workspace_bytes(C.byref(d), C.byref(_lib.VaeExt(**kw)), 128)
+    assert size() == 0
+    assert size(groups=8) > 0 and size(input_drop=0.5) >= 4 * 128 * 500 and size(flags=_lib.VAE_FLAG_INT8_INPUT) > 96 * 500
+    for bad in (dict(groups=-1), dict(groups=7), dict(input_drop=1.0), dict(input_drop=-0.5), dict(input_drop=float("nan")), dict(flags=2), dict(reserved=1)):
+        assert size(**bad) == -1
+    # enough for every smaller batch
+    top = size(groups=8)
+    for b in (1, 2, 64, 127):
+        assert L.ontovae_vae_ext_workspace_bytes(C.byref(d), C.byref(_lib.VaeExt(groups=8)), b) <= top
+
+
+def test_int8_workspace_of_a_model_covers_every_batch(L):
+    from onto_vae_amd import _lib
+    dims = _lib.Dims()
+    for L_, G, top in ((360, 20000, 700), (60, 1000, 5000), (228, 5892, 300)):
+        dims.L, dims.G = L_, G
+        have = L.ontovae_int8_workspace_bytes(C.byref(dims), top)
+        for b in list(range(1, top, 7)) + [top]:
+            fixed = have - L.ontovae_int8_linear_workspace_bytes(b, L_, G)
+            assert fixed >= L_ * G + 4 * L_ + 4 * L_ * b
+    assert L.ontovae_int8_workspace_bytes(C.byref(dims), 0) == -1
