@@ -593,7 +593,7 @@ enum { ONTOVAE_F32 = 0, ONTOVAE_BF16 = 1, ONTOVAE_F16 = 2 };
 enum { ONTOVAE_ACT_NONE = 0, ONTOVAE_ACT_RELU = 1, ONTOVAE_ACT_SILU = 2, ONTOVAE_ACT_GELU = 3 };
 
 /* Row m of x (row rows[m] of the n_src rows when rows != NULL), K elements at stride ldx, in 8 bits:
- *   scale[m] = max_k |x| / 127 (float32),  q[m * ldq + k] = rint(x / scale[m]) (the true quotient, ties to even) in [-127, 127].
+ *   scale[m] = max_k |x| * (1 / 127) (one float32 product),  q[m * ldq + k] = rint(x / scale[m]) (the true quotient, ties to even) in [-127, 127].
  * Columns [K, ldq) of q are set to 0 (pad ldq to a multiple of 64: ontovae_int8_matmul then takes its aligned path).
  * A zero row: scale 0.  A row with an infinity or a NaN, or a row index outside [0, n_src): scale NaN, q 0. */
 int ontovae_quantize_rows(const void* x, int32_t dtype, int64_t ldx, const int32_t* rows, int32_t n_src, int32_t M, int32_t K,

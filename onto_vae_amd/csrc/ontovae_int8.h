@@ -1,6 +1,6 @@
 // Products in 8-bit integers with one scale per row of each operand.
 //
-//   s_m = max_k |x_mk| / 127,  q_mk = rint(x_mk / s_m)          (ov_q8_rows_kernel)
+//   s_m = max_k |x_mk| * (1 / 127),  q_mk = rint(x_mk / s_m)      (ov_q8_rows_kernel)
 //   y_mn = s_m t_n sum_k q_mk w_nk + b_n                        (ov_q8_gemm_kernel), the sum exact in 32-bit integers
 //
 // Integer sums are exact in any order, so the K axis may be cut into slabs (ov_q8_combine_kernel) without a rounding.
@@ -14,9 +14,10 @@
 typedef int ov_i32x4 __attribute__((ext_vector_type(4)));
 typedef int ov_i32x16 __attribute__((ext_vector_type(16)));
 
-// A row's scale from the bits of its largest magnitude: NaN if the row holds an infinity or a NaN.
+// A row's scale from the bits of its largest magnitude: NaN if the row holds an infinity or a NaN.  A product with the float32
+// nearest to 1 / 127, as tensor libraries divide by a constant: a weight that such a program quantised has the same scale, bit for bit.
 __device__ __forceinline__ float ov_q8_scale(uint32_t amax_bits) {
-    return amax_bits >= 0x7f800000u ? __builtin_nanf("") : __builtin_bit_cast(float, amax_bits) / 127.0f;
+    return amax_bits >= 0x7f800000u ? __builtin_nanf("") : __builtin_bit_cast(float, amax_bits) * (1.0f / 127.0f);
 }
 
 // Rounding of the TRUE quotient x / s to the nearest integer, ties to even: x * (1 / s) is off by two roundings, so its
@@ -521,6 +522,7 @@ static void ov_q8_rows_launch(const void* x, int64_t ldx, const int32_t* rows, i
     else if (p <= 256) OV_Q8_ROWS(64, 4);
     else if (p <= 1024) OV_Q8_ROWS(256, 4);
     else if (p <= 2048) OV_Q8_ROWS(512, 4);
+    else if (p <= 5120 && M <= 512) OV_Q8_ROWS(1024, 5);      // one round of workgroups: fewer pieces one behind the other
     else if (p <= 5120) OV_Q8_ROWS(512, 10);
     else OV_Q8_ROWS(1024, 16);
 #undef OV_Q8_ROWS

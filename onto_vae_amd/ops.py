@@ -99,7 +99,7 @@ def _u64(v, what):
 
 # ---------------------------------------------------------------- 8-bit linear layers
 def quantize_rows(x, rows=None):
-    """(q, scale): the rows of a [..., K] tensor (of the rows x[rows] of a matrix) in 8 bits, scale = max|row| / 127 in float32 and
+    """(q, scale): the rows of a [..., K] tensor (of the rows x[rows] of a matrix) in 8 bits, scale = max|row| * (1 / 127) in float32 and
     q = x / scale rounded to the nearest integer, ties to even.  q has shape [..., K] and a row stride padded with zeros to a
     multiple of 64, the layout int8_matmul reads fastest.  A row that holds an infinity or a NaN (or a row index outside x) gets
     the scale NaN."""

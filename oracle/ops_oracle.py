@@ -19,7 +19,7 @@ def quantize_rows(x):
     amax = np.abs(x).max(1) if K else np.zeros(M)
     bad = ~np.isfinite(x).all(1)
     with np.errstate(all="ignore"):
-        s = (amax.astype(np.float32) / np.float32(127)).astype(np.float32)
+        s = (amax.astype(np.float32) * (np.float32(1) / np.float32(127))).astype(np.float32)
         q = np.rint(x / s.astype(np.float64)[:, None])
     q = np.where(np.isfinite(q) & ~bad[:, None] & (s > 0)[:, None], q, 0)
     s[bad] = np.nan
