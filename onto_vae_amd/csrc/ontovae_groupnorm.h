@@ -385,10 +385,10 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
     }
 }
 
-// column sums of part [2][R][C] in a fixed order: 16 channels x 16 rows at a time per workgroup
-__global__ __launch_bounds__(256) void ov_gn_param_kernel(const float* __restrict__ part, int64_t R, int C, float* __restrict__ dw,
-                                                          float* __restrict__ db) {
-    __shared__ float red[16][17];
+// column sums of part [2][R][C] in a fixed order: 16 channels x 64 rows at a time per workgroup, 8 loads in flight per thread
+__global__ __launch_bounds__(1024) void ov_gn_param_kernel(const float* __restrict__ part, int64_t R, int C, float* __restrict__ dw,
+                                                           float* __restrict__ db) {
+    __shared__ float red[64][17];
     float* out = blockIdx.y ? db : dw;
     if (!out) return;
     const float* src = part + (blockIdx.y ? R * C : 0);
@@ -396,21 +396,28 @@ __global__ __launch_bounds__(256) void ov_gn_param_kernel(const float* __restric
     float s[4] = {0.f, 0.f, 0.f, 0.f};
     if (c < C) {
         int64_t r = ty;
-        for (; r + 112 < R; r += 128) {
+        for (; r + 7 * 64 < R; r += 8 * 64) {
             float t[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) t[u] = src[(r + 16 * u) * C + c];
+            for (int u = 0; u < 8; ++u) t[u] = src[(r + 64 * u) * C + c];
 #pragma unroll
             for (int u = 0; u < 8; ++u) s[u & 3] += t[u];
         }
-        for (; r < R; r += 16) s[0] += src[r * C + c];
+        for (; r < R; r += 64) s[0] += src[r * C + c];
     }
     red[ty][tx] = (s[0] + s[1]) + (s[2] + s[3]);
+    __syncthreads();
+    if (ty < 8) {
+        float t = 0.f;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) t += red[ty * 8 + k][tx];
+        red[ty * 8][tx] = t;                              // read by this thread only, until the barrier
+    }
     __syncthreads();
     if (ty == 0 && c < C) {
         float t = 0.f;
 #pragma unroll
-        for (int k = 0; k < 16; ++k) t += red[k][tx];
+        for (int k = 0; k < 8; ++k) t += red[k * 8][tx];
         out[c] = t;
     }
 }
@@ -451,12 +458,18 @@ __device__ __forceinline__ OvGnPlace ov_gn_place(const OvGn& p, const OvGnTile& 
     return q;
 }
 
+// lanes of a wave that share one of ng groups of n terms: a power of two, all groups in one round of 256 threads if they fit
+__device__ __forceinline__ int ov_gn_lanes(int ng, int n) {
+    int lg = 64;
+    while (lg > 1 && (lg > n || lg * ng > 256)) lg >>= 1;
+    return lg;
+}
+
 // count-weighted combination of the chunks' (first, second) over a group; lanes of the workgroup share the groups out.
 // FWD: (mean, M2) by Chan's formula about the overall mean -> (mu, r).  Else: plain sums / count.
 template <bool FWD>
 __device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, const OvGnPlace& q, float2* st) {
-    int lg = 64;                                         // lanes per group
-    while (lg > 1 && (lg > t.chunks || lg * q.ng > 256)) lg >>= 1;
+    const int lg = ov_gn_lanes(q.ng, t.chunks);
     for (int g = threadIdx.x / lg; g < q.ng; g += 256 / lg) {
         const int l = threadIdx.x % lg;
         const float2* src = reinterpret_cast<const float2*>(t.part) + ((int64_t)q.n * t.chunks * p.groups + q.g0 + g);
@@ -566,15 +579,19 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
             st[c] = make_float2(a, b);
         }
         __syncthreads();
-        for (int g = tid; g < q.ng; g += 256) {
+        const int lg = ov_gn_lanes(q.ng, p.cg), l = tid % lg;
+        for (int g = tid / lg; g < q.ng; g += 256 / lg) {
             float a = 0.f, b = 0.f;
-            for (int k = 0; k < p.cg; ++k) a += st[g * p.cg + k].x;
+            for (int k = l; k < p.cg; k += lg) a += st[g * p.cg + k].x;
+            for (int o = lg / 2; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
             a /= (float)p.cg;
-            for (int k = 0; k < p.cg; ++k) {
+            for (int k = l; k < p.cg; k += lg) {
                 const float2 v = st[g * p.cg + k];
                 const float d = v.x - a;
                 b += v.y + d * d * (float)rows;
             }
+            for (int o = lg / 2; o > 0; o >>= 1) b += __shfl_xor(b, o, 64);
+            if (l != 0) continue;
             if (MODE == 0) reinterpret_cast<float2*>(t.part)[((int64_t)q.n * t.chunks + q.chunk) * p.groups + q.g0 + g] = make_float2(a, b);
             else cs[g] = make_float2(a, 1.f / sqrtf(b / (float)((int64_t)rows * p.cg) + p.eps));
         }
@@ -705,13 +722,16 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
             st[c] = make_float2(a * wc, e * wc);
         }
         __syncthreads();
-        for (int g = tid; g < q.ng; g += 256) {
+        const int lg = ov_gn_lanes(q.ng, p.cg), l = tid % lg;
+        for (int g = tid / lg; g < q.ng; g += 256 / lg) {
             float a = 0.f, e = 0.f;
-            for (int k = 0; k < p.cg; ++k) {
+            for (int k = l; k < p.cg; k += lg) {
                 const float2 v = st[g * p.cg + k];
                 a += v.x;
                 e += v.y;
             }
+            for (int o = lg / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); e += __shfl_xor(e, o, 64); }
+            if (l != 0) continue;
             if (MODE == 0) reinterpret_cast<float2*>(t.part)[ro * p.groups + q.g0 + g] = make_float2(a, e);
             else {
                 const float total = (float)((int64_t)p.S * p.cg);
@@ -889,7 +909,7 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         const int per = groups * q.lpg;
         q.wgs = q.lpg < 256 && per <= 128 && 256 % per == 0 ? 256 / per : 1;
         const int64_t want = std::max<int64_t>(262144 / (int64_t)per, 1);
-        const int64_t most = (int64_t)std::max((N + 7) / 8, std::min(N, 16)) * q.wgs;
+        const int64_t most = std::max((int64_t)(N + 7) / 8, std::min<int64_t>(N, 65536 / std::min(per * q.wgs, 65536))) * q.wgs;
         q.RS = (int)std::min<int64_t>(want, backward ? std::min<int64_t>(most, N) : N);
         q.chan_rows = q.wgs > 1 ? (q.RS + q.wgs - 1) / q.wgs : q.RS;
         q.chan_floats = backward ? 2 * q.chan_rows * C : 0;
@@ -911,8 +931,12 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         q.form = OV_GN_TILE1;
         if (bytes > 65536) {
             q.form = OV_GN_TILE;
-            const int most = (S + t.ty * 16 - 1) / (t.ty * 16);
-            t.chunks = (int)std::max<int64_t>(1, std::min<int64_t>(most, (1024 + wg - 1) / wg));
+            // up to 1024 workgroups of 16 rows a thread or more; where the samples are few, 256 of 4 rows or more, at most 128 a
+            // sample (4 x 1024 x 320 float32 with gelu: 31 -> 19 us forward, 54 -> 27 backward; 60 x 3000 x 40 lost a fifth
+            // with 900 workgroups of 4 rows, 1 x 4096 x 512 a fifth with 256 a sample)
+            const int64_t few = std::min<int64_t>((S + t.ty * 4 - 1) / (t.ty * 4), std::min<int64_t>((256 + wg - 1) / wg, 128));
+            const int64_t many = std::min<int64_t>((S + t.ty * 16 - 1) / (t.ty * 16), (1024 + wg - 1) / wg);
+            t.chunks = (int)std::max<int64_t>(1, std::max(few, many));
             t.rows = (S + t.chunks - 1) / t.chunks;
             t.chunks = (S + t.rows - 1) / t.rows;
             q.part_floats = 2LL * N * t.chunks * groups;
@@ -1033,7 +1057,7 @@ static void ov_gn_bwd_go(const void* dy, const void* x, const OvGn& p, OvGnPlan 
             hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 1, LIGHT>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
         }
     }
-    if (chan) hipLaunchKernelGGL(ov_gn_param_kernel, dim3((p.C + 15) / 16, 2), dim3(256), 0, st, chan, q.chan_rows, p.C, dw, db);
+    if (chan) hipLaunchKernelGGL(ov_gn_param_kernel, dim3((p.C + 15) / 16, 2), dim3(1024), 0, st, chan, q.chan_rows, p.C, dw, db);
 }
 
 template <typename T>

@@ -516,7 +516,7 @@ static void ov_q8_rows_launch(const void* x, int64_t ldx, const int32_t* rows, i
     const int p = (K + VE - 1) / VE;
     const T* xt = static_cast<const T*>(x);
 #define OV_Q8_ROWS(TH, NV) \
-    hipLaunchKernelGGL((ov_q8_rows_kernel<T, TH, NV>), dim3(TH < 256 ? (M + 3) / 4 : M), dim3(TH < 256 ? 256 : TH), 0, st, xt, ldx, rows, n_src, M, K, q, \
+    hipLaunchKernelGGL((ov_q8_rows_kernel<T, TH, NV>), dim3((unsigned)(TH < 256 ? ((int64_t)M + 3) / 4 : (int64_t)M)), dim3(TH < 256 ? 256 : TH), 0, st, xt, ldx, rows, n_src, M, K, q, \
                        ldq, kst, kpad, scale)
     if (p <= 64) OV_Q8_ROWS(64, 1);
     else if (p <= 256) OV_Q8_ROWS(64, 4);
@@ -545,6 +545,7 @@ extern "C" int ontovae_quantize_rows(const void* x, int32_t dtype, int64_t ldx, 
         ontovae_set_error("quantize_rows: M = %d, K = %d, n_src = %d, ldx = %lld, ldq = %lld", M, K, n_src, (long long)ldx, (long long)ldq);
         return ONTOVAE_EINVAL;
     }
+    if (K > (1 << 30)) { ontovae_set_error("quantize_rows: K = %d, rows of up to 2^30 elements", K); return ONTOVAE_EINVAL; }
     if (dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) { ontovae_set_error("quantize_rows: unknown element type %d", dtype); return ONTOVAE_EINVAL; }
     if (M == 0) return ONTOVAE_OK;
     if (!scale || (K > 0 && (!x || !q))) { ontovae_set_error("quantize_rows: NULL argument"); return ONTOVAE_EINVAL; }
@@ -647,7 +648,7 @@ static int ov_q8_matmul(const int8_t* a, int64_t lda, int64_t ast, const float* 
     return ONTOVAE_OK;
 }
 
-static bool ov_q8_too_many(int M, int N) { return ((int64_t)M + 31) / 32 * (((int64_t)N + 63) / 64) > INT32_MAX; }
+static bool ov_q8_too_many(int M, int N) { return std::max(M, N) > INT32_MAX - 1024 || ((int64_t)M + 31) / 32 * (((int64_t)N + 63) / 64) > INT32_MAX; }
 
 extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb,
                                    const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t dtype, int64_t ldy, void* workspace,

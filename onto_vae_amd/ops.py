@@ -85,7 +85,7 @@ def _rows(rows, x, what):
 def _vector(t, n, device, what, dtypes=(torch.float32,)):
     if t is None:
         return None
-    if t.shape != (n,) or t.dtype not in dtypes or t.device != device:
+    if t.dim() != 1 or t.shape[0] != n or t.dtype not in dtypes or t.device != device:
         raise ValueError(f"{what} must be {' / '.join(str(d).split('.')[-1] for d in dtypes)} [{n}] on {device}")
     return t.contiguous()
 
@@ -179,24 +179,27 @@ def int8_linear(x, weight, weight_scale, bias=None, rows=None, dtype=None):
 def _gn_args(x, groups, weight, bias, act, drop, seed, offset, what):
     _need_gpu(x, what)
     dt = _dtype(x, what)
-    if x.dim() < 2:
+    shape = x.shape
+    if len(shape) < 2:
         raise ValueError(f"{what}: x must be [N, ..., C], channels last")
-    N, Cn = _size(x.shape[0], what), _size(x.shape[-1], what)
-    S = _size(math.prod(x.shape[1:-1]), what)
-    groups = int(groups)
+    N, S, Cn = shape[0], math.prod(shape[1:-1]) if len(shape) > 2 else 1, shape[-1]
+    if max(N, S, Cn) > I32_MAX:
+        raise ValueError(f"{what}: a dimension of {tuple(shape)} exceeds {I32_MAX}")
+    groups, drop = int(groups), float(drop)
     if groups < 1 or Cn % groups or Cn < groups:
         raise ValueError(f"{what}: {groups} groups do not divide {Cn} channels")
     if act not in ACTIVATIONS:
         raise ValueError(f"{what}: act must be one of {sorted(ACTIVATIONS)}, got {act!r}")
-    if not 0.0 <= float(drop) <= 1.0:
+    if not 0.0 <= drop <= 1.0:
         raise ValueError(f"{what}: drop = {drop} outside [0, 1]")
-    both = tuple(dict.fromkeys((torch.float32, x.dtype)))
-    weight, bias = _vector(weight, Cn, x.device, f"{what}: weight", both), _vector(bias, Cn, x.device, f"{what}: bias", both)
-    if weight is not None and bias is not None and weight.dtype != bias.dtype:
-        raise ValueError(f"{what}: weight and bias must share one type")
-    par = weight if weight is not None else bias
-    wdt = torch.float32 if par is None else par.dtype
-    return dt, N, S, Cn, groups, weight, bias, wdt, ACTIVATIONS[act], float(drop), _u64(seed, f"{what}: seed"), _u64(offset, f"{what}: offset")
+    wdt = 0
+    if weight is not None or bias is not None:
+        both = (torch.float32, x.dtype)
+        weight, bias = _vector(weight, Cn, x.device, f"{what}: weight", both), _vector(bias, Cn, x.device, f"{what}: bias", both)
+        if weight is not None and bias is not None and weight.dtype != bias.dtype:
+            raise ValueError(f"{what}: weight and bias must share one type")
+        wdt = DTYPES[(bias if weight is None else weight).dtype]
+    return dt, N, S, Cn, groups, weight, bias, wdt, ACTIVATIONS[act], drop, _u64(seed, f"{what}: seed"), _u64(offset, f"{what}: offset")
 
 
 def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", drop=0.0, seed=0, offset=0):
@@ -211,12 +214,11 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", drop
     L = _lib.lib()
     with _on(x.device):
         y = torch.empty_like(x)
-        mean = torch.empty(N, groups, dtype=torch.float32, device=x.device)
-        rstd = torch.empty_like(mean)
-        if y.numel() == 0:          # no rows to take statistics of
+        mean, rstd = torch.empty(2, N, groups, dtype=torch.float32, device=x.device).unbind()
+        if N == 0 or S == 0:          # no rows to take statistics of
             return y, mean.zero_(), rstd.zero_()
         keep, ws, nbytes = _workspace(L.ontovae_group_norm_act_workspace_bytes(dt, N, S, Cn, groups, 0), x.device)
-        _lib.check(L.ontovae_group_norm_act(_p(x), dt, N, S, Cn, groups, _p(weight), _p(bias), DTYPES[wdt], float(eps), a, drop, seed,
+        _lib.check(L.ontovae_group_norm_act(_p(x), dt, N, S, Cn, groups, _p(weight), _p(bias), wdt, float(eps), a, drop, seed,
                                             offset, _p(y), _p(mean), _p(rstd), ws, nbytes, _stream(x.device)), "group_norm_act")
     return y, mean, rstd
 
@@ -235,12 +237,12 @@ def group_norm_act_backward(dy, x, mean, rstd, groups, weight=None, bias=None, a
     L = _lib.lib()
     with _on(x.device):
         dx = torch.empty_like(x)
-        dw = torch.empty(Cn, dtype=torch.float32, device=x.device) if weight is not None else None
-        db = torch.empty(Cn, dtype=torch.float32, device=x.device) if bias is not None else None
-        if x.numel() == 0:
+        dw, db = torch.empty(2, Cn, dtype=torch.float32, device=x.device).unbind()
+        dw, db = dw if weight is not None else None, db if bias is not None else None
+        if N == 0 or S == 0:
             return dx, dw.zero_() if dw is not None else None, db.zero_() if db is not None else None
         keep, ws, nbytes = _workspace(L.ontovae_group_norm_act_workspace_bytes(dt, N, S, Cn, groups, 1), x.device)
-        _lib.check(L.ontovae_group_norm_act_backward(_p(dy), _p(x), dt, N, S, Cn, groups, _p(weight), _p(bias), DTYPES[wdt], _p(mean),
+        _lib.check(L.ontovae_group_norm_act_backward(_p(dy), _p(x), dt, N, S, Cn, groups, _p(weight), _p(bias), wdt, _p(mean),
                                                      _p(rstd), a, drop, seed, offset, _p(dx), _p(dw), _p(db), ws, nbytes,
                                                      _stream(x.device)), "group_norm_act_backward")
     return dx, dw, db

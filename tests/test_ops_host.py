@@ -52,7 +52,7 @@ NULL = C.c_void_p(0)
 
 
 @pytest.mark.parametrize("change", [dict(M=-1), dict(K=-1), dict(ldx=3), dict(ldq=3), dict(dtype=3), dict(dtype=-1), dict(n_src=1), dict(x=NULL),
-                                    dict(q=NULL), dict(scale=NULL), dict(n_src=-1)])
+                                    dict(q=NULL), dict(scale=NULL), dict(n_src=-1), dict(K=(1 << 30) + 1, ldx=1 << 31, ldq=1 << 31)])
 def test_quantize_rows_refusals(L, change):
     a = dict(x=P, dtype=0, ldx=4, rows=NULL, n_src=2, M=2, K=4, q=P, ldq=4, scale=P, stream=NULL)
     a.update(change)
@@ -61,7 +61,7 @@ def test_quantize_rows_refusals(L, change):
 
 
 @pytest.mark.parametrize("change", [dict(M=-1), dict(N=-1), dict(K=-1), dict(lda=3), dict(ldb=3), dict(ldy=2), dict(K=131072, lda=1 << 20, ldb=1 << 20),
-                                    dict(dtype=7), dict(a=NULL), dict(b=NULL), dict(sa=NULL), dict(sb=NULL), dict(y=NULL)])
+                                    dict(dtype=7), dict(M=2 ** 31 - 1), dict(M=2 ** 30, N=2 ** 20, ldy=2 ** 20), dict(a=NULL), dict(b=NULL), dict(sa=NULL), dict(sb=NULL), dict(y=NULL)])
 def test_int8_matmul_refusals(L, change):
     a = dict(a=P, lda=4, sa=P, b=P, ldb=4, sb=P, bias=NULL, M=2, N=3, K=4, y=P, dtype=0, ldy=3, ws=NULL, nbytes=0, stream=NULL)
     a.update(change)
