@@ -476,7 +476,7 @@ __device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, c
         float a = 0.f, b = 0.f;
         for (int k = l; k < t.chunks; k += lg) {
             const float2 v = src[(int64_t)k * p.groups];
-            a += FWD ? v.x * (float)(ov_gn_tile_rows(p, t, k) * p.cg) : v.x;
+            a += FWD ? v.x * ((float)ov_gn_tile_rows(p, t, k) * (float)p.cg) : v.x;
             b += v.y;
         }
         for (int o = lg / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
@@ -486,7 +486,7 @@ __device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, c
             float d2 = 0.f;
             for (int k = l; k < t.chunks; k += lg) {
                 const float d = src[(int64_t)k * p.groups].x - mu;
-                d2 += d * d * (float)(ov_gn_tile_rows(p, t, k) * p.cg);
+                d2 += d * d * ((float)ov_gn_tile_rows(p, t, k) * (float)p.cg);
             }
             for (int o = lg / 2; o > 0; o >>= 1) d2 += __shfl_xor(d2, o, 64);
             if (l == 0) st[g] = make_float2(mu, 1.f / sqrtf((b + d2) / total + p.eps));
@@ -861,7 +861,8 @@ __global__ __launch_bounds__(1024) void ov_gn_any_param_kernel(const T* __restri
 
 static int ov_gn_check(const char* what, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, const void* w, const void* b, int32_t wdtype,
                        float eps, int32_t act, float drop, uint64_t seed, uint64_t offset, OvGn* p) {
-    if (N < 0 || S < 0 || C < 0 || groups < 1 || C % groups || (C > 0 && C < groups)) {
+    const int most = INT32_MAX - 65536;                   // indexes run past a size by up to a tile
+    if (N < 0 || S < 0 || C < 0 || N > most || S > most || C > most || groups < 1 || C % groups || (C > 0 && C < groups)) {
         ontovae_set_error("%s: N = %d, S = %d, C = %d, groups = %d (groups must divide C)", what, N, S, C, groups);
         return ONTOVAE_EINVAL;
     }
@@ -894,15 +895,15 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         q.form = OV_GN_ANY;
         return q;
     }
-    if (S == 1 && pieces <= 1024 * (8 / E)) {
+    if (S == 1 && pieces <= 2048) {
         q.form = OV_GN_ROW;
         if (pieces <= 64) {
             q.nv = 1;
             q.lpg = 8;
             while (q.lpg < pieces) q.lpg *= 2;
         } else {
-            q.lpg = pieces <= 64 * (16 / E) ? 64 : pieces <= 256 * (16 / E) ? 256 : 1024;
-            q.nv = 16 / E;                                // 1024 threads: half of it, 128 registers are all there are
+            q.lpg = pieces <= 128 ? 64 : pieces <= 512 ? 256 : 1024;
+            q.nv = pieces > 512 && pieces <= 1024 ? 1 : 2;        // two pieces of 1024 threads spill a few registers backward
         }
         // enough slots for four workgroups of 256 threads per CU.  Each row of gradient sums (a workgroup's where whole samples
         // fit it, else a slot's) is written and read once more: at most one to 8 samples
@@ -975,7 +976,7 @@ static int ov_gn_ready(const char* what, const OvGn& p, const OvGnPlan& q, const
         case 32: GO(32, 1); break;                                                             \
         case 64: if (q.nv == 1) { GO(64, 1); } else { GO(64, NVX); } break;                    \
         case 256: GO(256, NVX); break;                                                         \
-        default: GO(1024, NVX / 2); break;                                                         \
+        default: if (q.nv == 1) { GO(1024, 1); } else { GO(1024, NVX); } break;                                                         \
     }
 
 template <typename T, bool LIGHT>

@@ -180,7 +180,8 @@ GN_CASES = [   # N, S, C, groups
     (1, 1, 360, 8), (1, 1, 8, 1), (3, 1, 8, 8), (5, 1, 1000, 8), (130, 1, 1000, 40), (70, 1, 96, 1), (33, 1, 130, 13), (2, 1, 5893, 1),
     (9, 1, 5000, 5), (2, 1, 20000, 1), (3, 1, 40000, 2), (1, 1, 70001, 1), (700, 1, 64, 32),
     (2, 2, 8, 2), (3, 5, 30, 3), (2, 49, 320, 32), (1, 64, 128, 8), (4, 100, 77, 7), (2, 1024, 320, 32), (3, 1000, 96, 1), (1, 4096, 512, 32),
-    (2, 4097, 24, 4), (1, 20000, 16, 2), (2, 333, 1000, 8), (1, 7, 5893, 1), (64, 16, 320, 32), (1, 70000, 3, 3), (300, 3, 40, 4)]
+    (2, 4097, 24, 4), (1, 20000, 16, 2), (1, 1, 3, 3), (1, 2, 3, 1), (2, 1, 2, 2), (40, 1, 9000, 1), (3, 1, 16384, 1), (2, 1, 16385, 1), (17, 1, 4100, 2), (2, 3, 5000, 2), (700, 40, 24, 3),
+    (2, 333, 1000, 8), (1, 7, 5893, 1), (64, 16, 320, 32), (1, 70000, 3, 3), (300, 3, 40, 4)]
 
 
 def _gn_tol(o, x, t):

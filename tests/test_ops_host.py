@@ -91,7 +91,7 @@ GN = dict(x=P, dtype=0, N=2, S=3, C=8, groups=2, w=P, b=P, wdtype=0, eps=1e-5, a
           nbytes=1 << 30, stream=NULL)
 
 
-@pytest.mark.parametrize("change", [dict(N=-1), dict(S=-1), dict(C=-8), dict(groups=0), dict(groups=3), dict(groups=-2), dict(dtype=3), dict(wdtype=5),
+@pytest.mark.parametrize("change", [dict(N=-1), dict(S=-1), dict(C=-8), dict(N=2 ** 31 - 1), dict(S=2 ** 31 - 1), dict(C=2 ** 31 - 2), dict(groups=0), dict(groups=3), dict(groups=-2), dict(dtype=3), dict(wdtype=5),
                                     dict(act=4), dict(act=-1), dict(drop=-0.1), dict(drop=1.5), dict(drop=float("nan")), dict(eps=-1.0),
                                     dict(eps=float("nan")), dict(x=NULL), dict(y=NULL), dict(mean=NULL), dict(rstd=NULL)])
 def test_group_norm_act_refusals(L, change):
