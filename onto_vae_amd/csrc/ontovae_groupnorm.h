@@ -932,11 +932,12 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         q.form = OV_GN_TILE1;
         if (bytes > 65536) {
             q.form = OV_GN_TILE;
-            // up to 1024 workgroups of 16 rows a thread or more; where the samples are few, 256 of 4 rows or more, at most 128 a
+            // up to 768 workgroups, three a CU as the backward kernels' registers allow, of 16 rows a thread or more (32 x 4096 x 512 bf16
+            // trained: 236 us; 1024: 247, 2048: 262); where the samples are few, 256 of 4 rows or more, at most 128 a
             // sample (4 x 1024 x 320 float32 with gelu: 31 -> 19 us forward, 54 -> 27 backward; 60 x 3000 x 40 lost a fifth
             // with 900 workgroups of 4 rows, 1 x 4096 x 512 a fifth with 256 a sample)
             const int64_t few = std::min<int64_t>((S + t.ty * 4 - 1) / (t.ty * 4), std::min<int64_t>((256 + wg - 1) / wg, 128));
-            const int64_t many = std::min<int64_t>((S + t.ty * 16 - 1) / (t.ty * 16), (1024 + wg - 1) / wg);
+            const int64_t many = std::min<int64_t>((S + t.ty * 16 - 1) / (t.ty * 16), (768 + wg - 1) / wg);
             t.chunks = (int)std::max<int64_t>(1, std::max(few, many));
             t.rows = (S + t.chunks - 1) / t.chunks;
             t.chunks = (S + t.rows - 1) / t.rows;

@@ -559,10 +559,10 @@ static const int ov_q8_bm[5] = {32, 64, 128, 128, 256}, ov_q8_bn[5] = {128, 64, 
 
 // The form with the least estimated time: rounds of 256 workgroups at the share of the matrix rate that each tile reaches
 // (measured over 128 <= M, N <= 16384, 2048 <= K <= 20000), plus what cutting K costs: the slabs written and read, and a launch.
-// 8192^3: 256 x 256 524 us, 128 x 128 685, 64 x 64 912; 16384 x 360 x 20000: 128 x 192 188 us, 256 x 256 200, 128 x 128 230;
+// 8192^3: 256 x 256 524 us, 128 x 128 685, 64 x 64 912; 16384 x 360 x 20000: 128 x 192 174 us, 256 x 256 200, 128 x 128 230;
 // 4096 x 360 x 20000: 128 x 192 in 4 slabs 54 us, 64 x 64 uncut 75; 2048^3: 128 x 128 17.6 us, 64 x 64 19.6, 128 x 192 42.
 static OvQ8Plan ov_q8_plan(int M, int N, int K) {
-    static const double share[5] = {0.15, 0.24, 0.32, 0.30, 0.45};
+    static const double share[5] = {0.15, 0.24, 0.32, 0.33, 0.45};
     const int steps = std::max((K + 127) / 128, 1);
     OvQ8Plan best{};
     double least = 1e300;
