@@ -25,6 +25,11 @@ I32_MAX = 2 ** 31 - 1
 _SAME = contextlib.nullcontext()
 
 
+def _gpu(t, what):
+    if not t.is_cuda:
+        _need_gpu(t, what)
+
+
 def _on(device):
     """The tensors' device as the current one (entering torch's guard only when it changes something)."""
     return _SAME if torch.cuda.current_device() == device.index else torch.cuda.device(device)
@@ -52,22 +57,19 @@ def _dtype(t, what):
     return DTYPES[t.dtype]
 
 
-def _size(n, what):
-    if n > I32_MAX:
-        raise ValueError(f"{what}: a dimension of {n} exceeds {I32_MAX}")
-    return int(n)
-
-
 def _matrix(x, what):
     """[..., C] as a 2-D view with unit inner stride (copied only when its strides leave no other way)."""
     if x.dim() < 1:
         raise ValueError(f"{what}: at least one dimension expected")
     m = x if x.dim() == 2 else x.reshape(math.prod(x.shape[:-1]), x.shape[-1])
-    if m.stride(1) != 1 and m.shape[1] > 1 or m.stride(0) < m.shape[1] and m.shape[0] > 1:
+    R, Cn = m.shape
+    if R > I32_MAX or Cn > I32_MAX:
+        raise ValueError(f"{what}: a dimension of {tuple(m.shape)} exceeds {I32_MAX}")
+    ld, inner = m.stride()
+    if inner != 1 and Cn > 1 or ld < Cn and R > 1:
         m = m.contiguous()
-    _size(m.shape[0], what)
-    _size(m.shape[1], what)
-    return m, max(m.stride(0), m.shape[1])
+        ld = Cn
+    return m, max(ld, Cn)
 
 
 def _rows(rows, x, what):
@@ -103,7 +105,7 @@ def quantize_rows(x, rows=None):
     q = x / scale rounded to the nearest integer, ties to even.  q has shape [..., K] and a row stride padded with zeros to a
     multiple of 64, the layout int8_matmul reads fastest.  A row that holds an infinity or a NaN (or a row index outside x) gets
     the scale NaN."""
-    _need_gpu(x, "quantize_rows")
+    _gpu(x, "quantize_rows")
     dt = _dtype(x, "quantize_rows")
     rows = _rows(rows, x, "quantize_rows")
     xm, ld = _matrix(x, "quantize_rows")
@@ -125,7 +127,7 @@ def quantize_rows(x, rows=None):
 def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
     """y [..., N] = (a [..., K] . b [N, K]^T) a_scale[..., None] b_scale + bias: int8 operands with one float32 scale per row of each
     (quantize_rows), the sum over K (at most 131071) exact, bias float32 [N], y rounded once to `dtype`."""
-    _need_gpu(a, "int8_matmul")
+    _gpu(a, "int8_matmul")
     if a.dtype != torch.int8 or b.dtype != torch.int8 or b.dim() != 2 or a.dim() < 1 or a.shape[-1] != b.shape[1] or a.device != b.device:
         raise ValueError("int8_matmul: int8 a [..., K] and b [N, K] on one device expected")
     if dtype not in DTYPES:
@@ -151,7 +153,7 @@ def int8_matmul(a, a_scale, b, b_scale, bias=None, dtype=torch.float32):
 def int8_linear(x, weight, weight_scale, bias=None, rows=None, dtype=None):
     """x weight^T + bias with an 8-bit weight [N, K] (quantize_rows of the layer's float weight, done once) and the rows of x (of
     x[rows]) quantised on the way: one scale per token and per output channel.  dtype: that of y, x's by default."""
-    _need_gpu(x, "int8_linear")
+    _gpu(x, "int8_linear")
     dt = _dtype(x, "int8_linear")
     if dtype is None:
         dtype = x.dtype
@@ -177,7 +179,7 @@ def int8_linear(x, weight, weight_scale, bias=None, rows=None, dtype=None):
 
 # ---------------------------------------------------------------- group norm with an activation
 def _gn_args(x, groups, weight, bias, act, drop, seed, offset, what):
-    _need_gpu(x, what)
+    _gpu(x, what)
     dt = _dtype(x, what)
     shape = x.shape
     if len(shape) < 2:
@@ -253,7 +255,7 @@ def dropout(x, p, seed, offset=0, rows=None):
     """Inverted dropout of a [..., C] tensor (of the rows x[rows] of a matrix): each element is 0 with probability p, else divided
     by 1 - p.  The mask is a function of (seed, offset, row, channel) alone -- Philox4x32-10, 16 bits an element, so p is taken to
     the nearest 2^-16 -- and is never stored; use another offset for each draw.  A non-finite element in a dropped place gives 0."""
-    _need_gpu(x, "dropout")
+    _gpu(x, "dropout")
     dt = _dtype(x, "dropout")
     if not 0.0 <= float(p) <= 1.0:
         raise ValueError(f"dropout: p = {p} outside [0, 1]")
