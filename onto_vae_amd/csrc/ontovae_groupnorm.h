@@ -859,10 +859,11 @@ __global__ __launch_bounds__(1024) void ov_gn_any_param_kernel(const T* __restri
     }
 }
 
+#define OV_GN_MOST (INT32_MAX - 65536)                    // indexes run past a size by up to a tile
+
 static int ov_gn_check(const char* what, int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, const void* w, const void* b, int32_t wdtype,
                        float eps, int32_t act, float drop, uint64_t seed, uint64_t offset, OvGn* p) {
-    const int most = INT32_MAX - 65536;                   // indexes run past a size by up to a tile
-    if (N < 0 || S < 0 || C < 0 || N > most || S > most || C > most || groups < 1 || C % groups || (C > 0 && C < groups)) {
+    if (N < 0 || S < 0 || C < 0 || std::max({N, S, C}) > OV_GN_MOST || groups < 1 || C % groups || (C > 0 && C < groups)) {
         ontovae_set_error("%s: N = %d, S = %d, C = %d, groups = %d (groups must divide C)", what, N, S, C, groups);
         return ONTOVAE_EINVAL;
     }
@@ -907,10 +908,10 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         }
         // enough slots for four workgroups of 256 threads per CU.  Each row of gradient sums (a workgroup's where whole samples
         // fit it, else a slot's) is written and read once more: at most one to 8 samples
-        const int per = groups * q.lpg;
-        q.wgs = q.lpg < 256 && per <= 128 && 256 % per == 0 ? 256 / per : 1;
-        const int64_t want = std::max<int64_t>(262144 / (int64_t)per, 1);
-        const int64_t most = std::max((int64_t)(N + 7) / 8, std::min<int64_t>(N, 65536 / std::min(per * q.wgs, 65536))) * q.wgs;
+        const int64_t per = (int64_t)groups * q.lpg;          // threads of a sample, up to 2^34
+        q.wgs = q.lpg < 256 && per <= 128 && 256 % per == 0 ? 256 / (int)per : 1;
+        const int64_t want = std::max<int64_t>(262144 / per, 1);
+        const int64_t most = std::max<int64_t>(((int64_t)N + 7) / 8, std::min<int64_t>(N, 65536 / std::min<int64_t>(per * q.wgs, 65536))) * q.wgs;
         q.RS = (int)std::min<int64_t>(want, backward ? std::min<int64_t>(most, N) : N);
         q.chan_rows = q.wgs > 1 ? (q.RS + q.wgs - 1) / q.wgs : q.RS;
         q.chan_floats = backward ? 2 * q.chan_rows * C : 0;
@@ -954,7 +955,7 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
 static int64_t ov_gn_ws(const OvGnPlan& q) { return ((q.part_floats + 63) / 64 * 64 + q.chan_floats) * 4; }
 
 extern "C" int64_t ontovae_group_norm_act_workspace_bytes(int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, int32_t backward) {
-    if (N < 1 || S < 1 || C < 1 || groups < 1 || C % groups || dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) return 0;
+    if (N < 1 || S < 1 || C < 1 || std::max({N, S, C}) > OV_GN_MOST || groups < 1 || C % groups || dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) return 0;
     return ov_gn_ws(ov_gn_plan(dtype, N, S, C, groups, backward != 0));
 }
 
