@@ -10,6 +10,7 @@
 #include "ontovae_ops.h"
 
 #define OV_Q8_MAX_K 131071          // 128 * 128 * K < 2^31
+#define OV_Q8_MAX_MN (INT32_MAX - 1024)        // row and column indexes run past M and N by up to a tile
 
 typedef int ov_i32x4 __attribute__((ext_vector_type(4)));
 typedef int ov_i32x16 __attribute__((ext_vector_type(16)));
@@ -561,13 +562,13 @@ static const int ov_q8_bm[5] = {32, 64, 128, 128, 256}, ov_q8_bn[5] = {128, 64, 
 // (measured over 128 <= M, N <= 16384, 2048 <= K <= 20000), plus what cutting K costs: the slabs written and read, and a launch.
 // 8192^3: 256 x 256 524 us, 128 x 128 685, 64 x 64 912; 16384 x 360 x 20000: 128 x 192 174 us, 256 x 256 200, 128 x 128 230;
 // 4096 x 360 x 20000: 128 x 192 in 4 slabs 54 us, 64 x 64 uncut 75; 2048^3: 128 x 128 17.6 us, 64 x 64 19.6, 128 x 192 42.
-static OvQ8Plan ov_q8_plan(int M, int N, int K) {
+static OvQ8Plan ov_q8_plan(int64_t M, int64_t N, int K) {
     static const double share[5] = {0.15, 0.24, 0.32, 0.33, 0.45};
     const int steps = std::max((K + 127) / 128, 1);
     OvQ8Plan best{};
     double least = 1e300;
     for (int c = M <= 32 ? OV_Q8_T32 : OV_Q8_T64; c <= (M <= 32 ? OV_Q8_T32 : OV_Q8_T256); ++c) {
-        const int64_t t = (int64_t)((M + ov_q8_bm[c] - 1) / ov_q8_bm[c]) * ((N + ov_q8_bn[c] - 1) / ov_q8_bn[c]);
+        const int64_t t = ((M + ov_q8_bm[c] - 1) / ov_q8_bm[c]) * ((N + ov_q8_bn[c] - 1) / ov_q8_bn[c]);
         const int cut = (int)std::min<int64_t>((256 + t - 1) / t, std::max(steps / 4, 1));      // a slab has 4 steps at least
         for (int s : {1, cut}) {
             const int per = (steps + s - 1) / s, n = (steps + per - 1) / per;
@@ -614,7 +615,7 @@ static int ov_q8_gemm_launch(OvQ8Gemm g, const OvQ8Plan& p, bool direct, hipStre
 }
 
 extern "C" int64_t ontovae_int8_matmul_workspace_bytes(int32_t M, int32_t N, int32_t K) {
-    if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K) return 0;
+    if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K || std::max(M, N) > OV_Q8_MAX_MN) return 0;
     const OvQ8Plan p = ov_q8_plan(M, N, K);
     return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
 }
@@ -648,7 +649,7 @@ static int ov_q8_matmul(const int8_t* a, int64_t lda, int64_t ast, const float* 
     return ONTOVAE_OK;
 }
 
-static bool ov_q8_too_many(int M, int N) { return std::max(M, N) > INT32_MAX - 1024 || ((int64_t)M + 31) / 32 * (((int64_t)N + 63) / 64) > INT32_MAX; }
+static bool ov_q8_too_many(int M, int N) { return std::max(M, N) > OV_Q8_MAX_MN || ((int64_t)M + 31) / 32 * (((int64_t)N + 63) / 64) > INT32_MAX; }
 
 extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb,
                                    const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t dtype, int64_t ldy, void* workspace,
@@ -679,7 +680,7 @@ static int64_t ov_q8_blocks(int K) { return std::max<int64_t>(((int64_t)K + 127)
 static bool ov_q8_few(int M, int K) { return M <= 4 && K <= 32768 && (M <= 2 || K <= 20480); }
 
 extern "C" int64_t ontovae_int8_linear_workspace_bytes(int32_t M, int32_t N, int32_t K) {
-    if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K || ov_q8_few(M, K)) return 0;
+    if (M <= 0 || N <= 0 || K < 0 || K > OV_Q8_MAX_K || std::max(M, N) > OV_Q8_MAX_MN || ov_q8_few(M, K)) return 0;
     const int64_t head = (M * ov_q8_blocks(K) * 128 + 255) / 256 * 256 + ((int64_t)M * 4 + 255) / 256 * 256;
     return head + ontovae_int8_matmul_workspace_bytes(M, N, K);
 }
@@ -688,11 +689,12 @@ extern "C" int64_t ontovae_int8_linear_workspace_bytes(int32_t M, int32_t N, int
 int64_t ov_int8_linear_bytes_upto(int max_M, int N, int K) {
     int64_t slabs = 0;
     for (int c = 0; c < 5; ++c) {
-        const int64_t t = std::min<int64_t>((int64_t)((max_M + ov_q8_bm[c] - 1) / ov_q8_bm[c]) * ((N + ov_q8_bn[c] - 1) / ov_q8_bn[c]), 255);
+        const int64_t t = std::min<int64_t>((((int64_t)max_M + ov_q8_bm[c] - 1) / ov_q8_bm[c]) * (((int64_t)N + ov_q8_bn[c] - 1) / ov_q8_bn[c]), 255);
         slabs = std::max(slabs, (256 + t) * ov_q8_bm[c] * ov_q8_bn[c]);
     }
     const int64_t cuts = std::min<int64_t>(256, std::max((K + 127) / 128 / 4, 1));
-    slabs = std::min(slabs, cuts * max_M * N);
+    const int64_t one = std::min<int64_t>((int64_t)max_M * N, slabs);        // `slabs` stays below 2^26: no product wraps
+    slabs = std::min(slabs, cuts * one);
     return (max_M * ov_q8_blocks(K) * 128 + 255) / 256 * 256 + ((int64_t)max_M * 4 + 255) / 256 * 256 + slabs * 4;
 }
 

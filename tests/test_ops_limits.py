@@ -34,3 +34,24 @@ def test_group_norm_sizing_of_many_groups():
 def test_group_norm_sizing_past_the_sizes_it_takes(N, S, C, groups):
     """Sizes that the entry points refuse: no workspace, nothing divided by what wrapped to 0."""
     assert call(f"L.ontovae_group_norm_act_workspace_bytes(0, {N}, {S}, {C}, {groups}, 1)") == [0]
+
+
+@pytest.mark.parametrize("name", ["int8_matmul", "int8_linear"])
+def test_int8_sizing_at_the_ends(name):
+    """M or N next to 2^31: rounded up to whole tiles it passes 32 bits.  0 for the sizes that the entry points refuse; below them
+    the rows in 8 bits (linear) and no slabs, as there are tiles enough."""
+    f = f"L.ontovae_{name}_workspace_bytes"
+    assert call(f"{f}({TOP}, 64, 64)", f"{f}(64, {TOP}, 64)", f"{f}({TOP}, {TOP}, 64)", f"{f}({TOP - 1023}, 64, 64)") == [0] * 4
+    big = TOP - 1024
+    row = (big * 128 + 255) // 256 * 256 + (big * 4 + 255) // 256 * 256 if name == "int8_linear" else 0
+    few = 64 * 128 + 256 if name == "int8_linear" else 0
+    assert call(f"{f}({big}, 64, 64)", f"{f}(64, {big}, 64)") == [row, few]
+
+
+def test_int8_workspace_of_a_model_at_the_ends():
+    """What a model asks for its largest batch is enough for the largest batch itself."""
+    got = call(*(f"(lambda d: (setattr(d, 'L', {L}), setattr(d, 'G', {G}), L.ontovae_int8_workspace_bytes(C.byref(d), {B}), "
+                 f"L.ontovae_int8_linear_workspace_bytes({B}, {L}, {G}))[2:])(_lib.Dims())" for L, G, B in
+                 ((360, 1000, TOP - 1024), (360, 20000, 2 ** 30), (1, 1, TOP - 1024), (360, 20000, 16384))))
+    for (have, need), (L_, G, B) in zip(got, ((360, 1000, TOP - 1024), (360, 20000, 2 ** 30), (1, 1, TOP - 1024), (360, 20000, 16384))):
+        assert have >= need + L_ * G + 4 * L_ + 4 * L_ * B > 0
