@@ -730,6 +730,7 @@ extern "C" int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, co
     }
     if (M == 0 || N == 0) return ONTOVAE_OK;
     if (!sw || !y || (K > 0 && (!x || !w))) { ontovae_set_error("int8_linear: NULL argument"); return ONTOVAE_EINVAL; }
+    if (ov_q8_too_many(M, N)) { ontovae_set_error("int8_linear: M = %d, N = %d: too many tiles", M, N); return ONTOVAE_EINVAL; }
     const int64_t need = ontovae_int8_linear_workspace_bytes(M, N, K);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) {
         ontovae_set_error("int8_linear: workspace of %lld bytes, 256-B aligned, needed", (long long)need);
@@ -744,7 +745,6 @@ extern "C" int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, co
         OV_OPS_LAUNCH_CHECK("int8_linear");
         return ONTOVAE_OK;
     }
-    if (ov_q8_too_many(M, N)) { ontovae_set_error("int8_linear: M = %d, N = %d: too many tiles", M, N); return ONTOVAE_EINVAL; }
     const int64_t nb = ov_q8_blocks(K), kst = (int64_t)M * 128;
     char* p = static_cast<char*>(workspace);
     int8_t* q = reinterpret_cast<int8_t*>(p);

@@ -55,3 +55,12 @@ def test_int8_workspace_of_a_model_at_the_ends():
                  ((360, 1000, TOP - 1024), (360, 20000, 2 ** 30), (1, 1, TOP - 1024), (360, 20000, 16384))))
     for (have, need), (L_, G, B) in zip(got, ((360, 1000, TOP - 1024), (360, 20000, 2 ** 30), (1, 1, TOP - 1024), (360, 20000, 16384))):
         assert have >= need + L_ * G + 4 * L_ + 4 * L_ * B > 0
+
+
+@pytest.mark.parametrize("M", [1, 2, 4, 5])
+def test_int8_linear_refuses_more_columns_than_its_indexes_hold(M):
+    """The few-row form walks the weight rows with 32-bit steps of its grid: past 2^31 - 1024 rows they would wrap to negative ones.  (Its
+    refusal is read from the message: where there is no card a launch fails, too.)"""
+    for N in (TOP - 1023, TOP):
+        rc, text = call(f"L.ontovae_int8_linear(P, 0, 1, NULL, {M}, P, 1, P, NULL, {M}, {N}, 1, P, 0, {N}, P, 1 << 40, NULL)", "err()")
+        assert rc == -1 and "int8_linear" in text and str(N) in text
