@@ -587,7 +587,8 @@ int ontovae_vae_adamw_apply(const ontovae_vae_ctx_t* ctx, const ontovae_adamw_t*
  * onto_vae_amd/ops.py.  No counterpart in the reference, whose blocks are torch's Linear / BatchNorm1d / Dropout / ReLU
  * (onto_vae/modules.py:43-64, 116-133).  Element types: ONTOVAE_F32 / _BF16 / _F16; every sum and statistic is held in 32 bits,
  * each output is rounded once.  Asynchronous on `stream`, no allocation, safe under graph capture (seed and offset are
- * recorded by value: a replay draws the same mask).
+ * recorded by value: a replay draws the same mask).  Sizes that would take 2^32 threads or more in one launch are refused: dropout of
+ * more than 3.4e10 elements, group norm of more than 1.6e7 samples of several rows, 6.7e7 rows in 8 bits.
  * -------------------------------------------------------------------------------------------*/
 enum { ONTOVAE_F32 = 0, ONTOVAE_BF16 = 1, ONTOVAE_F16 = 2 };
 enum { ONTOVAE_ACT_NONE = 0, ONTOVAE_ACT_RELU = 1, ONTOVAE_ACT_SILU = 2, ONTOVAE_ACT_GELU = 3 };

@@ -102,7 +102,7 @@ template <typename T>
 static int ov_dropout_launch(const void* x, int64_t ldx, const int32_t* rows, int n_src, int R, int C, const OvDrop& d, void* y, hipStream_t st) {
     const uint32_t nb = ((uint32_t)C + 7) / 8;
     const int64_t wg = ((int64_t)R * nb + 255) / 256;
-    if (wg > INT32_MAX) { ontovae_set_error("dropout: %d x %d elements are too many for one launch", R, C); return ONTOVAE_EINVAL; }
+    if (!ov_ops_fits(wg, 256)) { ontovae_set_error("dropout: %d x %d elements are too many for one launch", R, C); return ONTOVAE_EINVAL; }
     hipLaunchKernelGGL(ov_dropout_kernel<T>, dim3((unsigned)wg), dim3(256), 0, st, static_cast<const T*>(x), ldx, rows, n_src, R, C, nb, d, static_cast<T*>(y));
     return ONTOVAE_OK;
 }

@@ -959,15 +959,21 @@ extern "C" int64_t ontovae_group_norm_act_workspace_bytes(int32_t dtype, int32_t
     return ov_gn_ws(ov_gn_plan(dtype, N, S, C, groups, backward != 0));
 }
 
-static int ov_gn_ready(const char* what, const OvGn& p, const OvGnPlan& q, const void* ws, int64_t bytes) {
+// sums: the gradients of weight or bias are wanted
+static int ov_gn_ready(const char* what, const OvGn& p, const OvGnPlan& q, bool sums, const void* ws, int64_t bytes) {
     const int64_t need = ov_gn_ws(q);
     if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255))) {
         ontovae_set_error("%s: workspace of %lld bytes, 256-B aligned, needed", what, (long long)need);
         return ONTOVAE_EINVAL;
     }
-    const int64_t wg = q.form == OV_GN_ROW ? ((int64_t)q.RS * p.groups * q.lpg + 255) / 256
+    const int threads = q.form == OV_GN_ROW ? std::max(q.lpg, 256) : q.form == OV_GN_ANY ? 1024 : 256;
+    const int64_t wg = q.form == OV_GN_ROW ? ((int64_t)q.RS * p.groups * q.lpg + threads - 1) / threads
                        : q.form == OV_GN_ANY ? (int64_t)p.N * p.groups : (int64_t)p.N * q.t.chunks * q.t.nblk;
-    if (wg > INT32_MAX) { ontovae_set_error("%s: N = %d with %d groups: too many workgroups", what, p.N, p.groups); return ONTOVAE_EINVAL; }
+    const int64_t sum_wg = !sums ? 0 : q.form == OV_GN_ANY ? ((int64_t)p.C + 63) / 64 : ((int64_t)p.C + 15) / 16;
+    if (!ov_ops_fits(wg, threads) || !ov_ops_fits(sum_wg, 1024)) {
+        ontovae_set_error("%s: N = %d, S = %d, C = %d with %d groups are too many for one launch", what, p.N, p.S, p.C, p.groups);
+        return ONTOVAE_EINVAL;
+    }
     return ONTOVAE_OK;
 }
 
@@ -1021,7 +1027,7 @@ extern "C" int ontovae_group_norm_act(const void* x, int32_t dtype, int32_t N, i
     if (N == 0 || S == 0 || C == 0) return ONTOVAE_OK;
     if (!x || !y || !mean || !rstd) { ontovae_set_error("group_norm_act: NULL argument"); return ONTOVAE_EINVAL; }
     const OvGnPlan q = ov_gn_plan(dtype, N, S, C, groups, false);
-    if ((rc = ov_gn_ready("group_norm_act", p, q, workspace, workspace_bytes))) return rc;
+    if ((rc = ov_gn_ready("group_norm_act", p, q, false, workspace, workspace_bytes))) return rc;
     hipStream_t st = reinterpret_cast<hipStream_t>(stream);
     switch (dtype) {
         case ONTOVAE_F32: ov_gn_fwd_launch<float>(x, p, q, y, mean, rstd, workspace, st); break;
@@ -1093,7 +1099,7 @@ extern "C" int ontovae_group_norm_act_backward(const void* dy, const void* x, in
     }
     if (!dy || !x || !mean || !rstd || !dx) { ontovae_set_error("group_norm_act_backward: NULL argument"); return ONTOVAE_EINVAL; }
     const OvGnPlan q = ov_gn_plan(dtype, N, S, C, groups, true);
-    if ((rc = ov_gn_ready("group_norm_act_backward", p, q, workspace, workspace_bytes))) return rc;
+    if ((rc = ov_gn_ready("group_norm_act_backward", p, q, dweight || dbias, workspace, workspace_bytes))) return rc;
     switch (dtype) {
         case ONTOVAE_F32: ov_gn_bwd_launch<float>(dy, x, p, q, mean, rstd, dx, dweight, dbias, workspace, st); break;
         case ONTOVAE_BF16: ov_gn_bwd_launch<ov_bf>(dy, x, p, q, mean, rstd, dx, dweight, dbias, workspace, st); break;

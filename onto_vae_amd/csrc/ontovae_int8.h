@@ -510,6 +510,18 @@ __global__ __launch_bounds__(256) void ov_q8_few_kernel(const T* __restrict__ x,
 }
 
 // ---------------------------------------------------------------- host
+// threads that share a row of p pieces; 64: four rows a workgroup
+static int ov_q8_row_threads(int p, int M) {
+    if (p <= 256) return 64;
+    if (p <= 1024) return 256;
+    if (p <= 2048) return 512;
+    return p <= 5120 && M > 512 ? 512 : 1024;                 // up to 512 rows, one round of workgroups: fewer pieces one behind the other
+}
+static bool ov_q8_rows_fit(int dtype, int M, int K) {
+    const int ve = dtype == ONTOVAE_F32 ? 4 : 8, th = ov_q8_row_threads((K + ve - 1) / ve, M);
+    return th < 256 ? ov_ops_fits(((int64_t)M + 3) / 4, 256) : ov_ops_fits(M, th);
+}
+
 template <typename T>
 static void ov_q8_rows_launch(const void* x, int64_t ldx, const int32_t* rows, int n_src, int M, int K, int8_t* q, int64_t ldq, int64_t kst,
                               int64_t kpad, float* scale, hipStream_t st) {
@@ -519,13 +531,12 @@ static void ov_q8_rows_launch(const void* x, int64_t ldx, const int32_t* rows, i
 #define OV_Q8_ROWS(TH, NV) \
     hipLaunchKernelGGL((ov_q8_rows_kernel<T, TH, NV>), dim3((unsigned)(TH < 256 ? ((int64_t)M + 3) / 4 : (int64_t)M)), dim3(TH < 256 ? 256 : TH), 0, st, xt, ldx, rows, n_src, M, K, q, \
                        ldq, kst, kpad, scale)
-    if (p <= 64) OV_Q8_ROWS(64, 1);
-    else if (p <= 256) OV_Q8_ROWS(64, 4);
-    else if (p <= 1024) OV_Q8_ROWS(256, 4);
-    else if (p <= 2048) OV_Q8_ROWS(512, 4);
-    else if (p <= 5120 && M <= 512) OV_Q8_ROWS(1024, 5);      // one round of workgroups: fewer pieces one behind the other
-    else if (p <= 5120) OV_Q8_ROWS(512, 10);
-    else OV_Q8_ROWS(1024, 16);
+    switch (ov_q8_row_threads(p, M)) {
+        case 64: if (p <= 64) { OV_Q8_ROWS(64, 1); } else { OV_Q8_ROWS(64, 4); } break;
+        case 256: OV_Q8_ROWS(256, 4); break;
+        case 512: if (p <= 2048) { OV_Q8_ROWS(512, 4); } else { OV_Q8_ROWS(512, 10); } break;
+        default: if (p <= 5120) { OV_Q8_ROWS(1024, 5); } else { OV_Q8_ROWS(1024, 16); } break;
+    }
 #undef OV_Q8_ROWS
 }
 
@@ -548,6 +559,7 @@ extern "C" int ontovae_quantize_rows(const void* x, int32_t dtype, int64_t ldx, 
     }
     if (K > (1 << 30)) { ontovae_set_error("quantize_rows: K = %d, rows of up to 2^30 elements", K); return ONTOVAE_EINVAL; }
     if (dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) { ontovae_set_error("quantize_rows: unknown element type %d", dtype); return ONTOVAE_EINVAL; }
+    if (!ov_q8_rows_fit(dtype, M, K)) { ontovae_set_error("quantize_rows: %d rows of %d are too many for one launch", M, K); return ONTOVAE_EINVAL; }
     if (M == 0) return ONTOVAE_OK;
     if (!scale || (K > 0 && (!x || !q))) { ontovae_set_error("quantize_rows: NULL argument"); return ONTOVAE_EINVAL; }
     return ov_q8_rows_any(x, dtype, ldx, rows, n_src, M, K, q, ldq, 128, ldq, scale, reinterpret_cast<hipStream_t>(stream));
@@ -620,13 +632,23 @@ extern "C" int64_t ontovae_int8_matmul_workspace_bytes(int32_t M, int32_t N, int
     return p.splits > 1 ? (int64_t)p.splits * M * N * 4 : 0;
 }
 
+// operands whose rows start on 16 B, at 32-bit offsets inside a tile
+static bool ov_q8_direct(const int8_t* a, int64_t lda, const int8_t* b, int64_t ldb) {
+    return ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (uintptr_t)lda | (uintptr_t)ldb) & 15) == 0 &&
+           std::max(lda, ldb) < (1 << 23);
+}
+// more tiles than one launch takes (tiles of 64 x 64 by 256 threads where the operands are not direct)
+static bool ov_q8_too_many(int64_t M, int64_t N, int K, bool direct) {
+    if (std::max(M, N) > OV_Q8_MAX_MN) return true;
+    const int cfg = direct ? ov_q8_plan(M, N, K).cfg : OV_Q8_T64;
+    return !ov_ops_fits(((M + ov_q8_bm[cfg] - 1) / ov_q8_bm[cfg]) * ((N + ov_q8_bn[cfg] - 1) / ov_q8_bn[cfg]), cfg >= OV_Q8_T192 ? 512 : 256);
+}
+
 // the product on checked arguments; column k of row m of a at (k / 128) ast + m lda + k % 128
 static int ov_q8_matmul(const int8_t* a, int64_t lda, int64_t ast, const float* sa, const int8_t* b, int64_t ldb, const float* sb, const float* bias,
                         int M, int N, int K, void* y, int dtype, int64_t ldy, void* workspace, hipStream_t st) {
     const OvQ8Plan p = ov_q8_plan(M, N, K);
-    // 16-B pieces at 32-bit offsets inside a tile's rows
-    const bool direct = ((reinterpret_cast<uintptr_t>(a) | reinterpret_cast<uintptr_t>(b) | (uintptr_t)lda | (uintptr_t)ldb) & 15) == 0 &&
-                        std::max(lda, ldb) < (1 << 23);
+    const bool direct = ov_q8_direct(a, lda, b, ldb);
     OvQ8Gemm g{a, lda, ast, b, ldb, sa, sb, bias, M, N, K, 0, 0, 0, static_cast<int32_t*>(workspace), y, ldy};
     int rc;
     if (p.splits > 1) {
@@ -649,8 +671,6 @@ static int ov_q8_matmul(const int8_t* a, int64_t lda, int64_t ast, const float* 
     return ONTOVAE_OK;
 }
 
-static bool ov_q8_too_many(int M, int N) { return std::max(M, N) > OV_Q8_MAX_MN || ((int64_t)M + 31) / 32 * (((int64_t)N + 63) / 64) > INT32_MAX; }
-
 extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa, const int8_t* b, int64_t ldb, const float* sb,
                                    const float* bias, int32_t M, int32_t N, int32_t K, void* y, int32_t dtype, int64_t ldy, void* workspace,
                                    int64_t workspace_bytes, void* stream) {
@@ -663,7 +683,7 @@ extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa
     if (dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) { ontovae_set_error("int8_matmul: unknown element type %d", dtype); return ONTOVAE_EINVAL; }
     if (M == 0 || N == 0) return ONTOVAE_OK;
     if (!sa || !sb || !y || (K > 0 && (!a || !b))) { ontovae_set_error("int8_matmul: NULL argument"); return ONTOVAE_EINVAL; }
-    if (ov_q8_too_many(M, N)) { ontovae_set_error("int8_matmul: M = %d, N = %d: too many tiles", M, N); return ONTOVAE_EINVAL; }
+    if (ov_q8_too_many(M, N, K, ov_q8_direct(a, lda, b, ldb))) { ontovae_set_error("int8_matmul: M = %d, N = %d: too many tiles", M, N); return ONTOVAE_EINVAL; }
     const int64_t need = ontovae_int8_matmul_workspace_bytes(M, N, K);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) {
         ontovae_set_error("int8_matmul: workspace of %lld bytes, 256-B aligned, needed", (long long)need);
@@ -730,7 +750,11 @@ extern "C" int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, co
     }
     if (M == 0 || N == 0) return ONTOVAE_OK;
     if (!sw || !y || (K > 0 && (!x || !w))) { ontovae_set_error("int8_linear: NULL argument"); return ONTOVAE_EINVAL; }
-    if (ov_q8_too_many(M, N)) { ontovae_set_error("int8_linear: M = %d, N = %d: too many tiles", M, N); return ONTOVAE_EINVAL; }
+    // (the rows in 8 bits are laid out in the workspace for the direct form)
+    if (ov_q8_too_many(M, N, K, ov_q8_direct(nullptr, 128, w, ldw)) || !ov_q8_rows_fit(dtype, M, K)) {
+        ontovae_set_error("int8_linear: M = %d, N = %d, K = %d are too many for one launch", M, N, K);
+        return ONTOVAE_EINVAL;
+    }
     const int64_t need = ontovae_int8_linear_workspace_bytes(M, N, K);
     if (need > 0 && (!workspace || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 255))) {
         ontovae_set_error("int8_linear: workspace of %lld bytes, 256-B aligned, needed", (long long)need);

@@ -11,6 +11,9 @@
         if (e_ != hipSuccess) { ontovae_set_error("%s: %s", what, hipGetErrorString(e_)); return ONTOVAE_EHIP; }      \
     } while (0)
 
+// one launch takes less than 2^32 threads along x
+static inline bool ov_ops_fits(int64_t workgroups, int threads) { return workgroups <= (int64_t)UINT32_MAX / threads; }
+
 typedef __bf16 ov_bf;
 typedef _Float16 ov_hf;
 

@@ -64,3 +64,54 @@ def test_int8_linear_refuses_more_columns_than_its_indexes_hold(M):
     for N in (TOP - 1023, TOP):
         rc, text = call(f"L.ontovae_int8_linear(P, 0, 1, NULL, {M}, P, 1, P, NULL, {M}, {N}, 1, P, 0, {N}, P, 1 << 40, NULL)", "err()")
         assert rc == -1 and "int8_linear" in text and str(N) in text
+
+
+def refused(expr, *words):
+    rc, text = call(expr, "err()")
+    assert rc == -1, (rc, text)           # the library's refusal, not the runtime's
+    assert all(w in text for w in words), text
+
+
+@pytest.mark.parametrize("R,C,dtype", [(2 ** 29, 64, 0), (2 ** 29, 57, 1), (TOP, 16, 2), (TOP, TOP, 0), (16, TOP - 7, 1), (17, TOP, 1)])
+def test_dropout_of_more_than_one_launch(R, C, dtype):
+    """One thread per 8 elements, less than 2^32 of them."""
+    refused(f"L.ontovae_dropout(P, {dtype}, {C}, NULL, {R}, {R}, {C}, 0.5, 1, 1, P, NULL)", "dropout", "too many")
+
+
+@pytest.mark.parametrize("N,S,C,groups", [
+    (1, 1, 2 ** 29, 2 ** 29),          # one sample of 2^32 threads
+    (1, 1, 2 ** 30, 2 ** 30),
+    (2 ** 24, 2, 8, 2),                # a workgroup a sample
+    (2 ** 24, 2, 8, 8),
+    (2 ** 22, 1, 16385, 1),            # the general form: 1024 threads a group
+    (2 ** 22, 2, 2049, 1),
+    (TOP - 65536, TOP - 65536, 8, 1)])
+def test_group_norm_of_more_than_one_launch(N, S, C, groups):
+    refused(f"L.ontovae_group_norm_act(P, 0, {N}, {S}, {C}, {groups}, P, P, 0, 1e-5, 0, 0.0, 0, 0, P, P, P, P, 1 << 62, NULL)",
+            "group_norm_act", "too many")
+    refused(f"L.ontovae_group_norm_act_backward(P, P, 0, {N}, {S}, {C}, {groups}, P, P, 0, P, P, 0, 0.0, 0, 0, P, P, P, P, 1 << 62, NULL)",
+            "group_norm_act_backward", "too many")
+
+
+def test_group_norm_parameter_gradients_of_more_than_one_launch():
+    """64 threads a channel: the gradient sums of 2^26 channels are refused before anything is written."""
+    for dw, db in (("P", "P"), ("P", "NULL"), ("NULL", "P")):
+        refused(f"L.ontovae_group_norm_act_backward(P, P, 0, 1, 1, {2 ** 26}, {2 ** 13}, P, P, 0, P, P, 0, 0.0, 0, 0, P, {dw}, {db}, P, 1 << 62, NULL)",
+                "group_norm_act_backward", "too many")
+
+
+@pytest.mark.parametrize("M,K,dtype", [(2 ** 26, 8, 0), (TOP, 1, 1), (2 ** 24, 2000, 0), (2 ** 23, 20000, 1), (2 ** 22, 50000, 1), (2 ** 24, 1 << 30, 1)])
+def test_quantizing_more_rows_than_one_launch_takes(M, K, dtype):
+    refused(f"L.ontovae_quantize_rows(P, {dtype}, {K}, NULL, {M}, {M}, {K}, P, {K}, P, NULL)", "quantize_rows", "too many")
+
+
+@pytest.mark.parametrize("M,N,K", [(2 ** 30, 2 ** 12, 64), (2 ** 20, 2 ** 17, 16), (32, TOP - 1024, 16)])
+def test_int8_products_of_more_than_one_launch(M, N, K):
+    """In tiles of 256 x 256, of 64 x 64 where the rows do not start on 16 bytes (the last two)."""
+    lda = K + 1 if K == 16 else K
+    refused(f"L.ontovae_int8_matmul(P, {lda}, P, P, {lda}, P, NULL, {M}, {N}, {K}, P, 0, {N}, P, 1 << 62, NULL)", "int8_matmul", "too many")
+    refused(f"L.ontovae_int8_linear(P, 0, {K}, NULL, {M}, P, {lda}, P, NULL, {M}, {N}, {K}, P, 0, {N}, P, 1 << 62, NULL)", "int8_linear", "too many")
+
+
+def test_int8_linear_of_more_rows_than_its_quantizer_takes():
+    refused(f"L.ontovae_int8_linear(P, 0, 8, NULL, {2 ** 26}, P, 8, P, NULL, {2 ** 26}, 1, 8, P, 0, 1, P, 1 << 62, NULL)", "int8_linear", "too many")
