@@ -554,7 +554,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
                         }
                         const float d = mb - m[k];
                         m[k] += d * wgt;
-                        m2[k] += s2 + d * d * cross;
+                        m2[k] += s2 + d * (d * cross);         // no rows before: d is the mean itself, its square may pass the type
                     }
                 };
                 if (nb == RB) merge(std::true_type{});
@@ -574,7 +574,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
             for (int k = 0; k < t.ty; ++k) {
                 const float2 v = cs[k * t.tx * E + c];
                 const float d = v.x - a;
-                b += v.y + d * d * (float)ov_gn_thread_rows(t, rows, k);
+                b += v.y + d * (d * (float)ov_gn_thread_rows(t, rows, k));      // a thread row without rows: 0
             }
             st[c] = make_float2(a, b);
         }

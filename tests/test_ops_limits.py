@@ -1,6 +1,6 @@
 """Sizes at the ends of the integer types: the sizing functions and the refusals of the dense-block operators, no GPU needed (a
-refusal comes before any pointer is used).  The calls run in a process of their own, so that one that ends its process fails
-its own test only."""
+refusal comes before any pointer is used).  Where a wrapped size could end the process, the calls run in one of their own."""
+import ctypes as C
 import os
 import subprocess
 import sys
@@ -30,10 +30,10 @@ def test_group_norm_sizing_of_many_groups():
         assert got == [8 * groups, 0, 8 * groups], groups
 
 
-@pytest.mark.parametrize("N,S,C,groups", [(TOP, 1, 8, 8), (1, TOP, 8, 8), (1, 1, TOP, 1), (TOP, TOP, TOP, 1)])
-def test_group_norm_sizing_past_the_sizes_it_takes(N, S, C, groups):
+@pytest.mark.parametrize("N,S,Cn,groups", [(TOP, 1, 8, 8), (1, TOP, 8, 8), (1, 1, TOP, 1), (TOP, TOP, TOP, 1)])
+def test_group_norm_sizing_past_the_sizes_it_takes(N, S, Cn, groups):
     """Sizes that the entry points refuse: no workspace, nothing divided by what wrapped to 0."""
-    assert call(f"L.ontovae_group_norm_act_workspace_bytes(0, {N}, {S}, {C}, {groups}, 1)") == [0]
+    assert call(f"L.ontovae_group_norm_act_workspace_bytes(0, {N}, {S}, {Cn}, {groups}, 1)") == [0]
 
 
 @pytest.mark.parametrize("name", ["int8_matmul", "int8_linear"])
@@ -67,18 +67,21 @@ def test_int8_linear_refuses_more_columns_than_its_indexes_hold(M):
 
 
 def refused(expr, *words):
-    rc, text = call(expr, "err()")
+    from onto_vae_amd import _lib
+    L = _lib.lib()
+    rc = eval(expr, dict(L=L, P=C.c_void_p(1 << 20), NULL=C.c_void_p(0)))
+    text = L.ontovae_last_error().decode()
     assert rc == -1, (rc, text)           # the library's refusal, not the runtime's
     assert all(w in text for w in words), text
 
 
-@pytest.mark.parametrize("R,C,dtype", [(2 ** 29, 64, 0), (2 ** 29, 57, 1), (TOP, 16, 2), (TOP, TOP, 0), (16, TOP - 7, 1), (17, TOP, 1)])
-def test_dropout_of_more_than_one_launch(R, C, dtype):
+@pytest.mark.parametrize("R,Cn,dtype", [(2 ** 29, 64, 0), (2 ** 29, 57, 1), (TOP, 16, 2), (TOP, TOP, 0), (16, TOP - 7, 1), (17, TOP, 1)])
+def test_dropout_of_more_than_one_launch(R, Cn, dtype):
     """One thread per 8 elements, less than 2^32 of them."""
-    refused(f"L.ontovae_dropout(P, {dtype}, {C}, NULL, {R}, {R}, {C}, 0.5, 1, 1, P, NULL)", "dropout", "too many")
+    refused(f"L.ontovae_dropout(P, {dtype}, {Cn}, NULL, {R}, {R}, {Cn}, 0.5, 1, 1, P, NULL)", "dropout", "too many")
 
 
-@pytest.mark.parametrize("N,S,C,groups", [
+@pytest.mark.parametrize("N,S,Cn,groups", [
     (1, 1, 2 ** 29, 2 ** 29),          # one sample of 2^32 threads
     (1, 1, 2 ** 30, 2 ** 30),
     (2 ** 24, 2, 8, 2),                # a workgroup a sample
@@ -86,10 +89,10 @@ def test_dropout_of_more_than_one_launch(R, C, dtype):
     (2 ** 22, 1, 16385, 1),            # the general form: 1024 threads a group
     (2 ** 22, 2, 2049, 1),
     (TOP - 65536, TOP - 65536, 8, 1)])
-def test_group_norm_of_more_than_one_launch(N, S, C, groups):
-    refused(f"L.ontovae_group_norm_act(P, 0, {N}, {S}, {C}, {groups}, P, P, 0, 1e-5, 0, 0.0, 0, 0, P, P, P, P, 1 << 62, NULL)",
+def test_group_norm_of_more_than_one_launch(N, S, Cn, groups):
+    refused(f"L.ontovae_group_norm_act(P, 0, {N}, {S}, {Cn}, {groups}, P, P, 0, 1e-5, 0, 0.0, 0, 0, P, P, P, P, 1 << 62, NULL)",
             "group_norm_act", "too many")
-    refused(f"L.ontovae_group_norm_act_backward(P, P, 0, {N}, {S}, {C}, {groups}, P, P, 0, P, P, 0, 0.0, 0, 0, P, P, P, P, 1 << 62, NULL)",
+    refused(f"L.ontovae_group_norm_act_backward(P, P, 0, {N}, {S}, {Cn}, {groups}, P, P, 0, P, P, 0, 0.0, 0, 0, P, P, P, P, 1 << 62, NULL)",
             "group_norm_act_backward", "too many")
 
 
