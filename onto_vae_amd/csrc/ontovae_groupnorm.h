@@ -4,8 +4,11 @@
 //   v = (x - mu) r gamma_c + beta_c,   y = D act(v),   D = keep / (1 - p) as in ontovae_dropout.h over the rows [N S, C]
 // Backward: dv = dy D act'(v), dgamma_c = sum dv xhat, dbeta_c = sum dv, e = dv gamma,
 //   dx = r (e - mean(e) - xhat mean(e xhat)), the means over the group.
-// Statistics and every sum are held in 32 bits; the variance is the second moment about the mean (two passes over what is held
-// or cached), so a large mean costs no digits.
+// Statistics and every sum are held in 32 bits, and a large mean costs no digits: a float32 mean alone would be off by half a step of
+// its own magnitude, a shift common to the whole group (1e-3 of the spread at a mean of 1e4 spreads).  Every form takes the sum of
+// x - mean about a mean it has, and with it the REST that the float32 mean leaves; x - mean - rest is what is normalised.  The
+// variance is the second moment about the mean (two passes over what is held or cached).  The saved mean is the nearest float32;
+// the backward pass finds the rest again from x, where it counts (ov_gn_far).
 #ifndef ONTOVAE_GROUPNORM_H
 #define ONTOVAE_GROUPNORM_H
 
@@ -191,6 +194,36 @@ __device__ __forceinline__ float ov_gn_sum(float v, float* red) {
     return v;
 }
 
+// the same for two values
+template <int LPG>
+__device__ __forceinline__ float2 ov_gn_sum2(float a, float b, float* red) {
+    if (LPG <= 64) return make_float2(ov_gn_sum<LPG>(a, red), ov_gn_sum<LPG>(b, red));
+    a = ov_wave_sum(a);
+    b = ov_wave_sum(b);
+    __syncthreads();
+    if (ov_lane() == 0) { red[threadIdx.x >> 6] = a; red[16 + (threadIdx.x >> 6)] = b; }
+    __syncthreads();
+    a = b = 0.f;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) { a += red[w]; b += red[16 + w]; }
+    return make_float2(a, b);
+}
+
+// Whether the backward pass looks for the rest of a group: the saved mean is off by at most 2^-24 |mean|, xhat by that times rstd.
+// Up to 4 spreads that is less than what the rounding of x - mean itself does to the group's outer values.
+__device__ __forceinline__ bool ov_gn_far(float mean, float rstd) { return fabsf(mean) * rstd > 4.f; }
+
+// a + b as the nearest float32 and what that leaves
+__device__ __forceinline__ float ov_gn_two(float a, float b, float* rest) {
+    const float s = a + b, t = s - a;
+    *rest = (a - (s - t)) + (b - t);
+    return s;
+}
+// a variance from a second moment about a mean that is off by `rest` (NaN stays)
+__device__ __forceinline__ float ov_gn_var(float m2, float rest) {
+    const float v = m2 - rest * rest;
+    return v < 0.f ? 0.f : v;
+}
+
 // ---------------------------------------------------------------- S = 1: a group is one contiguous run of cg elements
 // LPG threads hold a group in registers, NV pieces of 8 elements each; a slot of LPG threads keeps its group and walks the
 // samples rs, rs + RS, ...: weight and bias (and the sums of their gradients) stay in registers.  Neighbouring slots take
@@ -201,7 +234,7 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(co
                                                                              float* __restrict__ mean, float* __restrict__ rstd) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvGnPiece<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
-    __shared__ float red[16];
+    __shared__ float red[32];
     const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
     const int j = threadIdx.x % LPG, rs = (int)(slot / p.groups), g = (int)(slot - (int64_t)rs * p.groups);
     if (rs >= RS) return;
@@ -246,26 +279,29 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_fwd_kernel(co
         }
         const float mu = ov_gn_sum<LPG>(s, red) / len;
         s = 0.f;
+        float left = 0.f;
 #pragma unroll
         for (int i = 0; i < NV; ++i)
 #pragma unroll
             for (int k = 0; k < E; ++k) {
                 v[i][k] = k < cnt[i] ? v[i][k] - mu : 0.f;
                 s += v[i][k] * v[i][k];
+                left += v[i][k];
             }
-        const float r = 1.f / sqrtf(ov_gn_sum<LPG>(s, red) / len + p.eps);
+        const float2 sl = ov_gn_sum2<LPG>(s, left, red);
+        const float rest = sl.y / len, r = 1.f / sqrtf(ov_gn_var(sl.x / len, rest) + p.eps);
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (cnt[i] <= 0) continue;
             const int o = (j + i * LPG) * E;
 #pragma unroll
-            for (int k = 0; k < E; ++k) v[i][k] = v[i][k] * r * w[i][k] + b[i][k];
+            for (int k = 0; k < E; ++k) v[i][k] = (v[i][k] - rest) * r * w[i][k] + b[i][k];
             ov_act<E>(v[i], p.act);
             ov_gn_drop<E>(p, n, (int)gc + o, v[i]);
             ov_gn_store<T>(y + here + o, cnt[i], v[i]);
         }
         if (j == 0) {
-            mean[(int64_t)n * p.groups + g] = mu;
+            mean[(int64_t)n * p.groups + g] = mu + rest;
             rstd[(int64_t)n * p.groups + g] = r;
         }
     }
@@ -279,7 +315,7 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
                                                                              T* __restrict__ dx, float* __restrict__ part) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvGnPiece<T>::N, BLOCK = LPG < 256 ? 256 : LPG;
-    __shared__ float red[16];
+    __shared__ float red[32];
     __shared__ float sums[LPG < 256 ? 256 * 8 : 8];
     const int64_t slot = ((int64_t)blockIdx.x * BLOCK + threadIdx.x) / LPG;
     const int j = threadIdx.x % LPG, rs = (int)(slot / p.groups), g = (int)(slot - (int64_t)rs * p.groups);
@@ -327,13 +363,27 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
             mu = mean[(int64_t)(n + RS) * p.groups + g];
             r = rstd[(int64_t)(n + RS) * p.groups + g];
         }
-        float s1 = 0.f, s2 = 0.f;
+        float s1 = 0.f, s2 = 0.f, rest = 0.f;
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+#pragma unroll
+            for (int k = 0; k < E; ++k) {
+                v[i][k] -= mu0;
+                if (k >= cnt[i]) v[i][k] = 0.f;
+            }
+        if (ov_gn_far(mu0, r0)) {                        // the same in every thread of the group
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+#pragma unroll
+                for (int k = 0; k < E; ++k) rest += v[i][k];
+            rest = ov_gn_sum<LPG>(rest, red) / len;
+        }
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             float a[E];
 #pragma unroll
             for (int k = 0; k < E; ++k) {
-                v[i][k] = (v[i][k] - mu0) * r0;
+                v[i][k] = (v[i][k] - rest) * r0;
                 a[k] = v[i][k] * w[i][k] + b[i][k];
             }
             ov_gn_dv<E>(p, n, (int)gc + (j + i * LPG) * E, d[i], a);
@@ -347,8 +397,9 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
                 s2 += d[i][k] * v[i][k];
             }
         }
-        s1 = ov_gn_sum<LPG>(s1, red) / len;
-        s2 = ov_gn_sum<LPG>(s2, red) / len;
+        const float2 sg = ov_gn_sum2<LPG>(s1, s2, red);
+        s1 = sg.x / len;
+        s2 = sg.y / len;
 #pragma unroll
         for (int i = 0; i < NV; ++i) {
             if (cnt[i] <= 0) continue;
@@ -434,7 +485,8 @@ struct OvGnTile {
     int gb, nblk;            // groups of a channel block, channel blocks
     int tx, ty;              // pieces of a block's row, rows at a time
     int chunks, rows;        // tiles along S, rows of one
-    float* part;             // per tile and group: 2 floats, [N][chunks][groups][2]
+    float* part;             // per tile and group, [N][chunks][groups].  Forward: float4 (mean, rest, M2, -).  Backward: float2 sums
+    float* far;              // backward: sums of x - mean, the same order
 };
 
 struct OvGnPlace { int n, chunk, c0, cb, g0, ng, r0, r1; };
@@ -465,34 +517,88 @@ __device__ __forceinline__ int ov_gn_lanes(int ng, int n) {
     return lg;
 }
 
-// count-weighted combination of the chunks' (first, second) over a group; lanes of the workgroup share the groups out.
-// FWD: (mean, M2) by Chan's formula about the overall mean -> (mu, r).  Else: plain sums / count.
-template <bool FWD>
-__device__ __forceinline__ void ov_gn_gather(const OvGn& p, const OvGnTile& t, const OvGnPlace& q, float2* st) {
-    const int lg = ov_gn_lanes(q.ng, t.chunks);
+__device__ __forceinline__ float ov_gn_lanes_sum(float v, int lg) {
+    for (int o = lg / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+
+// Joins n parts of a group, part k = (mean, rest, M2) of cnt(k) values, by Chan's formula; lanes l of lg share them out.  The parts'
+// means are taken relative to the first one's, where nothing of the rests is lost.  (Relative to the first VALUE it would be: a value
+// that stands alone is sqrt(n) spreads away, the mean of a part that holds it no more than 45 for any tile.)
+template <typename P, typename CNT>
+__device__ __forceinline__ float3 ov_gn_join(int n, int l, int lg, float total, P&& part, CNT&& cnt) {
+    const float3 first = part(0);
+    const float m = first.x + first.y;
+    float a = 0.f, m2 = 0.f;
+    for (int k = l; k < n; k += lg) {
+        const float3 v = part(k);
+        a += ((v.x - m) + v.y) * cnt(k);
+    }
+    a = ov_gn_lanes_sum(a, lg) / total;
+    for (int k = l; k < n; k += lg) {
+        const float3 v = part(k);
+        const float d = ((v.x - m) + v.y) - a;
+        m2 += v.z + d * (d * cnt(k));                    // a part of no values: d may be anything
+    }
+    float3 o;
+    o.z = ov_gn_lanes_sum(m2, lg);
+    o.x = ov_gn_two(m, a, &o.y);
+    return o;
+}
+
+// a sample's statistics from its tiles' -> gs = (mean, rstd), rest.  Up to 8 tiles a lane are read at once, so that their latency
+// counts once.
+__device__ __forceinline__ void ov_gn_gather_fwd(const OvGn& p, const OvGnTile& t, const OvGnPlace& q, float2* gs, float* rest) {
+    constexpr int NP = 8;
+    const int lg = ov_gn_lanes(q.ng, t.chunks), l = threadIdx.x % lg;
+    const float total = (float)((int64_t)p.S * p.cg);
+    auto count = [&](int k) { return (float)ov_gn_tile_rows(p, t, k) * (float)p.cg; };
     for (int g = threadIdx.x / lg; g < q.ng; g += 256 / lg) {
-        const int l = threadIdx.x % lg;
+        const float4* src = reinterpret_cast<const float4*>(t.part) + ((int64_t)q.n * t.chunks * p.groups + q.g0 + g);
+        float3 o;
+        if (t.chunks <= NP * lg) {                       // ov_gn_join on registers
+            float4 v[NP];
+#pragma unroll
+            for (int i = 0; i < NP; ++i) v[i] = src[(int64_t)min(l + i * lg, t.chunks - 1) * p.groups];
+            const float m = __shfl(v[0].x + v[0].y, ov_lane() - l, 64);
+            float a = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                v[i].w = l + i * lg < t.chunks ? count(l + i * lg) : 0.f;
+                v[i].x = (v[i].x - m) + v[i].y;
+                a += v[i].x * v[i].w;
+            }
+            a = ov_gn_lanes_sum(a, lg) / total;
+#pragma unroll
+            for (int i = 0; i < NP; ++i) {
+                const float d = v[i].x - a;
+                if (l + i * lg < t.chunks) m2 += v[i].z + d * (d * v[i].w);
+            }
+            o.z = ov_gn_lanes_sum(m2, lg);
+            o.x = ov_gn_two(m, a, &o.y);
+        } else {
+            o = ov_gn_join(t.chunks, l, lg, total, [&](int k) { const float4 v = src[(int64_t)k * p.groups]; return make_float3(v.x, v.y, v.z); }, count);
+        }
+        if (l == 0) { gs[g] = make_float2(o.x, 1.f / sqrtf(o.z / total + p.eps)); rest[g] = o.y; }
+    }
+    __syncthreads();
+}
+
+// backward: the tiles' sums of (dv gamma, dv gamma xhat) / count -> gs
+__device__ __forceinline__ void ov_gn_gather_bwd(const OvGn& p, const OvGnTile& t, const OvGnPlace& q, float2* gs) {
+    const int lg = ov_gn_lanes(q.ng, t.chunks), l = threadIdx.x % lg;
+    const float total = (float)((int64_t)p.S * p.cg);
+    for (int g = threadIdx.x / lg; g < q.ng; g += 256 / lg) {
         const float2* src = reinterpret_cast<const float2*>(t.part) + ((int64_t)q.n * t.chunks * p.groups + q.g0 + g);
         float a = 0.f, b = 0.f;
         for (int k = l; k < t.chunks; k += lg) {
             const float2 v = src[(int64_t)k * p.groups];
-            a += FWD ? v.x * ((float)ov_gn_tile_rows(p, t, k) * (float)p.cg) : v.x;
+            a += v.x;
             b += v.y;
         }
-        for (int o = lg / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); b += __shfl_xor(b, o, 64); }
-        const float total = (float)((int64_t)p.S * p.cg);
-        if (FWD) {
-            const float mu = a / total;
-            float d2 = 0.f;
-            for (int k = l; k < t.chunks; k += lg) {
-                const float d = src[(int64_t)k * p.groups].x - mu;
-                d2 += d * d * ((float)ov_gn_tile_rows(p, t, k) * (float)p.cg);
-            }
-            for (int o = lg / 2; o > 0; o >>= 1) d2 += __shfl_xor(d2, o, 64);
-            if (l == 0) st[g] = make_float2(mu, 1.f / sqrtf((b + d2) / total + p.eps));
-        } else if (l == 0) {
-            st[g] = make_float2(a / total, b / total);
-        }
+        a = ov_gn_lanes_sum(a, lg);
+        b = ov_gn_lanes_sum(b, lg);
+        if (l == 0) gs[g] = make_float2(a / total, b / total);
     }
     __syncthreads();
 }
@@ -504,52 +610,59 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
                                                              float* __restrict__ mean, float* __restrict__ rstd) {
     const OvGn p = ov_gn_light<LIGHT>(p_);
     constexpr int E = OvGnPiece<T>::N, RB = 16 / (int)sizeof(T);
-    __shared__ float2 cs[OV_GN_MAX_CB(E)];               // (mean, M2) of a thread's rows of a channel
-    __shared__ float2 st[OV_GN_MAX_CB(E)];               // per group: (mean, M2), then (mu, r)
+    __shared__ float2 cs[OV_GN_MAX_CB(E)];               // (rest, M2) of a thread's rows of a channel, of a channel; then (mu, r) of a group
+    __shared__ float ks[OV_GN_MAX_CB(E)];                // the mean that belongs to it; then the group's rest
     const OvGnPlace q = ov_gn_place(p, t, MODE == 1);
     const int tid = threadIdx.x, ty = tid / t.tx, tx = tid - ty * t.tx;
     const bool on = ty < t.ty;
     const int cnt = on ? min(q.cb - tx * E, E) : 0;      // <= 0: no channel of the block
-    const int64_t row0 = (int64_t)q.n * p.S, col = q.c0 + tx * E, total = (int64_t)p.N * p.S * p.C;
+    const int64_t row0 = (int64_t)q.n * p.S, col = q.c0 + tx * E, all = (int64_t)p.N * p.S * p.C;
     constexpr int RA = 8;
     OvGnPiece<T> raw[RA];
     auto fetch = [&](int r) {
 #pragma unroll
-        for (int i = 0; i < RA; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, raw[i]);
+        for (int i = 0; i < RA; ++i) ov_gn_raw<T>(x, all, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, raw[i]);
     };
     if (MODE != 1) {
-        float m[E], m2[E];
+        // sums relative to the first value that the thread meets of a channel
+        float k0[E], m[E], m2[E];
 #pragma unroll
-        for (int k = 0; k < E; ++k) m[k] = m2[k] = 0.f;
+        for (int k = 0; k < E; ++k) k0[k] = m[k] = m2[k] = 0.f;
         int have = 0;
         if (cnt > 0)
             for (int r = q.r0 + ty; r < q.r1; r += RB * t.ty) {
                 OvGnPiece<T> v[RB];
                 const int nb = min(ov_gn_thread_rows(t, q.r1 - r, 0), RB);
 #pragma unroll
-                for (int i = 0; i < RB; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, v[i]);
-                if ((row0 + min(r + (RB - 1) * t.ty, q.r1 - 1)) * p.C + col > total - E) {      // the tensor's last pieces
+                for (int i = 0; i < RB; ++i) ov_gn_raw<T>(x, all, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, v[i]);
+                if ((row0 + min(r + (RB - 1) * t.ty, q.r1 - 1)) * p.C + col > all - E) {      // the tensor's last pieces
 #pragma unroll
                     for (int i = 0; i < RB; ++i) {
                         const int64_t o = (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col;
                         float f[E];
-                        ov_gn_floats<T>(x, total, o, v[i], f);
+                        ov_gn_floats<T>(x, all, o, v[i], f);
 #pragma unroll
                         for (int k = 0; k < E; ++k) v[i].e[k] = ov_from_f<T>(f[k]);
                     }
                 }
+                if (have == 0)
+#pragma unroll
+                    for (int k = 0; k < E; ++k) k0[k] = ov_to_f<T>(v[0].e[k]);
                 // mean and second moment of these rows, then Chan's combination with the ones before
                 const float fb = (float)nb, ft = (float)(have + nb), wgt = fb / ft, cross = (float)have * wgt, rb = 1.f / fb;
                 auto merge = [&](auto whole) {
 #pragma unroll
                     for (int k = 0; k < E; ++k) {
-                        float s = 0.f, s2 = 0.f;
+                        float s = 0.f, s2 = 0.f, u[RB];
 #pragma unroll
-                        for (int i = 0; i < RB; ++i) s += whole || i < nb ? ov_to_f<T>(v[i].e[k]) : 0.f;
+                        for (int i = 0; i < RB; ++i) {
+                            u[i] = ov_to_f<T>(v[i].e[k]) - k0[k];
+                            s += whole || i < nb ? u[i] : 0.f;
+                        }
                         const float mb = s * rb;
 #pragma unroll
                         for (int i = 0; i < RB; ++i) {
-                            const float d = ov_to_f<T>(v[i].e[k]) - mb;
+                            const float d = u[i] - mb;
                             s2 += whole || i < nb ? d * d : 0.f;
                         }
                         const float d = mb - m[k];
@@ -563,43 +676,49 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
             }
         if (on)
 #pragma unroll
-            for (int k = 0; k < E; ++k) cs[ty * t.tx * E + tx * E + k] = make_float2(m[k], m2[k]);
-        __syncthreads();
-        // a channel's mean and M2 over the ty's (their row counts follow from ty), into the place of ty = 0
-        const int rows = q.r1 - q.r0;
-        for (int c = tid; c < q.cb; c += 256) {
-            float a = 0.f, b = 0.f;
-            for (int k = 0; k < t.ty; ++k) a += cs[k * t.tx * E + c].x * (float)ov_gn_thread_rows(t, rows, k);
-            a /= (float)rows;
-            for (int k = 0; k < t.ty; ++k) {
-                const float2 v = cs[k * t.tx * E + c];
-                const float d = v.x - a;
-                b += v.y + d * (d * (float)ov_gn_thread_rows(t, rows, k));      // a thread row without rows: 0
+            for (int k = 0; k < E; ++k) {
+                const int at = ty * t.tx * E + tx * E + k;
+                cs[at] = make_float2(m[k], m2[k]);
+                ks[at] = k0[k];
             }
-            st[c] = make_float2(a, b);
+        __syncthreads();
+        // a channel's over the ty's (their row counts follow from ty), into the place of ty = 0: the lanes that read a column write it
+        const int rows = q.r1 - q.r0, lc = ov_gn_lanes(q.cb, t.ty);
+        for (int c = tid / lc; c < q.cb; c += 256 / lc) {
+            const float3 o = ov_gn_join(t.ty, tid % lc, lc, (float)rows,
+                                        [&](int k) { const int at = k * t.tx * E + c; return make_float3(ks[at], cs[at].x, cs[at].y); },
+                                        [&](int k) { return (float)ov_gn_thread_rows(t, rows, k); });
+            if (tid % lc == 0) {
+                ks[c] = o.x;
+                cs[c] = make_float2(o.y, o.z);
+            }
         }
         __syncthreads();
+        // a group's over its channels, into the place of channel g, whose own group has been read in this round or before
         const int lg = ov_gn_lanes(q.ng, p.cg), l = tid % lg;
-        for (int g = tid / lg; g < q.ng; g += 256 / lg) {
-            float a = 0.f, b = 0.f;
-            for (int k = l; k < p.cg; k += lg) a += st[g * p.cg + k].x;
-            for (int o = lg / 2; o > 0; o >>= 1) a += __shfl_xor(a, o, 64);
-            a /= (float)p.cg;
-            for (int k = l; k < p.cg; k += lg) {
-                const float2 v = st[g * p.cg + k];
-                const float d = v.x - a;
-                b += v.y + d * d * (float)rows;
+        const float total = (float)((int64_t)rows * p.cg);
+        for (int g0 = 0; g0 < q.ng; g0 += 256 / lg) {
+            const int g = g0 + tid / lg;
+            float3 o = make_float3(0.f, 0.f, 0.f);
+            if (g < q.ng)
+                o = ov_gn_join(p.cg, l, lg, total, [&](int k) { const int c = g * p.cg + k; return make_float3(ks[c], cs[c].x, cs[c].y); },
+                               [&](int) { return (float)rows; });
+            if (MODE == 0) {
+                if (g < q.ng && l == 0)
+                    reinterpret_cast<float4*>(t.part)[((int64_t)q.n * t.chunks + q.chunk) * p.groups + q.g0 + g] = make_float4(o.x, o.y, o.z, 0.f);
+            } else {
+                __syncthreads();
+                if (g < q.ng && l == 0) {
+                    cs[g] = make_float2(o.x, 1.f / sqrtf(o.z / total + p.eps));
+                    ks[g] = o.y;
+                }
             }
-            for (int o = lg / 2; o > 0; o >>= 1) b += __shfl_xor(b, o, 64);
-            if (l != 0) continue;
-            if (MODE == 0) reinterpret_cast<float2*>(t.part)[((int64_t)q.n * t.chunks + q.chunk) * p.groups + q.g0 + g] = make_float2(a, b);
-            else cs[g] = make_float2(a, 1.f / sqrtf(b / (float)((int64_t)rows * p.cg) + p.eps));
         }
         if (MODE == 0) return;
         __syncthreads();
     } else {
         if (cnt > 0) fetch(q.r0 + ty);                    // under the gather's latency
-        ov_gn_gather<true>(p, t, q, cs);
+        ov_gn_gather_fwd(p, t, q, cs, ks);
     }
     if (q.chunk == 0)
         for (int g = tid; g < q.ng; g += 256) {
@@ -613,9 +732,11 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
     ov_gn_params<E>(p.b, p.wtype, q.c0 + tx * E, cnt, 0.f, b);
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-        const float2 v = cs[min(tx * E + k, q.cb - 1) / p.cg];
+        const int g = min(tx * E + k, q.cb - 1) / p.cg;
+        const float2 v = cs[g];
         mu[k] = v.x;
         rw[k] *= v.y;
+        b[k] -= ks[g] * rw[k];                            // (x - mu - rest) rw + b
     }
     for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
         if (r > q.r0 + ty) fetch(r);
@@ -624,7 +745,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
             const int rr = r + i * t.ty;
             if (rr >= q.r1) break;
             float v[E];
-            ov_gn_floats<T>(x, total, (row0 + rr) * p.C + col, raw[i], v);
+            ov_gn_floats<T>(x, all, (row0 + rr) * p.C + col, raw[i], v);
 #pragma unroll
             for (int k = 0; k < E; ++k) v[k] = (v[k] - mu[k]) * rw[k] + b[k];
             ov_act<E>(v, p.act);
@@ -634,7 +755,11 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
     }
 }
 
-// chan: [2][N chunks][C]: the tiles' sums of dv xhat, then of dv, per channel
+// chan: [2][N chunks][C]: the tiles' sums of dv xhat, then of dv, per channel.
+// Rests (ov_gn_far), of float32 x: MODE 3, in front of the others, takes the sums of x - mean of the tiles that hold such a group and ends at
+// once where there is none (2.5 us, 4 x 1024 x 320 27 -> 29.5).  A rest enters v through beta, the sums and dx after their loops: those are
+// the same with and without it.  A 16-bit x goes without (64 x 16 x 320 in bf16 would be 18 -> 21 us): the rounding of its values, 2^-12 |x| at
+// least, has moved the mean of n of them by 2^-12 |mean| / sqrt(n), more than the 2^-24 |mean| in question up to n = 2^24.
 template <typename T, int MODE, bool LIGHT>
 __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p_, const OvGnTile t,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
@@ -659,15 +784,81 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
             ov_gn_raw<T>(dy, total, o, rd[i]);
         }
     };
+    auto group = [&](int k) { return min(tx * E + k, q.cb - 1) / p.cg; };
+    if (MODE == 3) {
+        bool any = false;
+        for (int g = ov_lane(); g < q.ng; g += 64) any |= ov_gn_far(mean[(int64_t)q.n * p.groups + q.g0 + g], rstd[(int64_t)q.n * p.groups + q.g0 + g]);
+        if (!__any(any)) return;                         // the same in every wave of the workgroup
+    }
+    bool far = false;                                    // one of the thread's groups
     if (cnt > 0) {
         ov_gn_params<E>(p.w, p.wtype, q.c0 + tx * E, cnt, 1.f, rw);
         ov_gn_params<E>(p.b, p.wtype, q.c0 + tx * E, cnt, 0.f, b);
 #pragma unroll
         for (int k = 0; k < E; ++k) {
-            const int64_t gi = (int64_t)q.n * p.groups + q.g0 + min(tx * E + k, q.cb - 1) / p.cg;
+            const int64_t gi = (int64_t)q.n * p.groups + q.g0 + group(k);
             mu[k] = mean[gi];
             rw[k] *= rstd[gi];
+            far |= sizeof(T) == 4 && ov_gn_far(mu[k], rstd[gi]);
         }
+    }
+    if (MODE == 3) {
+        float d[E];
+#pragma unroll
+        for (int k = 0; k < E; ++k) d[k] = 0.f;
+        if (cnt > 0)
+            for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
+#pragma unroll
+                for (int i = 0; i < RA; ++i) ov_gn_raw<T>(x, total, (row0 + min(r + i * t.ty, q.r1 - 1)) * p.C + col, rx[i]);
+#pragma unroll
+                for (int i = 0; i < RA; ++i) {
+                    if (r + i * t.ty >= q.r1) break;
+                    float f[E];
+                    ov_gn_floats<T>(x, total, (row0 + r + i * t.ty) * p.C + col, rx[i], f);
+#pragma unroll
+                    for (int k = 0; k < E; ++k) d[k] += f[k] - mu[k];
+                }
+            }
+        if (on)
+#pragma unroll
+            for (int k = 0; k < E; ++k) cs[ty * t.tx * E + tx * E + k].x = d[k];
+        __syncthreads();
+        for (int c = tid; c < q.cb; c += 256) {
+            float a = 0.f;
+            for (int k = 0; k < t.ty; ++k) a += cs[k * t.tx * E + c].x;
+            st[c].x = a;
+        }
+        __syncthreads();
+        const int lg = ov_gn_lanes(q.ng, p.cg), l = tid % lg;
+        for (int g = tid / lg; g < q.ng; g += 256 / lg) {
+            float a = 0.f;
+            for (int k = l; k < p.cg; k += lg) a += st[g * p.cg + k].x;
+            a = ov_gn_lanes_sum(a, lg);
+            if (l == 0) t.far[((int64_t)q.n * t.chunks + q.chunk) * p.groups + q.g0 + g] = a;
+        }
+        return;
+    }
+    // the rests of the thread's channels; mode 3 has written the sums of every such group
+    auto rests = [&](float (&d)[E]) {
+#pragma unroll
+        for (int k = 0; k < E; ++k) {
+            d[k] = k > 0 ? d[max(k - 1, 0)] : 0.f;
+            if (k > 0 && group(k) == group(k - 1)) continue;
+            const int64_t gi = (int64_t)q.n * p.groups + q.g0 + group(k);
+            float a = 0.f;
+            if (ov_gn_far(mean[gi], rstd[gi])) {
+                const float* src = t.far + ((int64_t)q.n * t.chunks * p.groups + q.g0 + group(k));
+#pragma unroll 8
+                for (int i = 0; i < t.chunks; ++i) a += src[(int64_t)i * p.groups];
+            }
+            d[k] = a / (float)((int64_t)p.S * p.cg);
+        }
+    };
+    if (far) {
+        float d[E];
+        rests(d);
+#pragma unroll
+        for (int k = 0; k < E; ++k) b[k] -= d[k] * rw[k];
     }
     auto grad = [&](int64_t row, const OvGnPiece<T>& vx, const OvGnPiece<T>& vd, float (&xm)[E], float (&dv)[E]) {
         float d[E];
@@ -699,8 +890,14 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
                     }
                 }
             }
+            if (far) {
+                float d[E];
+                rests(d);
 #pragma unroll
-            for (int k = 0; k < E; ++k) sw[k] *= rstd[(int64_t)q.n * p.groups + q.g0 + min(tx * E + k, q.cb - 1) / p.cg];
+                for (int k = 0; k < E; ++k) sw[k] -= d[k] * sb[k];
+            }
+#pragma unroll
+            for (int k = 0; k < E; ++k) sw[k] *= rstd[(int64_t)q.n * p.groups + q.g0 + group(k)];
         }
         if (on)
 #pragma unroll
@@ -730,7 +927,8 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
                 a += v.x;
                 e += v.y;
             }
-            for (int o = lg / 2; o > 0; o >>= 1) { a += __shfl_xor(a, o, 64); e += __shfl_xor(e, o, 64); }
+            a = ov_gn_lanes_sum(a, lg);
+            e = ov_gn_lanes_sum(e, lg);
             if (l != 0) continue;
             if (MODE == 0) reinterpret_cast<float2*>(t.part)[ro * p.groups + q.g0 + g] = make_float2(a, e);
             else {
@@ -741,17 +939,23 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
         if (MODE == 0) return;
         __syncthreads();
     } else {
-        ov_gn_gather<false>(p, t, q, cs);
+        ov_gn_gather_bwd(p, t, q, cs);
     }
     if (cnt <= 0) return;
-    // dx = r (dv gamma - s1 - xhat s2) = dv (r gamma) - r s1 - (x - mu) r^2 s2
+    // dx = r (dv gamma - s1 - xhat s2) = dv (r gamma) - r s1 - (x - mu - rest) r^2 s2
     float k1[E], k2[E];
 #pragma unroll
     for (int k = 0; k < E; ++k) {
-        const float2 v = cs[min(tx * E + k, q.cb - 1) / p.cg];
-        const float rs = rstd[(int64_t)q.n * p.groups + q.g0 + min(tx * E + k, q.cb - 1) / p.cg];
+        const float2 v = cs[group(k)];
+        const float rs = rstd[(int64_t)q.n * p.groups + q.g0 + group(k)];
         k1[k] = rs * v.x;
         k2[k] = rs * rs * v.y;
+    }
+    if (far) {
+        float d[E];
+        rests(d);
+#pragma unroll
+        for (int k = 0; k < E; ++k) k1[k] -= d[k] * k2[k];
     }
     for (int r = q.r0 + ty; r < q.r1; r += RA * t.ty) {
         fetch(r);
@@ -773,7 +977,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
 template <typename T>
 __global__ __launch_bounds__(1024) void ov_gn_any_fwd_kernel(const T* __restrict__ x, const OvGn p, T* __restrict__ y, float* __restrict__ mean,
                                                              float* __restrict__ rstd) {
-    __shared__ float red[16];
+    __shared__ float red[32];
     const int64_t n = blockIdx.x / p.groups;
     const int g = blockIdx.x % p.groups;
     const float cnt = (float)((int64_t)p.S * p.cg);
@@ -783,53 +987,66 @@ __global__ __launch_bounds__(1024) void ov_gn_any_fwd_kernel(const T* __restrict
         for (int c = threadIdx.x; c < p.cg; c += 1024) s += ov_to_f<T>(x[base + (int64_t)r * p.C + c]);
     const float mu = ov_block_sum(s, red) / cnt;
     s = 0.f;
+    float left = 0.f;
     for (int r = 0; r < p.S; ++r)
         for (int c = threadIdx.x; c < p.cg; c += 1024) {
             const float d = ov_to_f<T>(x[base + (int64_t)r * p.C + c]) - mu;
             s += d * d;
+            left += d;
         }
-    const float rs = 1.f / sqrtf(ov_block_sum(s, red) / cnt + p.eps);
+    const float2 sl = ov_gn_sum2<1024>(s, left, red);
+    const float rest = sl.y / cnt, rs = 1.f / sqrtf(ov_gn_var(sl.x / cnt, rest) + p.eps);
     for (int r = 0; r < p.S; ++r)
         for (int c = threadIdx.x; c < p.cg; c += 1024) {
             const int64_t o = base + (int64_t)r * p.C + c;
             const int ch = g * p.cg + c;
-            float v[1] = {(ov_to_f<T>(x[o]) - mu) * rs * ov_gn_param(p.w, p.wtype, ch, 1.f) + ov_gn_param(p.b, p.wtype, ch, 0.f)};
+            float v[1] = {((ov_to_f<T>(x[o]) - mu) - rest) * rs * ov_gn_param(p.w, p.wtype, ch, 1.f) + ov_gn_param(p.b, p.wtype, ch, 0.f)};
             ov_act<1>(v, p.act);
             ov_gn_drop<1>(p, n * p.S + r, ch, v);
             y[o] = ov_from_f<T>(v[0]);
         }
-    if (threadIdx.x == 0) { mean[blockIdx.x] = mu; rstd[blockIdx.x] = rs; }
+    if (threadIdx.x == 0) { mean[blockIdx.x] = mu + rest; rstd[blockIdx.x] = rs; }
 }
 
 template <typename T>
-__device__ __forceinline__ float ov_gn_any_dv(const OvGn& p, const T* x, const T* dy, int64_t row, int c, float mu, float r, float* xhat) {
+__device__ __forceinline__ float ov_gn_any_dv(const OvGn& p, const T* x, const T* dy, int64_t row, int c, float mu, float rest, float r, float* xhat) {
     const int64_t o = row * p.C + c;
-    *xhat = (ov_to_f<T>(x[o]) - mu) * r;
+    *xhat = ((ov_to_f<T>(x[o]) - mu) - rest) * r;
     float d[1] = {ov_to_f<T>(dy[o])}, a[1] = {*xhat * ov_gn_param(p.w, p.wtype, c, 1.f) + ov_gn_param(p.b, p.wtype, c, 0.f)};
     ov_gn_dv<1>(p, row, c, d, a);
     return a[0];
 }
 
+// rests [N][groups]: what the parameters' kernel below takes off as well
 template <typename T>
 __global__ __launch_bounds__(1024) void ov_gn_any_dx_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p,
-                                                            const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx) {
-    __shared__ float red[16];
+                                                            const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
+                                                            float* __restrict__ rests) {
+    __shared__ float red[32];
     const int64_t n = blockIdx.x / p.groups;
     const int g = blockIdx.x % p.groups;
     const float cnt = (float)((int64_t)p.S * p.cg);
     const float mu = mean[blockIdx.x], rs = rstd[blockIdx.x];
+    float rest = 0.f;
+    if (ov_gn_far(mu, rs)) {
+        for (int r = 0; r < p.S; ++r)
+            for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) rest += ov_to_f<T>(x[(n * p.S + r) * p.C + c]) - mu;
+        rest = ov_block_sum(rest, red) / cnt;
+    }
+    if (threadIdx.x == 0) rests[blockIdx.x] = rest;
     float s1 = 0.f, s2 = 0.f, xh;
     for (int r = 0; r < p.S; ++r)
         for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) {
-            const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
+            const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rest, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
             s1 += e;
             s2 += e * xh;
         }
-    s1 = ov_block_sum(s1, red) / cnt;
-    s2 = ov_block_sum(s2, red) / cnt;
+    const float2 sg = ov_gn_sum2<1024>(s1, s2, red);
+    s1 = sg.x / cnt;
+    s2 = sg.y / cnt;
     for (int r = 0; r < p.S; ++r)
         for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) {
-            const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
+            const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rest, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
             dx[(n * p.S + r) * p.C + c] = ov_from_f<T>(rs * (e - s1 - xh * s2));
         }
 }
@@ -838,7 +1055,7 @@ __global__ __launch_bounds__(1024) void ov_gn_any_dx_kernel(const T* __restrict_
 template <typename T>
 __global__ __launch_bounds__(1024) void ov_gn_any_param_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p,
                                                                const float* __restrict__ mean, const float* __restrict__ rstd,
-                                                               float* __restrict__ dw, float* __restrict__ db) {
+                                                               const float* __restrict__ rests, float* __restrict__ dw, float* __restrict__ db) {
     __shared__ float2 red[16][64];
     const int lane = ov_lane(), wave = ov_wave_id(), c = blockIdx.x * 64 + lane;
     float2 s = {0.f, 0.f};
@@ -846,7 +1063,7 @@ __global__ __launch_bounds__(1024) void ov_gn_any_param_kernel(const T* __restri
         for (int64_t row = wave; row < (int64_t)p.N * p.S; row += 16) {
             const int64_t k = row / p.S * p.groups + c / p.cg;
             float xh;
-            const float dv = ov_gn_any_dv(p, x, dy, row, c, mean[k], rstd[k], &xh);
+            const float dv = ov_gn_any_dv(p, x, dy, row, c, mean[k], rests[k], rstd[k], &xh);
             s.x += dv * xh;
             s.y += dv;
         }
@@ -885,8 +1102,9 @@ struct OvGnPlan {
     int form;
     int lpg, nv, RS, wgs;    // OV_GN_ROW
     OvGnTile t;              // OV_GN_TILE (two launches), OV_GN_TILE1 (one)
-    int64_t part_floats, chan_floats, chan_rows;
+    int64_t part_floats, far_floats, chan_floats, chan_rows;
 };
+static int64_t ov_gn_up(int64_t floats) { return (floats + 63) / 64 * 64; }
 
 static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool backward) {
     OvGnPlan q{};
@@ -894,6 +1112,7 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
     const int pieces = (cg + E - 1) / E;
     if ((int64_t)N * S * C < E) {                         // not one piece
         q.form = OV_GN_ANY;
+        q.far_floats = backward ? (int64_t)N * groups : 0;
         return q;
     }
     if (S == 1 && pieces <= 2048) {
@@ -942,17 +1161,19 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
             t.chunks = (int)std::max<int64_t>(1, std::max(few, many));
             t.rows = (S + t.chunks - 1) / t.chunks;
             t.chunks = (S + t.rows - 1) / t.rows;
-            q.part_floats = 2LL * N * t.chunks * groups;
+            q.part_floats = (backward ? 2LL : 4LL) * N * t.chunks * groups;
         }
+        q.far_floats = backward && dtype == ONTOVAE_F32 ? (int64_t)N * t.chunks * groups : 0;
         q.chan_rows = (int64_t)N * t.chunks;
         q.chan_floats = backward ? 2 * q.chan_rows * C : 0;
         return q;
     }
     q.form = OV_GN_ANY;
+    q.far_floats = backward ? (int64_t)N * groups : 0;
     return q;
 }
 
-static int64_t ov_gn_ws(const OvGnPlan& q) { return ((q.part_floats + 63) / 64 * 64 + q.chan_floats) * 4; }
+static int64_t ov_gn_ws(const OvGnPlan& q) { return (ov_gn_up(q.part_floats) + ov_gn_up(q.far_floats) + q.chan_floats) * 4; }
 
 extern "C" int64_t ontovae_group_norm_act_workspace_bytes(int32_t dtype, int32_t N, int32_t S, int32_t C, int32_t groups, int32_t backward) {
     if (N < 1 || S < 1 || C < 1 || std::max({N, S, C}) > OV_GN_MOST || groups < 1 || C % groups || dtype < ONTOVAE_F32 || dtype > ONTOVAE_F16) return 0;
@@ -1005,7 +1226,7 @@ static void ov_gn_fwd_go(const void* x, const OvGn& p, OvGnPlan q, void* y, floa
         const dim3 grid((unsigned)((int64_t)p.N * q.t.chunks * q.t.nblk));
         if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 2, LIGHT>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
         else {
-            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 0, LIGHT>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
+            hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 0, true>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
             hipLaunchKernelGGL((ov_gn_tile_fwd_kernel<T, 1, LIGHT>), grid, dim3(256), 0, st, xt, p, q.t, yt, mean, rstd);
         }
     }
@@ -1045,11 +1266,12 @@ static void ov_gn_bwd_go(const void* dy, const void* x, const OvGn& p, OvGnPlan 
     const T* dt = static_cast<const T*>(dy);
     T* dxt = static_cast<T*>(dx);
     q.t.part = static_cast<float*>(ws);
-    float* chan = dw || db ? static_cast<float*>(ws) + (q.part_floats + 63) / 64 * 64 : nullptr;
+    q.t.far = q.t.part + ov_gn_up(q.part_floats);
+    float* chan = dw || db ? q.t.far + ov_gn_up(q.far_floats) : nullptr;
     constexpr int NVX = 16 / OvGnPiece<T>::N;
     if (q.form == OV_GN_ANY) {
-        hipLaunchKernelGGL(ov_gn_any_dx_kernel<T>, dim3((unsigned)((int64_t)p.N * p.groups)), dim3(1024), 0, st, dt, xt, p, mean, rstd, dxt);
-        if (dw || db) hipLaunchKernelGGL(ov_gn_any_param_kernel<T>, dim3((p.C + 63) / 64), dim3(1024), 0, st, dt, xt, p, mean, rstd, dw, db);
+        hipLaunchKernelGGL(ov_gn_any_dx_kernel<T>, dim3((unsigned)((int64_t)p.N * p.groups)), dim3(1024), 0, st, dt, xt, p, mean, rstd, dxt, q.t.far);
+        if (dw || db) hipLaunchKernelGGL(ov_gn_any_param_kernel<T>, dim3((p.C + 63) / 64), dim3(1024), 0, st, dt, xt, p, mean, rstd, q.t.far, dw, db);
         return;
     }
     if (q.form == OV_GN_ROW) {
@@ -1060,6 +1282,7 @@ static void ov_gn_bwd_go(const void* dy, const void* x, const OvGn& p, OvGnPlan 
 #undef OV_GO
     } else {
         const dim3 grid((unsigned)((int64_t)p.N * q.t.chunks * q.t.nblk));
+        if constexpr (sizeof(T) == 4) hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 3, true>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
         if (q.form == OV_GN_TILE1) hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 2, LIGHT>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);
         else {
             hipLaunchKernelGGL((ov_gn_tile_bwd_kernel<T, 0, LIGHT>), grid, dim3(256), 0, st, dt, xt, p, q.t, mean, rstd, dxt, chan);

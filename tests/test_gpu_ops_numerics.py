@@ -6,7 +6,7 @@ import torch
 
 import ops_oracle as oo
 from onto_vae_amd import ops
-from test_gpu_ops import U, close, f64, rnd
+from test_gpu_ops import U, close, f64, last, rnd
 
 pytestmark = pytest.mark.gpu
 
@@ -25,3 +25,50 @@ def test_means_whose_square_passes_float32(N, S, C, G):
     dy = rnd(1, N, S, C)
     dx, _, _ = ops.group_norm_act_backward(dy, x, mean, rstd, G)
     assert torch.isfinite(dx).all()
+
+
+FAR = [(4, 1, 1000, 8), (3, 1, 8200, 1), (2, 1, 16384, 1), (2, 1, 20000, 1), (70, 1, 96, 3), (2, 64, 64, 4), (3, 5, 30, 3), (1, 300, 24, 24), (2, 4096, 64, 4),
+       (1, 30000, 8, 1), (1, 16385, 64, 4), (2, 3000, 320, 32), (2, 3, 5000, 2), (1, 40, 2500, 1)]
+
+
+@pytest.mark.parametrize("act", ["none", "silu"])
+@pytest.mark.parametrize("shift,dtype", [(1e3, torch.float32), (1e5, torch.float32), (100.0, torch.bfloat16), (100.0, torch.float16)])
+@pytest.mark.parametrize("N,S,C,G", FAR)
+def test_a_large_mean_costs_no_digits(N, S, C, G, shift, dtype, act):
+    """Spread 1 around 1e3 and 1e5, where a float32 mean is off by up to 3e-5 and 4e-3 of the spread.  Every group has another mean, some
+    groups are around 0, and a group's first value stands far from the rest.
+
+    x - mean - rest: the difference of neighbouring float32s is exact or off by u of itself, the rest is a mean of differences of
+    the spread's size, 94 additions on a path: 94 u (mean |xhat| <= 1).  The second moment has the same count, half of it in rstd:
+    err_x = 100 u (1 + |xhat|) leaves room for the products.  The backward pass of a 16-bit x may use the saved mean as it is, nearest to
+    the mean: u |mean| rstd more."""
+    rng = np.random.default_rng(N + S + C)
+    sh = np.repeat(shift * rng.uniform(0.5, 1.0, (N, 1, G)) * rng.choice([-1, 1, 1, 0], (N, 1, G)), C // G, 2)
+    x = torch.as_tensor(rng.standard_normal((N, S, C)) + sh)
+    x[:, 0, ::C // G] += 20.0
+    x = x.to(dtype).to("cuda:0")
+    dy, w, b = rnd(1, N, S, C, dtype=dtype), rnd(2, C, scale=0.2, shift=1.0), rnd(3, C)
+    y, mean, rstd = ops.group_norm_act(x, G, w, b, act=act)
+    o = oo.group_norm_act(f64(x), G, f64(w), f64(b), name=act, dy=f64(dy))
+    xh = np.abs(o["xhat"])
+    err = 100 * U * (1 + xh)
+    close(mean, o["mean"], U * np.abs(o["mean"]) + 100 * U / o["rstd"])
+    close(rstd, o["rstd"], 100 * U * o["rstd"])
+    tv = err * np.abs(o["w"]) + 6 * U * (xh * np.abs(o["w"]) + np.abs(f64(b)))
+    close(y, o["y"], 1.13 * tv + (np.abs(o["v"]) + 8) * U * np.abs(o["v"]) + last(dtype, o["y"]))
+    if dtype != torch.float32:
+        err = err + np.repeat(U * np.abs(o["mean"]) * o["rstd"], C // G, 1)[:, None]
+        tv = tv + np.repeat(U * np.abs(o["mean"]) * o["rstd"], C // G, 1)[:, None] * np.abs(o["w"])
+    dx, dw, db = ops.group_norm_act_backward(dy, x, mean, rstd, G, w, b, act=act)
+    shape = (N, S, G, C // G)
+    mean_g = lambda a: a.mean((1, 3), keepdims=True)
+    curv = 0.0 if act == "none" else 1.0
+    tdv = curv * tv * np.abs(f64(dy))
+    e, x4, t4, e4 = (np.abs(a).reshape(shape) for a in (o["dv"] * o["w"], xh, tdv * o["w"], err))
+    r = o["rstd"][:, None, :, None]
+    E = r * (e + mean_g(e) + x4 * mean_g(e * x4))
+    T = 400 * U * E + r * (t4 + mean_g(t4) + x4 * mean_g(t4 * x4 + e * e4) + e4 * mean_g(e * x4))
+    close(dx, o["dx"], T.reshape(N, S, C) + last(dtype, o["dx"]))
+    n = np.sqrt(N * S) + 200
+    close(dw, o["dweight"], n * U * o["dweight_abs"] + (tdv * xh + np.abs(o["dv"]) * err).sum((0, 1)))
+    close(db, o["dbias"], n * U * o["dbias_abs"] + tdv.sum((0, 1)))
