@@ -436,6 +436,20 @@ __global__ __launch_bounds__(LPG < 256 ? 256 : LPG) void ov_gn_row_bwd_kernel(co
     }
 }
 
+// A thread's sum of any number of terms in three levels of 64: a path of 64 + 64 + n / 4096 additions instead of n.
+struct OvGnLong {
+    float a = 0.f, b = 0.f, c = 0.f;
+    int n = 0;
+    __device__ __forceinline__ void add(float v) {
+        a += v;
+        if ((++n & 63) == 0) {
+            b += a;
+            a = 0.f;
+            if ((n & 4095) == 0) { c += b; b = 0.f; }
+        }
+    }
+    __device__ __forceinline__ float sum() const { return (a + b) + c; }
+};
 // column sums of part [2][R][C] in a fixed order: 16 channels x 64 rows at a time per workgroup, 8 loads in flight per thread
 __global__ __launch_bounds__(1024) void ov_gn_param_kernel(const float* __restrict__ part, int64_t R, int C, float* __restrict__ dw,
                                                            float* __restrict__ db) {
@@ -444,19 +458,18 @@ __global__ __launch_bounds__(1024) void ov_gn_param_kernel(const float* __restri
     if (!out) return;
     const float* src = part + (blockIdx.y ? R * C : 0);
     const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4, c = blockIdx.x * 16 + tx;
-    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    OvGnLong s;
     if (c < C) {
         int64_t r = ty;
         for (; r + 7 * 64 < R; r += 8 * 64) {
             float t[8];
 #pragma unroll
             for (int u = 0; u < 8; ++u) t[u] = src[(r + 64 * u) * C + c];
-#pragma unroll
-            for (int u = 0; u < 8; ++u) s[u & 3] += t[u];
+            s.add(((t[0] + t[4]) + (t[1] + t[5])) + ((t[2] + t[6]) + (t[3] + t[7])));
         }
-        for (; r < R; r += 64) s[0] += src[r * C + c];
+        for (; r < R; r += 64) s.add(src[r * C + c]);
     }
-    red[ty][tx] = (s[0] + s[1]) + (s[2] + s[3]);
+    red[ty][tx] = s.sum();
     __syncthreads();
     if (ty < 8) {
         float t = 0.f;
@@ -982,19 +995,17 @@ __global__ __launch_bounds__(1024) void ov_gn_any_fwd_kernel(const T* __restrict
     const int g = blockIdx.x % p.groups;
     const float cnt = (float)((int64_t)p.S * p.cg);
     const int64_t base = n * p.S * p.C + (int64_t)g * p.cg;
-    float s = 0.f;
+    OvGnLong s, s2, left;
     for (int r = 0; r < p.S; ++r)
-        for (int c = threadIdx.x; c < p.cg; c += 1024) s += ov_to_f<T>(x[base + (int64_t)r * p.C + c]);
-    const float mu = ov_block_sum(s, red) / cnt;
-    s = 0.f;
-    float left = 0.f;
+        for (int c = threadIdx.x; c < p.cg; c += 1024) s.add(ov_to_f<T>(x[base + (int64_t)r * p.C + c]));
+    const float mu = ov_block_sum(s.sum(), red) / cnt;
     for (int r = 0; r < p.S; ++r)
         for (int c = threadIdx.x; c < p.cg; c += 1024) {
             const float d = ov_to_f<T>(x[base + (int64_t)r * p.C + c]) - mu;
-            s += d * d;
-            left += d;
+            s2.add(d * d);
+            left.add(d);
         }
-    const float2 sl = ov_gn_sum2<1024>(s, left, red);
+    const float2 sl = ov_gn_sum2<1024>(s2.sum(), left.sum(), red);
     const float rest = sl.y / cnt, rs = 1.f / sqrtf(ov_gn_var(sl.x / cnt, rest) + p.eps);
     for (int r = 0; r < p.S; ++r)
         for (int c = threadIdx.x; c < p.cg; c += 1024) {
@@ -1029,21 +1040,22 @@ __global__ __launch_bounds__(1024) void ov_gn_any_dx_kernel(const T* __restrict_
     const float mu = mean[blockIdx.x], rs = rstd[blockIdx.x];
     float rest = 0.f;
     if (ov_gn_far(mu, rs)) {
+        OvGnLong left;
         for (int r = 0; r < p.S; ++r)
-            for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) rest += ov_to_f<T>(x[(n * p.S + r) * p.C + c]) - mu;
-        rest = ov_block_sum(rest, red) / cnt;
+            for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) left.add(ov_to_f<T>(x[(n * p.S + r) * p.C + c]) - mu);
+        rest = ov_block_sum(left.sum(), red) / cnt;
     }
     if (threadIdx.x == 0) rests[blockIdx.x] = rest;
-    float s1 = 0.f, s2 = 0.f, xh;
+    float xh;
+    OvGnLong l1, l2;
     for (int r = 0; r < p.S; ++r)
         for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) {
             const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rest, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
-            s1 += e;
-            s2 += e * xh;
+            l1.add(e);
+            l2.add(e * xh);
         }
-    const float2 sg = ov_gn_sum2<1024>(s1, s2, red);
-    s1 = sg.x / cnt;
-    s2 = sg.y / cnt;
+    const float2 sg = ov_gn_sum2<1024>(l1.sum(), l2.sum(), red);
+    const float s1 = sg.x / cnt, s2 = sg.y / cnt;
     for (int r = 0; r < p.S; ++r)
         for (int c = g * p.cg + threadIdx.x; c < (g + 1) * p.cg; c += 1024) {
             const float e = ov_gn_any_dv(p, x, dy, n * p.S + r, c, mu, rest, rs, &xh) * ov_gn_param(p.w, p.wtype, c, 1.f);
@@ -1058,15 +1070,16 @@ __global__ __launch_bounds__(1024) void ov_gn_any_param_kernel(const T* __restri
                                                                const float* __restrict__ rests, float* __restrict__ dw, float* __restrict__ db) {
     __shared__ float2 red[16][64];
     const int lane = ov_lane(), wave = ov_wave_id(), c = blockIdx.x * 64 + lane;
-    float2 s = {0.f, 0.f};
+    OvGnLong sw, sb;
     if (c < p.C)
         for (int64_t row = wave; row < (int64_t)p.N * p.S; row += 16) {
             const int64_t k = row / p.S * p.groups + c / p.cg;
             float xh;
             const float dv = ov_gn_any_dv(p, x, dy, row, c, mean[k], rests[k], rstd[k], &xh);
-            s.x += dv * xh;
-            s.y += dv;
+            sw.add(dv * xh);
+            sb.add(dv);
         }
+    float2 s = make_float2(sw.sum(), sb.sum());
     red[wave][lane] = s;
     __syncthreads();
     if (wave == 0 && c < p.C) {

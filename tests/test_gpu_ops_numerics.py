@@ -72,3 +72,47 @@ def test_a_large_mean_costs_no_digits(N, S, C, G, shift, dtype, act):
     n = np.sqrt(N * S) + 200
     close(dw, o["dweight"], n * U * o["dweight_abs"] + (tdv * xh + np.abs(o["dv"]) * err).sum((0, 1)))
     close(db, o["dbias"], n * U * o["dbias_abs"] + tdv.sum((0, 1)))
+
+
+@pytest.mark.parametrize("S,C,G", [(4096, 4096, 1), (2000, 5893, 1), (65536, 2050, 1), (1, 3000000, 1), (512, 9000, 3)])
+def test_long_sums_of_wide_groups(S, C, G):
+    """Groups too wide for the tiles, one workgroup each.  All squares about the mean are alike, and so are all terms of the gradients'
+    sums: in one chain of additions their roundings would all go the same way.  In three levels of 64 a path has at most
+    64 + 64 + n / 4096 / 1024 + 30 < 200 additions: 200 u of the sum of magnitudes, half of it in rstd."""
+    g = torch.Generator(device="cuda:0").manual_seed(S + C)
+    sign = torch.randint(0, 2, (1, S, C), generator=g, device="cuda:0", dtype=torch.int8).mul_(2).sub_(1)
+    x, dy = 0.3 * sign.float() + 0.7, 0.37 * sign.float() + 0.11
+    y, mean, rstd = ops.group_norm_act(x, G)
+    w = torch.ones(C, device="cuda:0")
+    dx, dw, db = ops.group_norm_act_backward(dy, x, mean, rstd, G, w, w)
+    for k in range(G):
+        sl = slice(k * C // G, (k + 1) * C // G)
+        xd, dd = x[..., sl].double(), dy[..., sl].double()
+        mu = xd.mean()
+        xd -= mu
+        r = float(1 / torch.sqrt((xd * xd).mean() + 1e-5))
+        assert abs(float(mean[0, k]) - float(mu)) <= U * abs(float(mu)) + 200 * U / r
+        assert abs(float(rstd[0, k]) - r) <= 105 * U * r
+        xd *= r
+        assert float(((y[..., sl].double() - xd).abs() - 210 * U * (1 + xd.abs())).max()) <= 0
+        p = dd * xd
+        for got, terms in ((dw[sl], p), (db[sl], dd)):
+            assert float(((got.double() - terms.sum((0, 1))).abs() - 320 * U * terms.abs().sum((0, 1))).max()) <= 0      # and xhat's 100 u
+        s1, s2 = dd.mean(), p.mean()
+        E = r * (dd.abs() + dd.abs().mean() + xd.abs() * p.abs().mean())
+        want = r * (dd - s1 - xd * s2)
+        assert float(((dx[..., sl].double() - want).abs() - 600 * U * E).max()) <= 0
+
+
+@pytest.mark.parametrize("N,S,C,G", [(1 << 22, 2, 8, 2), (1 << 20, 1, 8, 2)])
+def test_parameter_gradients_of_many_samples(N, S, C, G):
+    """Two-valued groups, so that all terms of a channel's sums are alike: 8 summands of one sample's or slot's rows, then the same 200 additions."""
+    pat = torch.tensor([1.0, -1.0], device="cuda:0").repeat(S * C // 2).view(1, S, C)
+    x, dy = (0.3 * pat).repeat(N, 1, 1), (0.37 * pat + 0.11).repeat(N, 1, 1)
+    w = torch.ones(C, device="cuda:0")
+    _, mean, rstd = ops.group_norm_act(x, G)
+    _, dw, db = ops.group_norm_act_backward(dy, x, mean, rstd, G, w, w)
+    r = 1 / np.sqrt(float(x[0, 0, 0].double() ** 2) + 1e-5)
+    d = dy[0].double()
+    close(dw, f64((d * x[0].double() * r).sum(0)) * N, 320 * U * f64((d * x[0].double() * r).abs().sum(0)) * N)
+    close(db, f64(d.sum(0)) * N, 208 * U * f64(d.abs().sum(0)) * N)
