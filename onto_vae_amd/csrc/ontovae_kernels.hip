@@ -328,6 +328,28 @@ extern "C" int64_t ontovae_bf16_workspace_bytes(const ontovae_dims_t* dims, int3
 // =================================================================================================
 // Encoder: BatchNorm (+ dropout + ReLU), feature-major, one wave per feature
 // =================================================================================================
+// the ranks' all-gathered (mean, M2, rows) blocks, S of them with that stride: Chan's combination; rest: what the rounding of the
+// global mean leaves (each rank combines for itself, all alike)
+__device__ __forceinline__ void ov_bn_ranks(const float* __restrict__ stats, int S, int64_t stride, int L, int l, float* mean, float* var, float* rest) {
+    float n = 0.f, m = 0.f;
+    for (int r = 0; r < S; ++r) {
+        const float nr = stats[r * stride + 2 * L];
+        n += nr;
+        m += nr * stats[r * stride + l];
+    }
+    m /= n;
+    float m2 = 0.f, left = 0.f;
+    for (int r = 0; r < S; ++r) {
+        const float nr = stats[r * stride + 2 * L];
+        const float dm = stats[r * stride + l] - m;
+        m2 += stats[r * stride + L + l] + nr * dm * dm;
+        left += nr * dm;
+    }
+    *mean = m;
+    *var = m2 / n;
+    *rest = left / n;
+}
+
 // h[l, b] = b0[l] + sum_s slab[s][l][b]                 (split-K combine of x W0^T, modules.py:46)
 // train: batch statistics (biased variance), running buffers updated (modules.py:47)
 // a = relu(dropout(gamma * xhat + beta))                (modules.py:47-49: BN, Dropout, ReLU)
@@ -350,7 +372,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_kernel(const float* __restrict_
     const int wave = ov_wave_id();
     float* xr = xhat + (int64_t)l * ldb;
     float* ar = a + (int64_t)l * ldb;
-    float mean, var;
+    float mean, var, rest = 0.f;
     if (mode != 3 && mode != 5) {
         const float bias = b0[l];
         float s = 0.f;
@@ -407,22 +429,8 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_kernel(const float* __restrict_
             var = q / (float)B;
         }
     } else if (mode == 5) {
-        // the ranks' all-gathered (mean, M2, rows) blocks, S of them with stride slab_stride: Chan's combination
         if (wave != 0) return;
-        float n = 0.f, m = 0.f;
-        for (int r = 0; r < S; ++r) {
-            const float nr = stats[r * slab_stride + 2 * L];
-            n += nr;
-            m += nr * stats[r * slab_stride + l];
-        }
-        mean = m / n;
-        float m2 = 0.f;
-        for (int r = 0; r < S; ++r) {
-            const float nr = stats[r * slab_stride + 2 * L];
-            const float dm = stats[r * slab_stride + l] - mean;
-            m2 += stats[r * slab_stride + L + l] + nr * dm * dm;
-        }
-        var = m2 / n;
+        ov_bn_ranks(stats, S, slab_stride, L, l, &mean, &var, &rest);
     } else {
         if (wave != 0) return;
         mean = stats[l];
@@ -447,7 +455,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_kernel(const float* __restrict_
     for (int b = lane; b < ldb; b += 64) {
         float xh = 0.f, y = 0.f;
         if (b < B) {
-            xh = (xr[b] - mean) * invstd;
+            xh = ((xr[b] - mean) - rest) * invstd;
             y = xh * g + be;
             if (dropping) y *= ov_dropout_scale(drop, seed, rng_off, OV_RNG_DROP, (uint64_t)l * 0x100000000ull + b);
             y = fmaxf(y, 0.f);
@@ -504,7 +512,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
         }
         mean = ov_wg_sum256(sum, red) / (float)B;
         // the rounding of the mean shifts every xhat of the row alike, and with them a whole row of dW0: what is left of the mean
-        // is summed in the same pass as the squares and taken off
+        // is summed in the same pass as the squares and taken off; a data-parallel rank sends the mean that is left of both
         float q = 0.f, left = 0.f;
         for (int b = tid * 4; b < ldb; b += 1024) {
             const f32x4 h4 = *reinterpret_cast<const f32x4*>(xr + b);       // this thread's own stores
@@ -518,26 +526,16 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
         q = ov_wg_sum256(q, red);
         rest = ov_wg_sum256(left, red) / (float)B;
         if (mode == 2) {
-            if (tid == 0) { stats[l] = mean; stats[L + l] = q; }
+            if (tid == 0) {
+                const float m2 = q - (float)B * rest * rest;
+                stats[l] = mean + rest;
+                stats[L + l] = m2 < 0.f ? 0.f : m2;
+            }
             return;
         }
         var = q / (float)B;
     } else if (mode == 5) {
-        // the ranks' all-gathered (mean, M2, rows) blocks, S of them with stride slab_stride: Chan's combination
-        float n = 0.f, m = 0.f;
-        for (int r = 0; r < S; ++r) {
-            const float nr = stats[r * slab_stride + 2 * L];
-            n += nr;
-            m += nr * stats[r * slab_stride + l];
-        }
-        mean = m / n;
-        float m2 = 0.f;
-        for (int r = 0; r < S; ++r) {
-            const float nr = stats[r * slab_stride + 2 * L];
-            const float dm = stats[r * slab_stride + l] - mean;
-            m2 += stats[r * slab_stride + L + l] + nr * dm * dm;
-        }
-        var = m2 / n;
+        ov_bn_ranks(stats, S, slab_stride, L, l, &mean, &var, &rest);
     } else {                       // mode 3
         mean = stats[l];
         var = stats[L + l];
