@@ -2,7 +2,9 @@
 
 Functions on device tensors like onto_vae_amd.stats: the arithmetic is in libontovae_hip.so (ontovae_quantize_rows,
 ontovae_int8_matmul, ontovae_group_norm_act, ontovae_dropout of include/ontovae_hip.h), torch allocates the buffers, there is no CPU
-path.  Forward and backward are explicit calls, no autograd graph is recorded.  Tensors are float32, bfloat16 or float16, channels
+path.  Forward and backward are explicit calls, no autograd graph is recorded (group_norm_act, dropout and int8_linear warn where an x that
+requires grad comes in with grad mode on: the graph ends there; inside a torch.autograd.Function, under torch.no_grad() or on
+x.detach() they do not).  Tensors are float32, bfloat16 or float16, channels
 last ([..., C]); every sum and statistic is held in 32 bits and each output is rounded once.  Work is queued on the
 current stream of the tensors' device, which need not be the current device.
 
@@ -11,6 +13,7 @@ The models use these operators through set_precision('int8') and VAE(norm='group
 """
 import contextlib
 import math
+import warnings
 
 import torch
 
@@ -28,6 +31,11 @@ _SAME = contextlib.nullcontext()
 def _gpu(t, what):
     if not t.is_cuda:
         _need_gpu(t, what)
+
+
+def _no_graph(x, what):
+    if x.requires_grad and torch.is_grad_enabled():
+        warnings.warn(f"{what} records no autograd graph: its result does not require grad though x does", stacklevel=3)
 
 
 def _on(device):
@@ -154,6 +162,7 @@ def int8_linear(x, weight, weight_scale, bias=None, rows=None, dtype=None):
     """x weight^T + bias with an 8-bit weight [N, K] (quantize_rows of the layer's float weight, done once) and the rows of x (of
     x[rows]) quantised on the way: one scale per token and per output channel.  dtype: that of y, x's by default."""
     _gpu(x, "int8_linear")
+    _no_graph(x, "int8_linear")
     dt = _dtype(x, "int8_linear")
     if dtype is None:
         dtype = x.dtype
@@ -210,6 +219,7 @@ def group_norm_act(x, groups, weight=None, bias=None, eps=1e-5, act="none", drop
     probability `drop` (masked as `dropout` masks y: same seed and offset, same mask).  mean, rstd: float32 [N, groups], for
     group_norm_act_backward."""
     dt, N, S, Cn, groups, weight, bias, wdt, a, drop, seed, offset = _gn_args(x, groups, weight, bias, act, drop, seed, offset, "group_norm_act")
+    _no_graph(x, "group_norm_act")
     if not float(eps) >= 0.0:
         raise ValueError(f"group_norm_act: eps = {eps}")
     x = x.contiguous()
@@ -256,6 +266,7 @@ def dropout(x, p, seed, offset=0, rows=None):
     by 1 - p.  The mask is a function of (seed, offset, row, channel) alone -- Philox4x32-10, 16 bits an element, so p is taken to
     the nearest 2^-16 -- and is never stored; use another offset for each draw.  A non-finite element in a dropped place gives 0."""
     _gpu(x, "dropout")
+    _no_graph(x, "dropout")
     dt = _dtype(x, "dropout")
     if not 0.0 <= float(p) <= 1.0:
         raise ValueError(f"dropout: p = {p} outside [0, 1]")
