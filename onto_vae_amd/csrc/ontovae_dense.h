@@ -226,6 +226,7 @@ static int64_t ov_vae_ext_carve(const OvVaeNet& n, const ontovae_vae_ext_t& e, i
         w.row = take(4LL * max_batch * n.fmax);
         w.drow = take(4LL * max_batch * n.fmax);
         w.dpar = take(8LL * n.fmax);
+        w.gn_bytes = 256;                            // batches of less than 8 elements, in the operator's general form
         auto per = [&](const OvVaeLayer& l) {
             w.h[l.bn_index] = take(4LL * max_batch * l.out);
             w.mean[l.bn_index] = take(4LL * max_batch * e.groups);

@@ -116,3 +116,10 @@ def test_parameter_gradients_of_many_samples(N, S, C, G):
     d = dy[0].double()
     close(dw, f64((d * x[0].double() * r).sum(0)) * N, 320 * U * f64((d * x[0].double() * r).abs().sum(0)) * N)
     close(db, f64(d.sum(0)) * N, 208 * U * f64(d.abs().sum(0)) * N)
+
+
+@pytest.mark.parametrize("B", [1, 2, 3])
+def test_a_model_of_few_units_takes_a_short_batch(B):
+    """A batch of less than 8 elements takes the general form, whose workspace a model sized for 128 rows has to hold as well."""
+    from test_gpu_dense_block import check_step
+    check_step(B, 0.0, 0.0, enc=(5,), dec=(4,), Z=3, groups=1)
