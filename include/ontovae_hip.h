@@ -75,7 +75,7 @@ typedef struct ontovae_dims {
 int ontovae_plan_create(int32_t K, const uint8_t* const* masks, const int32_t* rows,
                         const int32_t* cols, int32_t nu, ontovae_plan_t** out);
 /* Same plan from a link list (child, parent) in mask coordinates: layer[i], row[i], col[i] name a
- * one in mask layer[i].  This is the dense-free path for large ontologies (SURVEY.md 8(f)1). */
+ * one in mask layer[i].  This is the dense-free path for large ontologies. */
 int ontovae_plan_create_from_links(int32_t K, const int32_t* rows, const int32_t* cols, int32_t nu,
                                    int64_t n_links, const int32_t* layer, const int32_t* row,
                                    const int32_t* col, ontovae_plan_t** out);
@@ -240,7 +240,7 @@ typedef struct ontovae_ctx {
 #define ONTOVAE_FLAG_CB_GENE_FWD 128u   /* training forward of the gene layer on 32-column blocks (gathers from L2) instead of the LDS-panel kernel */
 #define ONTOVAE_FLAG_WIDE_GENE_TILES 8u /* gene layer: waves that span 64-256 batch columns instead of XCD-pinned 32-column blocks */
 /* Any other bit is refused with ONTOVAE_EINVAL (measurement switches exist only in -DOV_MEASUREMENT_SWITCHES builds). */
-/* BASELINE.json configs[4], "bf16 MFMA variant": the two large dense products of a pass -- x W0^T (onto_vae/modules.py:46) and its
+/* The bf16-MFMA variant: the two large dense products of a pass -- x W0^T (onto_vae/modules.py:46) and its
  * weight gradient dW0 = dh x -- take their inputs rounded to bf16 and accumulate in fp32 on v_mfma_f32_32x32x16_bf16; weights,
  * optimizer state and every other operation stay fp32.  Stated tolerance against the fp32 reference path (tests): loss 2e-2
  * relative per step, pathway activities cosine >= 0.999 per sample.  Needs ctx->bf16_ws, ctx->Gr (dW0 is staged there) and
@@ -257,7 +257,7 @@ typedef struct ontovae_ctx {
 #define ONTOVAE_FLAG_INT8_ENCODER 256u
 #define ONTOVAE_FLAG_NO_RIDERS     16u  /* weight gradient of the gene rows as its own launch instead of inside the backward chain's */
 #define ONTOVAE_FLAG_SIDE_STREAM    4u  /* run the decoder weight gradient and dWh on a library-owned second stream, forked from
-                                           and joined into the caller's stream with events (off by default: on this pool the event
+                                           and joined into the caller's stream with events (off by default: the event
                                            hand-offs cost about what the overlap gains) */
 
 int64_t ontovae_workspace_bytes(const ontovae_dims_t* dims, int32_t max_batch);
@@ -311,9 +311,10 @@ int ontovae_train_step(const ontovae_ctx_t* ctx, const float* x, const int32_t* 
 
 /* Data-parallel step in three phases around the caller's collectives (RCCL via torch.distributed);
  * the reference has no counterpart (single device), the contract is "equal to the single-device
- * step on the global batch" (SURVEY.md 8(e)):
- *   phase 0: encoder GEMM + local BN partial statistics -> bn_stats [2, L] {sum, sum of squares}
- *            caller: all-reduce SUM of bn_stats, passes global batch size in B_global
+ * step on the global batch":
+ *   phase 0: encoder GEMM + local BN partial statistics -> bn_stats [2, L] {mean, M2 = sum of squares about it}
+ *            caller: combines the ranks' into {mean, biased variance} (Chan), passes global batch size in B_global; or all-gathers
+ *            them for phase 16 + R below
  *   phase 1: BN normalise .. decoder .. backward down to BN -> bn_bwd_stats [2, L] {sum dy, sum dy*xhat}
  *            caller: all-reduce SUM of bn_bwd_stats
  *   phase 2: BN backward, dW0; all gradients land in ctx->Gr; loss_out holds LOCAL rec/kl sums.
@@ -325,7 +326,7 @@ int ontovae_train_step_dp(const ontovae_ctx_t* ctx, int32_t phase, const float* 
 
 /* Phase 3 of ontovae_train_step_dp is phase 2 without the dW0 product (BatchNorm backward only); ontovae_dw0_rows then
  * forms rows [l0, l1) of dW0 = dh x (the local rows' contribution) into ctx->Gr, so that the caller can all-reduce W0's
- * gradient in contiguous row panels, each panel's exchange under the next panel's product (SURVEY.md 8(e) bucket 3; row
+ * gradient in contiguous row panels, each panel's exchange under the next panel's product (row
  * panels instead of gene-column panels because rows are contiguous in the flat buffer).  No counterpart in the
  * reference (single device). */
 int ontovae_dw0_rows(const ontovae_ctx_t* ctx, const float* x, const int32_t* xidx, int32_t B, int32_t l0, int32_t l1,
@@ -445,7 +446,7 @@ int ontovae_dense_to_vals(const float* dense, int64_t ld, const int32_t* entry_r
                           const int32_t* entry_col, int64_t k0, int64_t k1, float* vals, void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * Statistics of a perturbation screen (SURVEY.md section 8(f) rank 3), all on device memory.
+ * Statistics of a perturbation screen, all on device memory.
  *
  * Ontobj.wilcox_test (onto_vae/ontobj.py:651-701) runs, per term or gene i,
  *   scipy.stats.wilcoxon(perturbed[:, i], control[:, i], zero_method='zsplit', alternative=...)  (:673)
@@ -486,7 +487,7 @@ int ontovae_to_feature_major(const float* src, int64_t src_ld, int32_t B, int32_
                              int64_t dst_ld, void* stream);
 
 /* ------------------------------------------------------------------------------------------
- * The plain VAE sibling (SURVEY.md 8(f) rank 4): reference class VAE (onto_vae/vae_model.py:913-1140) = Encoder
+ * The plain VAE sibling: reference class VAE (onto_vae/vae_model.py:913-1140) = Encoder
  * (onto_vae/modules.py:15-84, any number of [Linear, BatchNorm1d, Dropout, ReLU] blocks, then the mu / log_var heads with
  * Dropout(z_drop)) + dense Decoder (modules.py:94-154: the same blocks, then a Linear to the genes).  Same conventions as
  * above: one flat fp32 parameter buffer (ontovae_vae_layout gives the offsets, in floats), moments M / V and gradients Gr in

@@ -1,5 +1,4 @@
-// bf16-MFMA variant of the two large dense products of the OntoVAE step ("bf16 MFMA variant with
-// stated tolerance"): inputs rounded to bf16 (round to nearest even), products accumulated in fp32 on
+// bf16-MFMA variant of the two large dense products of the OntoVAE step: inputs rounded to bf16 (round to nearest even), products accumulated in fp32 on
 // v_mfma_f32_32x32x16_bf16, master weights, optimizer state and everything outside these two products in fp32.
 //
 //   encoder forward   h  [L, B] = W0 [L, G] . x^T        (reference onto_vae/modules.py:46)
@@ -166,7 +165,7 @@ __global__ __launch_bounds__(256) void ov_bf16_gemm_tn_kernel(const OvBfGemm p) 
 }
 
 // -------------------------------------------------------------------------------------------------
-// Second version of the product kernel (round 3): the same 128 x 128 tile, operand order and summation order as
+// Second form of the product kernel: the same 128 x 128 tile, operand order and summation order as
 // ov_bf16_gemm_tn_kernel (bit-identical sums), built like ov_gemm_lds2_kernel: two LDS stages and ONE barrier per 64-deep
 // K-step, the fragments of the next 16 k read while the current 4 MFMAs run (two register sets), global loads two steps ahead,
 // the next step's first fragments read across the barrier.  EPI 0: fp32 tile to slab z.  EPI 1 (dW0): the tile is the

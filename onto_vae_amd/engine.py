@@ -126,7 +126,7 @@ class Engine:
             raise ValueError(f"decoder layer {i}: expected shape {(cout, cin)}, got {tuple(dense.shape)}")
         dense = dense.contiguous()
         k0, k1 = self.plan.layer_entries[i]
-        if self.device.type != "cuda":      # a model can be constructed, loaded and saved without the GPU (INTEGRATION.md)
+        if self.device.type != "cuda":      # a model can be constructed, loaded and saved without the GPU
             er, ec = self._entry_rc()
             r, c = er[k0:k1].long(), ec[k0:k1].long()
             self.layer_vals(i, buf).copy_(dense[r, c])
@@ -274,7 +274,7 @@ class Engine:
         self._ctx = None
 
     def set_precision(self, mfma_dtype):
-        """'f32' (default: everything in float32, the reference's precision) or 'bf16' (BASELINE.json configs[4]: the two
+        """'f32' (default: everything in float32, the reference's precision) or 'bf16' (the two
         large dense products x W0^T and dW0 = dh x on bf16 MFMA with fp32 accumulation; weights and AdamW stay fp32) or 'int8'
         (inference passes take x W0^T in 8-bit integers, one scale per row of x and of W0; training passes stay float32)."""
         if mfma_dtype not in ("f32", "bf16", "int8"):

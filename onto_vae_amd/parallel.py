@@ -1,6 +1,5 @@
 """Data-parallel training: one process per GPU, torch.distributed (backend "nccl" = RCCL over
-xGMI) for the three exchanges a step needs.  The reference is single-device (SURVEY.md section 2
-row 12); the contract is that an R-rank step equals the single-device step on the global batch:
+xGMI) for the three exchanges a step needs.  The reference is single-device; the contract is that an R-rank step equals the single-device step on the global batch:
 
   * every rank sees the same global batch order and takes rows shard_bounds(B, R, r) of it;
   * SyncBN forward: all-gather of per-rank (mean, M2, n), combined with Chan's formula;
@@ -55,8 +54,8 @@ class _HostStaged:
     the same on every rank, as a communicator's order is): it waits for the issue-time event on a copy stream, copies the
     buffer into a pinned mirror, runs the collective on the mirror, copies the result back in place and records an event.
 
-    Why not hand gloo the device tensors: its own staging of them stalled with two processes on one GPU (DESIGN.md section 5
-    has what is known); and staging every collective synchronously, as round 2 did, never left a handle outstanding under
+    Why not hand gloo the device tensors: its own staging of them stalled with two processes on one GPU; and
+    staging every collective synchronously would never leave a handle outstanding under
     later launches, so ordering and buffer-reuse errors of the panel loop could not show before an 8-GPU run."""
 
     _inst = {}

@@ -1,7 +1,7 @@
 """Synthetic ontologies and expression data for tests and benchmarks.
 
-The generators follow SURVEY.md section 8(d) draw for draw, so the counts quoted
-there (4 595 term-term links, 159 732 gene-term links, 520 551 expanded
+The draws are in a fixed order, so the same counts
+(4 595 term-term links, 159 732 gene-term links, 520 551 expanded
 non-zeros for GOBP-syn) are reproduced on any machine from the numpy seed alone.
 
 The mask format is the reference's input contract
@@ -20,7 +20,7 @@ FULLGO_SYN_SEED = 20250118
 
 
 def synthetic_links(counts, n_genes, rng):
-    """Draw term->parent and gene->parent links (SURVEY.md 8(d) steps 2-3)."""
+    """Draw term->parent and gene->parent links."""
     counts = list(counts)
     K = len(counts)
     off = np.concatenate([[0], np.cumsum(counts)]).astype(np.int64)

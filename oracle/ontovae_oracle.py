@@ -7,7 +7,7 @@ is independent of torch.autograd.  It exists to check the HIP path
 __graft_entry__.smoke() and bench.py's cpu_baseline may import it; the product
 path never does (and fails loudly when the HIP library is missing).
 
-Parity pin: the reference ships no tests or golden vectors (SURVEY.md section 4), so
+Parity pin: the reference ships no tests or golden vectors, so
 this oracle is pinned by fixtures generated from the *imported reference itself*
 in the build container (tools/gen_golden.py -> tests/golden/*.npz, checked by
 tests/test_oracle_golden.py).
@@ -300,7 +300,7 @@ class OracleOntoVAE:
 
     def train_step(self, x, eps, lr, kl_coeff, scales=None):
         """One body of train_round (vae_model.py:156-176).  Returns (rec, kl, loss).  With self.phase_seconds a dict, the
-        wall time of the five phases BASELINE.md's CPU protocol names is added to it: forward (encoder, decoder, loss),
+        wall time of five phases is added to it: forward (encoder, decoder, loss),
         backward, grad_mask, adamw, clamp."""
         ph, t0 = self.phase_seconds, time.perf_counter()
         rec, kl, loss, g = self.gradients(x, eps, kl_coeff, scales)
