@@ -57,9 +57,9 @@ __device__ __forceinline__ float ov_drop_apply(const OvDrop& d, const OvPhilox& 
 }
 
 // One block of 8 elements per thread, 16 B a load whatever the alignment.  Its place in the matrix is one 64-bit division per
-// workgroup and a small one per thread.  Bound by memory: 16384 x 20000 bf16 in 327 us (4.0 TB/s where a copy runs at 4.9; with
-// the draws left out 321), 16384 x 10000 float32 in 243.  Two, four or eight blocks in flight per thread: 337, 340, 377 us (bf16), 277,
-// 286, 293 (float32); more waves hide the latency better than more loads.
+// workgroup and a small one per thread.  Bound by memory: 16384 x 20000 bf16 in 274 us (4.8 TB/s where a copy runs at
+// 4.9; the draws take 2 % of it), 16384 x 10000 float32 in 230.  Two, four or eight blocks in flight per thread are 3 to 15 % slower in
+// bf16 and 14 to 20 % in float32: more waves hide the latency better than more loads.
 template <typename T>
 __global__ __launch_bounds__(256) void ov_dropout_kernel(const T* __restrict__ x, int64_t ldx, const int32_t* __restrict__ rows, int n_src,
                                                          int R, int C, uint32_t nb, OvDrop d, T* __restrict__ y) {

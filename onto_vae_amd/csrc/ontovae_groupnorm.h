@@ -770,7 +770,7 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
 
 // chan: [2][N chunks][C]: the tiles' sums of dv xhat, then of dv, per channel.
 // Rests (ov_gn_far), of float32 x: MODE 3, in front of the others, takes the sums of x - mean of the tiles that hold such a group and ends at
-// once where there is none (2.5 us, 4 x 1024 x 320 27 -> 29.5).  A rest enters v through beta, the sums and dx after their loops: those are
+// once where there is none (2.5 us: 4 x 1024 x 320 27 -> 29.5; 53 where every group has one).  A rest enters v through beta, the sums and dx after their loops: those are
 // the same with and without it.  A 16-bit x goes without (64 x 16 x 320 in bf16 would be 18 -> 21 us): the rounding of its values, 2^-12 |x| at
 // least, has moved the mean of n of them by 2^-12 |mean| / sqrt(n), more than the 2^-24 |mean| in question up to n = 2^24.
 template <typename T, int MODE, bool LIGHT>
@@ -986,7 +986,9 @@ __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict
 }
 
 // ---------------------------------------------------------------- any shape: groups too wide for the forms above
-// one workgroup per (sample, group), everything re-read from the cache
+// (more than 2048 channels over several rows, more than 16384 in one), and tensors of less than 8 elements.  One workgroup per
+// (sample, group), everything re-read from the cache, however long the sample: 4 x 1024 x 4096 bf16 of one group 4.9 ms forward and 7.4
+// backward where 0.014 and 0.020 would be the memory's time.
 template <typename T>
 __global__ __launch_bounds__(1024) void ov_gn_any_fwd_kernel(const T* __restrict__ x, const OvGn p, T* __restrict__ y, float* __restrict__ mean,
                                                              float* __restrict__ rstd) {
@@ -1166,8 +1168,8 @@ static OvGnPlan ov_gn_plan(int dtype, int N, int S, int C, int groups, bool back
         if (bytes > 65536) {
             q.form = OV_GN_TILE;
             // up to 768 workgroups, three a CU as the backward kernels' registers allow, of 16 rows a thread or more (32 x 4096 x 512 bf16
-            // trained: 236 us; 1024: 247, 2048: 262); where the samples are few, 256 of 4 rows or more, at most 128 a
-            // sample (4 x 1024 x 320 float32 with gelu: 31 -> 19 us forward, 54 -> 27 backward; 60 x 3000 x 40 lost a fifth
+            // trained: 230 us; 5 % more with 1024, 11 % with 2048); where the samples are few, 256 of 4 rows or more, at most 128 a
+            // sample (4 x 1024 x 320 float32 with gelu: 31 -> 18 us forward, 54 -> 30 backward; 60 x 3000 x 40 lost a fifth
             // with 900 workgroups of 4 rows, 1 x 4096 x 512 a fifth with 256 a sample)
             const int64_t few = std::min<int64_t>((S + t.ty * 4 - 1) / (t.ty * 4), std::min<int64_t>((256 + wg - 1) / wg, 128));
             const int64_t many = std::min<int64_t>((S + t.ty * 16 - 1) / (t.ty * 16), (768 + wg - 1) / wg);

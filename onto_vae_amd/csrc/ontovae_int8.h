@@ -176,7 +176,8 @@ struct OvQ8Gemm {
 // index xor-ed with bits of the row (the source address is permuted, LDS is written in lane order): a wave's 16-B fragment
 // reads then spread over all 64 banks.  Rows beyond M / N repeat the last one, their results are dropped.  The last, partial step
 // of K is loaded with its bytes masked, so nothing is assumed of what stands behind column K.
-// !DIRECT: operands whose rows do not start on 16 B; the same loads through registers, unaligned.
+// !DIRECT: operands whose rows do not start on 16 B; the same loads through registers, unaligned, in tiles of 64 x 64 with the slabs of the
+// tile that aligned rows would get (8192 x 4096 x 4096 390 us where aligned rows take 146; few rows alike, 16 us).
 // T = int32_t: the raw sums to slab blockIdx.y.
 template <int BM, int BN, int WM, int WN, int BK, int ST, bool DIRECT, typename T>
 __global__ __launch_bounds__((BM / WM) * (BN / WN) * 64) void ov_q8_gemm_kernel(const OvQ8Gemm g) {
@@ -572,8 +573,8 @@ static const int ov_q8_bm[5] = {32, 64, 128, 128, 256}, ov_q8_bn[5] = {128, 64, 
 
 // The form with the least estimated time: rounds of 256 workgroups at the share of the matrix rate that each tile reaches
 // (measured over 128 <= M, N <= 16384, 2048 <= K <= 20000), plus what cutting K costs: the slabs written and read, and a launch.
-// 8192^3: 256 x 256 524 us, 128 x 128 685, 64 x 64 912; 16384 x 360 x 20000: 128 x 192 174 us, 256 x 256 200, 128 x 128 230;
-// 4096 x 360 x 20000: 128 x 192 in 4 slabs 54 us, 64 x 64 uncut 75; 2048^3: 128 x 128 17.6 us, 64 x 64 19.6, 128 x 192 42.
+// 8192^3: 256 x 256 518 us, 128 x 192 656, 128 x 128 684, 64 x 64 905; 16384 x 360 x 20000: 128 x 192 167 us, 256 x 256 in slabs 191,
+// 128 x 128 229; 4096 x 360 x 20000: 128 x 192 in 4 slabs 55 us, 64 x 64 uncut 76; 2048^3: 128 x 128 18.2 us, 128 x 192 19.0, 64 x 64 19.7.
 static OvQ8Plan ov_q8_plan(int64_t M, int64_t N, int K) {
     static const double share[5] = {0.15, 0.24, 0.32, 0.33, 0.45};
     const int steps = std::max((K + 127) / 128, 1);
@@ -694,7 +695,8 @@ extern "C" int ontovae_int8_matmul(const int8_t* a, int64_t lda, const float* sa
 
 // ---- linear layer with its input quantised on the way
 // The rows in 8 bits live in the workspace in blocks of 128 columns, [K / 128][M][128]: a step of a tile then reads one
-// contiguous run instead of one cache line from each of its rows (16384 x 20000 against 360 columns: 207 -> 183 us).
+// contiguous run instead of one cache line from each of its rows (16384 x 20000 against 360 columns: 12 % of the
+// product).
 static int64_t ov_q8_blocks(int K) { return std::max<int64_t>(((int64_t)K + 127) / 128, 1); }
 // few rows: the fused kernel.  Up to 4 rows and 8 pieces of 16 columns per thread (K <= 32768), 32 registers a row
 static bool ov_q8_few(int M, int K) { return M <= 4 && K <= 32768 && (M <= 2 || K <= 20480); }

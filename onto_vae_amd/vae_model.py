@@ -2,9 +2,9 @@
 
 Constructor, method names, arguments, return types, printed strings, error messages and the
 state_dict layout follow the reference; the arithmetic runs in libontovae_hip.so.
-Differences that a caller can observe are listed in INTEGRATION.md (no autograd graph on the
+Differences that a caller can observe: no autograd graph on the
 returned tensors; eps and dropout masks come from a Philox stream, not from torch's generator;
-losses are fetched once per epoch instead of once per step).
+losses are fetched once per epoch instead of once per step.
 """
 import numpy as np
 import torch
@@ -141,7 +141,7 @@ class OntoVAE(nn.Module):
         gradient) on bf16 MFMA with fp32 accumulation, parameters, optimizer and everything else float32 (stated tolerance
         against the float32 path: loss 2e-2 relative per step, activities cosine >= 0.999); 'int8': inference passes take
         x W0^T in 8-bit integers with one scale per sample and per hidden unit (onto_vae_amd.ops.int8_linear; activities
-        cosine >= 0.999), training passes stay float32."""
+        cosine >= 0.999; faster than 'bf16' from about a thousand samples a pass, not below), training passes stay float32."""
         self._engine.set_precision(mfma_dtype)
         return self
 
@@ -261,7 +261,7 @@ class OntoVAE(nn.Module):
     def train_model(self, modelpath, lr=1e-4, kl_coeff=1e-4, batch_size=128, epochs=300, run=None, resume=None):
         """vae_model.py:215-273: 80/20 split (seed 42), AdamW defaults, best-val checkpointing.
 
-        resume (not in the reference, SURVEY.md 8(f) rank 2): path of a checkpoint written by this method; training
+        resume (not in the reference): path of a checkpoint written by this method; training
         continues after the epoch it holds, with its parameters, optimizer state, batch order and random streams, so
         that the continued run equals the uninterrupted one (with dropout off or on)."""
         indices = np.random.RandomState(seed=42).permutation(self.X.shape[0])
@@ -348,7 +348,7 @@ class OntoVAE(nn.Module):
         nbuf = 3
         rows = min(step, N)
         # Staging into pinned memory is host work.  torch's copy_ converts float64 -> float32 on all its threads already
-        # (measured on the GPU box: 8.0 ms per 4096 x 20000 batch, 123 GB/s of host memory traffic, against 5.7 ms for the copy
+        # (measured: 8.0 ms per 4096 x 20000 batch, 123 GB/s of host memory traffic, against 5.7 ms for the copy
         # up: the conversion, not the bus, paces a float64 dataset at ~500 k samples/s); a same-dtype copy is ONE memcpy
         # thread (24 GB/s), so float32 sources are dealt to a few threads instead (copy_ releases the GIL).
         import concurrent.futures as _cf
