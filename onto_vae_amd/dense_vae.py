@@ -31,7 +31,7 @@ class DenseEngine:
         self.groups, self.input_drop, self.int8 = int(groups), float(input_drop), False
         if self.groups < 0 or any(w % self.groups for w in enc + dec if self.groups):
             raise ValueError(f"groups = {groups} must divide every width of layer_dims_enc / layer_dims_dec")
-        if not 0.0 <= self.input_drop < 1.0:
+        if not 0.0 <= C.c_float(self.input_drop).value < 1.0:          # as the library sees it
             raise ValueError(f"input_drop = {input_drop} outside [0, 1)")
         d = _lib.VaeDims()
         d.G, d.Z, d.n_enc, d.n_dec = int(in_features), int(latent_dim), len(enc), len(dec)

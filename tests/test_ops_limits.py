@@ -118,3 +118,12 @@ def test_int8_products_of_more_than_one_launch(M, N, K):
 
 def test_int8_linear_of_more_rows_than_its_quantizer_takes():
     refused(f"L.ontovae_int8_linear(P, 0, 8, NULL, {2 ** 26}, P, 8, P, NULL, {2 ** 26}, 1, 8, P, 0, 1, P, 1 << 62, NULL)", "int8_linear", "too many")
+
+
+@pytest.mark.parametrize("p", [1.0, 1 - 1e-9, -0.1, float("nan")])
+def test_input_drop_is_refused_where_the_library_would_refuse_it(p):
+    """1 - 1e-9 is 1 in float32: refused when the model is built, not in its first training step."""
+    import numpy as np
+    from onto_vae_amd.vae_model import VAE
+    with pytest.raises(ValueError, match="input_drop"):
+        VAE(np.zeros((2, 12)), [8], [8], 4, input_drop=p)
