@@ -535,9 +535,10 @@ __device__ __forceinline__ float ov_gn_lanes_sum(float v, int lg) {
     return v;
 }
 
-// Joins n parts of a group, part k = (mean, rest, M2) of cnt(k) values, by Chan's formula; lanes l of lg share them out.  The parts'
-// means are taken relative to the first one's, where nothing of the rests is lost.  (Relative to the first VALUE it would be: a value
-// that stands alone is sqrt(n) spreads away, the mean of a part that holds it no more than 45 for any tile.)
+// Joins n parts of a group, part k = (mean, rest, M2) of cnt(k) values, by Chan's formula; lanes l of lg share them out.  Means are
+// taken relative to the first part's, so that their differences are of the spread's size and the rests count.  (Not relative to a
+// single value: one that stands alone is up to sqrt(n) spreads away from the others, and the differences would be rounded at that size;
+// the mean of a part that holds it is at most 45 away in any tile.)
 template <typename P, typename CNT>
 __device__ __forceinline__ float3 ov_gn_join(int n, int l, int lg, float total, P&& part, CNT&& cnt) {
     const float3 first = part(0);
@@ -769,10 +770,11 @@ __global__ __launch_bounds__(256) void ov_gn_tile_fwd_kernel(const T* __restrict
 }
 
 // chan: [2][N chunks][C]: the tiles' sums of dv xhat, then of dv, per channel.
-// Rests (ov_gn_far), of float32 x: MODE 3, in front of the others, takes the sums of x - mean of the tiles that hold such a group and ends at
-// once where there is none (2.5 us: 4 x 1024 x 320 27 -> 29.5; 53 where every group has one).  A rest enters v through beta, the sums and dx after their loops: those are
-// the same with and without it.  A 16-bit x goes without (64 x 16 x 320 in bf16 would be 18 -> 21 us): the rounding of its values, 2^-12 |x| at
-// least, has moved the mean of n of them by 2^-12 |mean| / sqrt(n), more than the 2^-24 |mean| in question up to n = 2^24.
+// Rests (ov_gn_far) of a float32 x: MODE 3, in front of the others, takes the sums of x - mean of the tiles that hold such a group and
+// ends at once where there is none (2.5 us: 4 x 1024 x 320 27 -> 29.5; 53 where every group has one).  A rest enters v through
+// beta, the sums and dx after their loops: those are the same with and without it.  A 16-bit x goes without (64 x 16 x 320 in bf16
+// would be 18 -> 21 us): the rounding of its values, 2^-12 |x| at least, has moved the mean of n of them by 2^-12 |mean| / sqrt(n), more
+// than the 2^-24 |mean| in question up to n = 2^24.
 template <typename T, int MODE, bool LIGHT>
 __global__ __launch_bounds__(256) void ov_gn_tile_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, const OvGn p_, const OvGnTile t,
                                                              const float* __restrict__ mean, const float* __restrict__ rstd, T* __restrict__ dx,
