@@ -752,8 +752,9 @@ extern "C" int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, co
     }
     if (M == 0 || N == 0) return ONTOVAE_OK;
     if (!sw || !y || (K > 0 && (!x || !w))) { ontovae_set_error("int8_linear: NULL argument"); return ONTOVAE_EINVAL; }
-    // (the rows in 8 bits are laid out in the workspace for the direct form)
-    if (ov_q8_too_many(M, N, K, ov_q8_direct(nullptr, 128, w, ldw)) || !ov_q8_rows_fit(dtype, M, K)) {
+    // the few-row form has its own, small grid; for the others the rows in 8 bits are laid out in the workspace for the direct form
+    const bool few = ov_q8_few(M, K);
+    if (std::max(M, N) > OV_Q8_MAX_MN || (!few && (ov_q8_too_many(M, N, K, ov_q8_direct(nullptr, 128, w, ldw)) || !ov_q8_rows_fit(dtype, M, K)))) {
         ontovae_set_error("int8_linear: M = %d, N = %d, K = %d are too many for one launch", M, N, K);
         return ONTOVAE_EINVAL;
     }
@@ -762,7 +763,7 @@ extern "C" int ontovae_int8_linear(const void* x, int32_t dtype, int64_t ldx, co
         ontovae_set_error("int8_linear: workspace of %lld bytes, 256-B aligned, needed", (long long)need);
         return ONTOVAE_EINVAL;
     }
-    if (ov_q8_few(M, K)) {
+    if (few) {
         hipStream_t st = reinterpret_cast<hipStream_t>(stream);
         OvQ8Gemm g{nullptr, 0, 0, w, ldw, nullptr, sw, bias, M, N, K, 0, 0, 0, nullptr, y, ldy};
         if (dtype == ONTOVAE_F32) ov_q8_few_launch<float>(x, ldx, rows, n_src, M, g, ydtype, st);

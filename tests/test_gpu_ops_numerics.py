@@ -123,3 +123,18 @@ def test_a_model_of_few_units_takes_a_short_batch(B):
     """A batch of less than 8 elements takes the general form, whose workspace a model sized for 128 rows has to hold as well."""
     from test_gpu_dense_block import check_step
     check_step(B, 0.0, 0.0, enc=(5,), dec=(4,), Z=3, groups=1)
+
+
+def test_int8_linear_of_more_columns_than_tiles():
+    """One row against 2^30 + 64 weights of one column each: more 64 x 64 tiles than a launch takes, but the few-row form has none.  Its last
+    weights and results stand past 32-bit byte offsets."""
+    N = (1 << 30) + 64
+    x = torch.full((1, 1), 2.0, device="cuda:0")
+    w = torch.empty(N, 1, dtype=torch.int8, device="cuda:0")
+    w.view(-1).copy_(torch.arange(7, dtype=torch.int8, device="cuda:0").sub_(3).repeat(N // 7 + 1)[:N])
+    y = ops.int8_linear(x, w, torch.ones(N, device="cuda:0"))
+    s = float(ops.quantize_rows(x)[1])
+    step = 1 << 26
+    for k in list(range(0, N, step)):
+        got, want = y[0, k:k + step].double(), w[k:k + step, 0].double() * (127 * s)
+        assert float(((got - want).abs() - 3 * U * want.abs()).max()) <= 0
