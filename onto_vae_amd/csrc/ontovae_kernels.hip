@@ -328,6 +328,13 @@ extern "C" int64_t ontovae_bf16_workspace_bytes(const ontovae_dims_t* dims, int3
 // =================================================================================================
 // Encoder: BatchNorm (+ dropout + ReLU), feature-major, one wave per feature
 // =================================================================================================
+// a data-parallel rank's (mean, M2) of a feature: the mean with what its rounding left, the nearest float32 to the rows' mean
+__device__ __forceinline__ void ov_bn_send(float mean, float m2, float rest, int B, bool writes, float* __restrict__ stats, int L, int l) {
+    if (!writes) return;
+    m2 -= (float)B * rest * rest;
+    stats[l] = mean + rest;
+    stats[L + l] = m2 < 0.f ? 0.f : m2;                   // NaN stays
+}
 // the ranks' all-gathered (mean, M2, rows) blocks, S of them with that stride: Chan's combination; rest: what the rounding of the
 // global mean leaves (each rank combines for itself, all alike)
 __device__ __forceinline__ void ov_bn_ranks(const float* __restrict__ stats, int S, int64_t stride, int L, int l, float* mean, float* var, float* rest) {
@@ -413,17 +420,15 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_kernel(const float* __restrict_
             var = rvar[l];
         } else {
             mean = ov_wave_sum(s) / (float)B;
-            float q = 0.f;
+            float q = 0.f, left = 0.f;
             for (int b = lane; b < B; b += 64) {
                 const float dlt = xr[b] - mean;
                 q += dlt * dlt;
+                left += dlt;
             }
             q = ov_wave_sum(q);
             if (mode == 2) {
-                if (lane == 0) {
-                    stats[l] = mean;
-                    stats[L + l] = q;
-                }
+                ov_bn_send(mean, q, ov_wave_sum(left) / (float)B, B, lane == 0, stats, L, l);
                 return;
             }
             var = q / (float)B;
@@ -512,7 +517,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
         }
         mean = ov_wg_sum256(sum, red) / (float)B;
         // the rounding of the mean shifts every xhat of the row alike, and with them a whole row of dW0: what is left of the mean
-        // is summed in the same pass as the squares and taken off; a data-parallel rank sends the mean that is left of both
+        // is summed in the same pass as the squares and taken off
         float q = 0.f, left = 0.f;
         for (int b = tid * 4; b < ldb; b += 1024) {
             const f32x4 h4 = *reinterpret_cast<const f32x4*>(xr + b);       // this thread's own stores
@@ -526,11 +531,7 @@ __global__ __launch_bounds__(256) void ov_bn_fwd_wide_kernel(const float* __rest
         q = ov_wg_sum256(q, red);
         rest = ov_wg_sum256(left, red) / (float)B;
         if (mode == 2) {
-            if (tid == 0) {
-                const float m2 = q - (float)B * rest * rest;
-                stats[l] = mean + rest;
-                stats[L + l] = m2 < 0.f ? 0.f : m2;
-            }
+            ov_bn_send(mean, q, rest, B, tid == 0, stats, L, l);
             return;
         }
         var = q / (float)B;
